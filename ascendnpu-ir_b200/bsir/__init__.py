@@ -747,6 +747,233 @@ def matmul_w4a16(a: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, z
     return out
 
 
+# ---------------------------------------------------------------------------- microscaled 4-bit floats (MXFP4)
+def _on_device(*ts: Optional[torch.Tensor]) -> None:
+    """The operands must live on the current CUDA device, whose stream the call goes to."""
+    cur = torch.cuda.current_device()
+    for t in ts:
+        if t is not None and (not t.is_cuda or t.device.index != cur):
+            raise BsirError(-9, f"an operand is on {t.device}, the current device is cuda:{cur}")
+
+
+def _code_rows(rows: int, cols: int, device) -> torch.Tensor:
+    """uint8 [rows, cols] with 16-byte aligned rows, as the products want codes and exponents."""
+    return torch.empty((rows, (cols + 15) // 16 * 16), dtype=torch.uint8, device=device)[:, :cols]
+
+
+def _byte_rows(t: torch.Tensor, rows: int, cols: int, what: str) -> int:
+    """Row stride of a uint8 [rows, cols] tensor with contiguous rows."""
+    if t.dtype != torch.uint8:
+        raise BsirError(-4, f"{what}: expected uint8, got {t.dtype}")
+    if tuple(t.shape) != (rows, cols):
+        raise BsirError(-2, f"{what}: expected [{rows}, {cols}], got {list(t.shape)}")
+    if cols > 1 and t.stride(1) != 1:
+        raise BsirError(-3, f"{what}: innermost dimension must be unit-stride")
+    return t.stride(0) if rows > 1 else max(cols, 1)
+
+
+def _quant_mxfp4(x: torch.Tensor, along: bool, down: bool, outs: Sequence[Optional[torch.Tensor]]):
+    rows, cols, rs = _rows(x)
+    res, args = [], []
+    for want, r, c, q, s in ((along, rows, cols, outs[0], outs[1]), (down, cols, rows, outs[2], outs[3])):
+        if not want:
+            args += [C.c_void_p(0), C.c_int64(0), C.c_void_p(0), C.c_int64(0)]
+            continue
+        q = _code_rows(r, (c + 1) // 2, x.device) if q is None else q
+        s = _code_rows(r, (c + 31) // 32, x.device) if s is None else s
+        args += [_ptr(q), C.c_int64(_byte_rows(q, r, (c + 1) // 2, "quant_mxfp4: codes")),
+                 _ptr(s), C.c_int64(_byte_rows(s, r, (c + 31) // 32, "quant_mxfp4: exponents"))]
+        res += [q, s]
+    _on_device(x, *res)
+    _check(lib().bsir_quant_mxfp4(_dt(x), C.c_int64(rows), C.c_int64(cols), _ptr(x), C.c_int64(rs), *args, _stream()))
+    return tuple(res)
+
+
+def quant_mxfp4(x: torch.Tensor, axis: int = 1, q: Optional[torch.Tensor] = None, scale: Optional[torch.Tensor] = None):
+    """A [rows, cols] matrix (f32, f16, bf16) as microscaled 4-bit floats -> (codes, exponents), both uint8.
+
+    axis 1: blocks of 32 along the rows, codes [rows, ceil(cols / 2)], exponents [rows, ceil(cols / 32)].  axis 0: blocks
+    down the columns with the result transposed, codes [cols, ceil(rows / 2)], exponents [cols, ceil(rows / 32)] -- the
+    form in which a product that contracts the rows takes it.  Results made here have 16-byte aligned rows."""
+    if axis not in (0, 1, -1, -2):
+        raise BsirError(-5, f"quant_mxfp4: axis {axis} of a 2-D tensor")
+    if axis % 2:
+        return _quant_mxfp4(x, True, False, (q, scale, None, None))
+    return _quant_mxfp4(x, False, True, (None, None, q, scale))
+
+
+def quant_mxfp4_both(x: torch.Tensor, q: Optional[torch.Tensor] = None, scale: Optional[torch.Tensor] = None,
+                     qt: Optional[torch.Tensor] = None, scale_t: Optional[torch.Tensor] = None):
+    """Both forms of :func:`quant_mxfp4` from one read of x -> (codes, exponents, transposed codes, transposed exponents):
+    what the two products of a linear layer's backward pass take of the output's gradient."""
+    return _quant_mxfp4(x, True, True, (q, scale, qt, scale_t))
+
+
+def dequant_mxfp4(q: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype = torch.float32, cols: Optional[int] = None,
+                  out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Codes and exponents -> [rows, cols] values of ``dtype`` (f32, f16, bf16); cols defaults to two per byte of codes."""
+    if q.dim() != 2:
+        raise BsirError(-2, "dequant_mxfp4: expected 2-D codes")
+    rows = q.shape[0]
+    cols = 2 * q.shape[1] if cols is None else int(cols)
+    qs = _byte_rows(q, rows, (cols + 1) // 2, "dequant_mxfp4: codes")
+    ss = _byte_rows(scale, rows, (cols + 31) // 32, "dequant_mxfp4: exponents")
+    out = torch.empty((rows, cols), dtype=dtype, device=q.device) if out is None else out
+    orows, ocols, os_ = _rows(out)
+    if (orows, ocols) != (rows, cols):
+        raise BsirError(-2, f"dequant_mxfp4: out {list(out.shape)} for [{rows}, {cols}]")
+    _on_device(q, scale, out)
+    _check(lib().bsir_dequant_mxfp4(_dt(out), C.c_int64(rows), C.c_int64(cols), _ptr(q), C.c_int64(qs), _ptr(scale), C.c_int64(ss),
+                                    _ptr(out), C.c_int64(os_), _stream()))
+    return out
+
+
+class MatmulMxfp4Desc(C.Structure):
+    _fields_ = [("out_dtype", C.c_int32), ("bias_dtype", C.c_int32), ("m", C.c_int64), ("n", C.c_int64), ("k", C.c_int64),
+                ("a", C.c_void_p), ("lda", C.c_int64), ("scale_a", C.c_void_p), ("ldsa", C.c_int64),
+                ("b", C.c_void_p), ("ldb", C.c_int64), ("batch_stride_b", C.c_int64),
+                ("scale_b", C.c_void_p), ("ldsb", C.c_int64), ("batch_stride_sb", C.c_int64),
+                ("bias", C.c_void_p), ("bias_stride", C.c_int64), ("offsets", C.c_void_p), ("groups", C.c_int64),
+                ("out", C.c_void_p), ("ldo", C.c_int64)]
+
+
+def matmul_mxfp4(a: torch.Tensor, scale_a: torch.Tensor, b: torch.Tensor, scale_b: torch.Tensor, *,
+                 bias: Optional[torch.Tensor] = None, offsets: Optional[torch.Tensor] = None,
+                 out_dtype: Optional[torch.dtype] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``C = cast(A @ B^T + bias)`` of microscaled 4-bit matrices: codes a [m, k / 2] and b [n, k / 2] with their exponents
+    [.., ceil(k / 32)], f32 accumulation, C bf16 unless ``out_dtype`` (f32, f16, bf16) or ``out`` says otherwise.
+
+    With ``offsets`` (int32 [groups + 1] on the device) b, scale_b are [groups, n, ..] and rows offsets[g] .. offsets[g + 1]
+    of a meet matrix g (and bias [groups, n], or [n] for all): the experts' products.  Rows that no group holds keep
+    what ``out`` had in them.  Rows of codes and exponents start 16-byte aligned (:func:`quant_mxfp4` makes them so)."""
+    if a.dim() != 2 or b.dim() != (3 if offsets is not None else 2) or scale_b.dim() != b.dim():
+        raise BsirError(-2, "matmul_mxfp4: a [m, k / 2], b [n, k / 2] or, with offsets, [groups, n, k / 2]")
+    m, kb = a.shape
+    n, groups = b.shape[-2], b.shape[0] if offsets is not None else 1
+    ks = (2 * kb + 31) // 32
+    d = MatmulMxfp4Desc()
+    d.lda = _byte_rows(a, m, kb, "matmul_mxfp4: a")
+    d.ldsa = _byte_rows(scale_a, m, ks, "matmul_mxfp4: scale_a")
+    if b.shape[-1] != kb or tuple(scale_b.shape) != (*b.shape[:-1], ks):
+        raise BsirError(-2, f"matmul_mxfp4: b {list(b.shape)} and scale_b {list(scale_b.shape)} for {kb} bytes of codes and {ks} exponents a row")
+    b2, s2 = (b, scale_b) if offsets is None else (b[0], scale_b[0]) if groups else (b.reshape(0, kb), scale_b.reshape(0, ks))
+    d.ldb = _byte_rows(b2, n, kb, "matmul_mxfp4: b")
+    d.ldsb = _byte_rows(s2, n, ks, "matmul_mxfp4: scale_b")
+    if out is None:
+        out = torch.empty((m, n), dtype=out_dtype or torch.bfloat16, device=a.device)
+    elif out_dtype is not None and out.dtype != out_dtype:
+        raise BsirError(-4, f"matmul_mxfp4: out is {out.dtype}, out_dtype {out_dtype}")
+    orows, ocols, d.ldo = _rows(out)
+    if (orows, ocols) != (m, n):
+        raise BsirError(-2, f"matmul_mxfp4: out {list(out.shape)} for [{m}, {n}]")
+    if offsets is not None:
+        if offsets.dtype != torch.int32 or offsets.dim() != 1 or offsets.shape[0] != groups + 1 or not offsets.is_contiguous():
+            raise BsirError(-2, f"matmul_mxfp4: offsets must be contiguous int32 [{groups + 1}]")
+        d.offsets, d.groups = offsets.data_ptr(), groups
+        d.batch_stride_b, d.batch_stride_sb = b.stride(0), scale_b.stride(0)
+    if bias is not None:
+        if bias.shape[-1] != n or bias.dim() not in (1, 2) or (bias.dim() == 2 and (offsets is None or bias.shape[0] != groups)):
+            raise BsirError(-2, f"matmul_mxfp4: bias {list(bias.shape)} for {n} columns")
+        if n > 1 and bias.stride(-1) != 1:
+            raise BsirError(-3, "matmul_mxfp4: innermost dimension of bias must be unit-stride")
+        d.bias, d.bias_dtype, d.bias_stride = bias.data_ptr(), _dt(bias), (bias.stride(0) if bias.dim() == 2 else 0)
+    _on_device(a, scale_a, b, scale_b, out, bias, offsets)
+    d.out_dtype, d.m, d.n, d.k = _dt(out), m, n, 2 * kb
+    d.a, d.scale_a, d.b, d.scale_b, d.out = a.data_ptr(), scale_a.data_ptr(), b.data_ptr(), scale_b.data_ptr(), out.data_ptr()
+    _check(lib().bsir_matmul_mxfp4(C.byref(d), _stream()))
+    return out
+
+
+# ---------------------------------------------------------------------------- mixtures of experts
+def _choices(slots: torch.Tensor, what: str):
+    if slots.dim() != 2 or slots.dtype != torch.int32 or not slots.is_contiguous():
+        raise BsirError(-2, f"{what}: slots must be contiguous int32 [tokens, top_k]")
+    return slots.shape
+
+
+def _weights(w: Optional[torch.Tensor], slots: torch.Tensor, what: str):
+    if w is not None and (w.shape != slots.shape or not w.is_contiguous()):
+        raise BsirError(-2, f"{what}: weights must be contiguous {list(slots.shape)}")
+    return F32 if w is None else _dt(w)
+
+
+def expert_sort(ids: torch.Tensor, experts: int, offsets: Optional[torch.Tensor] = None, slots: Optional[torch.Tensor] = None):
+    """ids [tokens, top_k] (int32, int64; outside 0 .. experts - 1: no expert) -> (offsets int32 [experts + 1], slots int32
+    [tokens, top_k]): rows offsets[e] .. offsets[e + 1] belong to expert e, slots holds each choice's row or -1."""
+    if ids.dim() != 2 or not ids.is_contiguous():
+        raise BsirError(-2, "expert_sort: ids must be contiguous [tokens, top_k]")
+    tokens, top_k = ids.shape
+    offsets = torch.empty(experts + 1, dtype=torch.int32, device=ids.device) if offsets is None else offsets
+    slots = torch.empty((tokens, top_k), dtype=torch.int32, device=ids.device) if slots is None else slots
+    if offsets.dtype != torch.int32 or tuple(offsets.shape) != (experts + 1,) or not offsets.is_contiguous():
+        raise BsirError(-2, f"expert_sort: offsets must be contiguous int32 [{experts + 1}]")
+    if _choices(slots, "expert_sort") != ids.shape:
+        raise BsirError(-2, f"expert_sort: slots {list(slots.shape)} for ids {list(ids.shape)}")
+    _on_device(ids, offsets, slots)
+    _check(lib().bsir_expert_sort(_dt(ids), C.c_int64(tokens), C.c_int64(top_k), C.c_int64(experts), _ptr(ids), _ptr(offsets), _ptr(slots),
+                                  _stream()))
+    return offsets, slots
+
+
+def expert_dispatch(x: torch.Tensor, slots: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """out[slots[t, j]] = x[t] for a [tokens, cols] tensor of any element type; masked choices (-1) are skipped and rows of
+    out that no choice names keep their contents.  out defaults to tokens x top_k rows of zeros behind the last expert's."""
+    tokens, top_k = _choices(slots, "expert_dispatch")
+    rows, cols, rs = _rows(x)
+    if rows != tokens:
+        raise BsirError(-2, f"expert_dispatch: {rows} rows of x for {tokens} tokens")
+    out = torch.zeros((tokens * top_k, cols), dtype=x.dtype, device=x.device) if out is None else out
+    orows, ocols, os_ = _rows(out)
+    if ocols != cols or out.dtype != x.dtype:
+        raise BsirError(-2, f"expert_dispatch: out {list(out.shape)} {out.dtype} for {cols} columns of {x.dtype}")
+    _on_device(x, slots, out)
+    _check(lib().bsir_expert_dispatch(_dt(x), C.c_int64(tokens), C.c_int64(top_k), C.c_int64(cols), _ptr(x), C.c_int64(rs), _ptr(slots),
+                                      C.c_int64(orows), _ptr(out), C.c_int64(os_), _stream()))
+    return out
+
+
+def expert_combine(y: torch.Tensor, slots: torch.Tensor, weights: Optional[torch.Tensor] = None,
+                   out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """out[t] = sum_j weights[t, j] * y[slots[t, j]] over the choices that are not masked, f32 sums rounded once.  Without
+    weights (all 1) it is the gradient of :func:`expert_dispatch`."""
+    tokens, top_k = _choices(slots, "expert_combine")
+    rows, cols, ys = _rows(y)
+    wdt = _weights(weights, slots, "expert_combine")
+    out = torch.empty((tokens, cols), dtype=y.dtype, device=y.device) if out is None else out
+    orows, ocols, os_ = _rows(out)
+    if (orows, ocols) != (tokens, cols) or out.dtype != y.dtype:
+        raise BsirError(-2, f"expert_combine: out {list(out.shape)} {out.dtype} for [{tokens}, {cols}] of {y.dtype}")
+    _on_device(y, slots, weights, out)
+    _check(lib().bsir_expert_combine(_dt(y), C.c_int64(tokens), C.c_int64(top_k), C.c_int64(cols), C.c_int64(rows), _ptr(y), C.c_int64(ys),
+                                     _ptr(slots), wdt, _ptr(weights), _ptr(out), C.c_int64(os_), _stream()))
+    return out
+
+
+def expert_combine_grad(dout: torch.Tensor, y: torch.Tensor, slots: torch.Tensor, weights: Optional[torch.Tensor] = None,
+                        out: Optional[torch.Tensor] = None, dweights: Optional[torch.Tensor] = None):
+    """The gradient of :func:`expert_combine` -> (dy, dweights): dy[slots[t, j]] = weights[t, j] * dout[t] (``out``; rows
+    that no choice names keep their contents, zeros when it is made here), dweights[t, j] = <dout[t], y[slots[t, j]]> in
+    f32, 0 for a masked choice."""
+    tokens, top_k = _choices(slots, "expert_combine_grad")
+    rows, cols, ys = _rows(y)
+    drows, dcols, ds = _rows(dout)
+    if (drows, dcols) != (tokens, cols) or dout.dtype != y.dtype:
+        raise BsirError(-2, f"expert_combine_grad: dout {list(dout.shape)} {dout.dtype} for [{tokens}, {cols}] of {y.dtype}")
+    wdt = _weights(weights, slots, "expert_combine_grad")
+    dy = torch.zeros((rows, cols), dtype=y.dtype, device=y.device) if out is None else out
+    dw = torch.empty((tokens, top_k), dtype=torch.float32, device=y.device) if dweights is None else dweights
+    yrows, ycols, dys = _rows(dy)
+    if (yrows, ycols) != (rows, cols) or dy.dtype != y.dtype:
+        raise BsirError(-2, f"expert_combine_grad: out {list(dy.shape)} {dy.dtype} for [{rows}, {cols}] of {y.dtype}")
+    if dw.dtype != torch.float32 or dw.shape != slots.shape or not dw.is_contiguous():
+        raise BsirError(-2, f"expert_combine_grad: dweights must be contiguous f32 {list(slots.shape)}")
+    _on_device(dout, y, slots, weights, dy, dw)
+    _check(lib().bsir_expert_combine_grad(_dt(y), C.c_int64(tokens), C.c_int64(top_k), C.c_int64(cols), C.c_int64(rows), _ptr(dout),
+                                          C.c_int64(ds), _ptr(y), C.c_int64(ys), _ptr(slots), wdt, _ptr(weights), _ptr(dy), C.c_int64(dys),
+                                          _ptr(dw), _stream()))
+    return dy, dw
+
+
 # ---------------------------------------------------------------------------- compiled-kernel ABI
 def register_kernel(name: str, kind: str, *, fn: int = 0, dtype: int = F32, dst_dtype: int = F32,
                     round_mode: str = "rint", overflow_mode: str = "wrap", flags: int = 0,

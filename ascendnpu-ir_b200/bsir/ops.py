@@ -1,7 +1,8 @@
 """Operator surface under the reference's op names (layer B3): torch CUDA tensors in, attribute keywords spelled as
 in the reference IR.  Every function here is the library call of the same name in the package root."""
-from . import (cast, compare, copy, default_round_mode, elemwise_binary, elemwise_unary, load, matmul_w4a16, matmul_w8a8,
-               quant_per_token_i8, reduce, reduce_with_index, rms_norm, select, softmax, store, vadd, vdiv, vmul, vsub)
+from . import (cast, compare, copy, default_round_mode, dequant_mxfp4, elemwise_binary, elemwise_unary, expert_combine,
+               expert_combine_grad, expert_dispatch, expert_sort, load, matmul_mxfp4, matmul_w4a16, matmul_w8a8, quant_mxfp4,
+               quant_mxfp4_both, quant_per_token_i8, reduce, reduce_with_index, rms_norm, select, softmax, store, vadd, vdiv, vmul, vsub)
 
 # hfusion.* / linalg.* / hivm.hir.* spellings
 hfusion_cast = cast

@@ -1,0 +1,463 @@
+// mxfp4_gemm.cu -- products of microscaled 4-bit matrices (MXFP4, see mxfp4_quant.cu) on the tensor core:
+//   C[i, j] = cast_rint( sum_k A[i, k] * B[j, k] + bias[j] ),   A[i, k] = code * 2^(exponent byte of (i, k / 32) - 127)
+// for one B, or row groups of A against a B of their own (the experts' products of a mixture-of-experts layer: rows
+// offsets[e] .. offsets[e + 1] of A meet B[e]; other rows of C are left as they were).
+//
+// tcgen05.mma kind::mxf4.block_scale multiplies 64 elements of K an instruction and applies both exponents on the way
+// into the f32 accumulator, four times the rate of a 16-bit product.  Codes come by TMA into 128-byte-swizzled tiles
+// (a 128-byte row is 256 elements of K); the exponents have to lie in tensor memory: row r of an operand tile at lane
+// r % 32, column r / 32, four bytes (128 elements of K) a cell, the same in all four lane quadrants.  The exponent
+// matrices keep the plain [rows, K / 32] layout, so groups may start at any row: TMA brings [rows x 16 bytes] (512
+// elements of K), and four warps, one a quadrant, move them shared memory -> registers -> tensor memory.
+//
+// A persistent kernel, one CTA per SM, 320 threads:
+//   warp 0      TMA producer of codes (a ring of stages of 256 elements of K) and exponents (a ring of 512)
+//   warp 1      MMA issuer
+//   warps 2-5   epilogue: accumulator -> bias -> rounding -> C
+//   warps 6-9   exponents into tensor memory, two buffers
+// Few rows run with the operands swapped: 128 rows of B are the instruction's M side and BN rows of A its N side, so
+// that a tile of weights is streamed for as few as 16 rows of A.
+#include <mutex>
+
+#include "tc_ptx.cuh"
+
+namespace bsir {
+namespace {
+
+constexpr int kTileM = 128;
+constexpr int kStageK = 256;       // elements of K a stage: one 128-byte swizzle row of codes
+constexpr int kChunkK = 512;       // elements of K of a 16-byte piece of exponents
+constexpr int kThreads = 320;
+constexpr int kMaxGroups = 1024;
+
+struct MxParams {
+  int64_t m, n;
+  int k_blocks;                    // stages of a tile
+  const int32_t *offsets;          // [groups + 1] or null: one group of all rows
+  int groups;
+  const void *bias;
+  int64_t bias_stride;             // elements between the groups' biases
+  int32_t bias_dtype, out_dtype;
+  void *out;
+  int64_t ldo;
+  int *err;
+};
+
+template <int BN>
+struct MxCfg {
+  static constexpr int kStage = (kTileM + BN) * 128;
+  static constexpr int kStages = BN >= 256 ? 4 : BN >= 128 ? 6 : BN >= 64 ? 7 : 9;
+  static constexpr int kSfStage = (kTileM + BN) * 16;
+  static constexpr int kSfStages = 4;
+  static constexpr int kAccs = BN >= 256 ? 1 : 2;
+  // columns of tensor memory: accumulators, then two buffers of 4 x (4 + kSfN) cells of exponents
+  static constexpr int kSfN = BN >= 128 ? BN / 32 : 4;
+  static constexpr int kSfCols = 4 * (4 + kSfN);
+  static constexpr int kSfBase = kAccs * BN;
+  static constexpr int kCols = kSfBase + 2 * kSfCols;
+  static constexpr int kTmemCols = kCols <= 128 ? 128 : kCols <= 256 ? 256 : 512;
+  static constexpr int kSfOff = kStages * kStage;
+  static constexpr int kBarOff = kSfOff + kSfStages * kSfStage;
+  static constexpr int kTableOff = kBarOff + 512;                    // tiles before a group; first row and end of each
+  static constexpr int kSmem = kTableOff + (3 * kMaxGroups + 1) * 4 + 1024 /*alignment*/;
+  static_assert(kCols <= 512, "tensor memory");
+  static_assert(kSmem <= 227 * 1024, "shared memory");
+};
+
+__device__ __forceinline__ void mma_mxf4(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(tmem_d),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+      : "memory");
+}
+// e2m1 x e2m1, exponents E8M0, both K-major; `sf_id` (0 or 2): which two of a cell's four bytes belong to these 64
+// elements of K
+__device__ __forceinline__ uint32_t mx_idesc(int n, int m, uint32_t sf_id) {
+  return (sf_id << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n >> 3) << 17) | (1u << 23) | (static_cast<uint32_t>(m >> 7) << 27) | (sf_id << 29);
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t *r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+      "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
+__device__ __forceinline__ float load_float(const void *p, int32_t dtype, int64_t i) {
+  if (dtype == BSIR_F32) return static_cast<const float *>(p)[i];
+  const unsigned short h = static_cast<const unsigned short *>(p)[i];
+  return dtype == BSIR_F16 ? __half2float(__ushort_as_half(h)) : __uint_as_float(static_cast<uint32_t>(h) << 16);
+}
+__device__ __forceinline__ void store_out(const MxParams &p, int64_t at, float f) {
+  if (p.out_dtype == BSIR_F32) static_cast<float *>(p.out)[at] = f;
+  else if (p.out_dtype == BSIR_F16) static_cast<__half *>(p.out)[at] = __float2half_rn(f);
+  else static_cast<__nv_bfloat16 *>(p.out)[at] = __float2bfloat16_rn(f);
+}
+
+// Where a tile lies: `tile_start[g]` tiles come before group g; within a group the row tiles run fastest, so that
+// CTAs working at the same time share columns of B.
+struct MxTile {
+  int group, row0, row_end, n0;
+};
+template <int ROWS, int COLS>
+__device__ __forceinline__ void find_tile(int tile, const int *tile_start, const int *row_start, int &group, MxTile &t) {
+  while (tile >= tile_start[group + 1]) ++group;            // a role's tiles only go up
+  const int first = row_start[2 * group], end = row_start[2 * group + 1];
+  const int row_tiles = (end - first + ROWS - 1) / ROWS;
+  const int local = tile - tile_start[group];
+  t.group = group;
+  t.row0 = first + (local % row_tiles) * ROWS;
+  t.row_end = end;
+  t.n0 = (local / row_tiles) * COLS;
+}
+
+template <int BN, bool SWAP>
+__global__ void __launch_bounds__(kThreads, 1)
+    mxfp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_m, const __grid_constant__ CUtensorMap tmap_n,
+                      const __grid_constant__ CUtensorMap tmap_sm, const __grid_constant__ CUtensorMap tmap_sn, MxParams p) {
+  using Cfg = MxCfg<BN>;
+  constexpr int kRows = SWAP ? BN : kTileM;       // rows of A and columns of C (rows of B) a tile
+  constexpr int kColsC = SWAP ? kTileM : BN;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  uint8_t *gen = smem_raw + (base - raw);
+  const uint32_t bars = base + Cfg::kBarOff;
+  auto full_bar = [&](int s) { return bars + 8u * s; };
+  auto empty_bar = [&](int s) { return bars + 8u * (Cfg::kStages + s); };
+  auto sf_full_bar = [&](int s) { return bars + 8u * (2 * Cfg::kStages + s); };
+  auto sf_empty_bar = [&](int s) { return bars + 8u * (2 * Cfg::kStages + Cfg::kSfStages + s); };
+  constexpr int kB2 = 2 * Cfg::kStages + 2 * Cfg::kSfStages;
+  auto st_full_bar = [&](int b) { return bars + 8u * (kB2 + b); };        // exponents in tensor memory
+  auto st_empty_bar = [&](int b) { return bars + 8u * (kB2 + 2 + b); };
+  auto acc_full_bar = [&](int b) { return bars + 8u * (kB2 + 4 + b); };
+  auto acc_empty_bar = [&](int b) { return bars + 8u * (kB2 + 6 + b); };
+  static_assert(8 * (kB2 + 8) + 16 <= 512, "barriers");
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(gen + Cfg::kBarOff + 8 * (kB2 + 8));
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+  int *tile_start = reinterpret_cast<int *>(gen + Cfg::kTableOff);         // [groups + 1]
+  int *row_start = tile_start + kMaxGroups + 1;                            // [groups][2]: first row, end
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  pdl_launch_dependents();
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < Cfg::kStages; ++s) { mbar_init(full_bar(s), 1); mbar_init(empty_bar(s), 1); }
+    for (int s = 0; s < Cfg::kSfStages; ++s) { mbar_init(sf_full_bar(s), 1); mbar_init(sf_empty_bar(s), 4); }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(st_full_bar(b), 4); mbar_init(st_empty_bar(b), 1);
+      mbar_init(acc_full_bar(b), 1); mbar_init(acc_empty_bar(b), 4);
+    }
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    prefetch_tmap(&tmap_m); prefetch_tmap(&tmap_n); prefetch_tmap(&tmap_sm); prefetch_tmap(&tmap_sn);
+  }
+  if (warp == 1) tmem_alloc(smem_u32(tmem_slot), Cfg::kTmemCols);
+  pdl_wait();                       // no global memory is touched before this
+  if (warp == 2) {                  // the groups' rows (clamped to what exists) and tiles
+    const int col_tiles = static_cast<int>((p.n + kColsC - 1) / kColsC);
+    int before = 0, reached = 0;
+    for (int g0 = 0; g0 < p.groups; g0 += 32) {
+      const int g = g0 + lane;
+      // rows start where the largest offset so far says: groups never overlap, whatever the offsets hold
+      int64_t first = 0, end = p.m;
+      if (p.offsets) {
+        int64_t o = p.offsets[g < p.groups ? g : p.groups];
+        o = o < 0 ? 0 : o > p.m ? p.m : o;
+        int top = static_cast<int>(o);
+#pragma unroll
+        for (int s = 1; s < 32; s <<= 1) {
+          const int up = __shfl_up_sync(0xffffffffu, top, s);
+          if (lane >= s) top = max(top, up);
+        }
+        top = max(top, reached);
+        first = top;
+        int next = p.offsets[g + 1 < p.groups ? g + 1 : p.groups];
+        next = next < 0 ? 0 : next > p.m ? static_cast<int>(p.m) : next;
+        end = max(top, next);
+        reached = __shfl_sync(0xffffffffu, top, 31);
+      }
+      int tiles = 0;
+      if (g < p.groups) {
+        row_start[2 * g] = static_cast<int>(first);
+        row_start[2 * g + 1] = static_cast<int>(end);
+        tiles = static_cast<int>((end - first + kRows - 1) / kRows) * col_tiles;
+      }
+      int inc = tiles;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += up;
+      }
+      if (g < p.groups) tile_start[g + 1] = before + inc;
+      before += __shfl_sync(0xffffffffu, inc, 31);
+    }
+    if (lane == 0) tile_start[0] = 0;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const int total_tiles = tile_start[p.groups];
+  const int chunks = (p.k_blocks + 1) / 2;
+  int group = 0;
+  MxTile t;
+
+  if (warp == 0) {
+    // ---------------- TMA producer
+    if (lane == 0) {
+      int stage = 0, sf = 0;
+      uint32_t phase = 0, sf_phase = 0;
+      bool ok = true;
+      for (int tile = blockIdx.x; tile < total_tiles && ok; tile += gridDim.x) {
+        find_tile<kRows, kColsC>(tile, tile_start, row_start, group, t);
+        const int m0 = SWAP ? t.n0 : t.row0, n0 = SWAP ? t.row0 : t.n0;
+        const int zm = SWAP ? t.group : 0, zn = SWAP ? 0 : t.group;
+        for (int kb = 0; kb < p.k_blocks; ++kb) {
+          if ((kb & 1) == 0) {
+            if (!mbar_wait(sf_empty_bar(sf), sf_phase ^ 1u, abort_flag, p.err)) { ok = false; break; }
+            const uint32_t dst = base + Cfg::kSfOff + sf * Cfg::kSfStage;
+            mbar_expect_tx(sf_full_bar(sf), Cfg::kSfStage);
+            tma_load_3d(dst, &tmap_sm, kb * (kStageK / 32), m0, zm, sf_full_bar(sf));
+            tma_load_3d(dst + kTileM * 16, &tmap_sn, kb * (kStageK / 32), n0, zn, sf_full_bar(sf));
+            if (++sf == Cfg::kSfStages) { sf = 0; sf_phase ^= 1u; }
+          }
+          if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag, p.err)) { ok = false; break; }
+          const uint32_t dst = base + stage * Cfg::kStage;
+          mbar_expect_tx(full_bar(stage), Cfg::kStage);
+          tma_load_3d(dst, &tmap_m, kb * 128, m0, zm, full_bar(stage));
+          tma_load_3d(dst + kTileM * 128, &tmap_n, kb * 128, n0, zn, full_bar(stage));
+          if (++stage == Cfg::kStages) { stage = 0; phase ^= 1u; }
+        }
+      }
+      if (!ok) {      // gave up: let the copies in flight land before the CTA leaves
+        for (int s = 0; s < Cfg::kStages; ++s)
+          for (int i = 0; i < 200000; ++i)
+            if (mbar_try_wait(full_bar(s), 0) || mbar_try_wait(full_bar(s), 1)) break;
+        for (int s = 0; s < Cfg::kSfStages; ++s)
+          for (int i = 0; i < 200000; ++i)
+            if (mbar_try_wait(sf_full_bar(s), 0) || mbar_try_wait(sf_full_bar(s), 1)) break;
+      }
+    }
+  } else if (warp == 1) {
+    // ---------------- MMA issuer
+    if (lane == 0) {
+      const uint32_t idesc0 = mx_idesc(BN, kTileM, 0), idesc2 = mx_idesc(BN, kTileM, 2);
+      int stage = 0, b = 0, acc = 0;
+      uint32_t phase = 0, b_phase = 0, acc_phase = 0;
+      bool ok = true;
+      for (int tile = blockIdx.x; tile < total_tiles && ok; tile += gridDim.x) {
+        if (!mbar_wait(acc_empty_bar(acc), acc_phase ^ 1u, abort_flag, p.err)) break;
+        tc_fence_after();
+        const uint32_t d = tmem + static_cast<uint32_t>(acc * BN);
+        for (int c = 0; c < chunks && ok; ++c) {
+          if (!mbar_wait(st_full_bar(b), b_phase, abort_flag, p.err)) { ok = false; break; }
+          const uint32_t sf = tmem + static_cast<uint32_t>(Cfg::kSfBase + b * Cfg::kSfCols);
+          for (int h = 0; h < 2 && 2 * c + h < p.k_blocks; ++h) {
+            if (!mbar_wait(full_bar(stage), phase, abort_flag, p.err)) { ok = false; break; }
+            tc_fence_after();
+            const uint32_t sm = base + stage * Cfg::kStage, sn = sm + kTileM * 128;
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk) {
+              const uint32_t cell = static_cast<uint32_t>(2 * h + (kk >> 1));
+              mma_mxf4(d, make_desc(sm + kk * 32, 16, 1024), make_desc(sn + kk * 32, 16, 1024), (kk & 1) ? idesc2 : idesc0, sf + cell * 4,
+                       sf + 16 + cell * Cfg::kSfN, (c | h | kk) ? 1u : 0u);
+            }
+            tc_commit(empty_bar(stage));
+            if (++stage == Cfg::kStages) { stage = 0; phase ^= 1u; }
+          }
+          if (!ok) break;
+          tc_commit(st_empty_bar(b));
+          b ^= 1;
+          if (b == 0) b_phase ^= 1u;
+        }
+        if (!ok) break;
+        tc_commit(acc_full_bar(acc));
+        if (++acc == Cfg::kAccs) { acc = 0; acc_phase ^= 1u; }
+      }
+    }
+  } else if (warp >= 6) {
+    // ---------------- exponents: shared memory -> registers -> this warp's quadrant of tensor memory
+    const uint32_t quad = static_cast<uint32_t>(warp & 3) * 32u << 16;
+    int sf = 0, b = 0;
+    uint32_t sf_phase = 0, b_phase = 0;
+    bool ok = true;
+    for (int tile = blockIdx.x; tile < total_tiles && ok; tile += gridDim.x) {
+      for (int c = 0; c < chunks; ++c) {
+        if (!mbar_wait(sf_full_bar(sf), sf_phase, abort_flag, p.err)) { ok = false; break; }
+        const uint4 *src = reinterpret_cast<const uint4 *>(gen + Cfg::kSfOff + sf * Cfg::kSfStage);
+        uint32_t rm[16], rn[4 * Cfg::kSfN];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint4 w = src[j * 32 + lane];
+          rm[j] = w.x; rm[4 + j] = w.y; rm[8 + j] = w.z; rm[12 + j] = w.w;
+        }
+#pragma unroll
+        for (int j = 0; j < Cfg::kSfN; ++j) {
+          const bool have = j * 32 + lane < BN;
+          const uint4 w = have ? src[kTileM + j * 32 + lane] : make_uint4(0, 0, 0, 0);
+          rn[j] = w.x; rn[Cfg::kSfN + j] = w.y; rn[2 * Cfg::kSfN + j] = w.z; rn[3 * Cfg::kSfN + j] = w.w;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(sf_empty_bar(sf));
+        if (++sf == Cfg::kSfStages) { sf = 0; sf_phase ^= 1u; }
+        if (!mbar_wait(st_empty_bar(b), b_phase ^ 1u, abort_flag, p.err)) { ok = false; break; }
+        tc_fence_after();
+        const uint32_t dst = tmem + quad + static_cast<uint32_t>(Cfg::kSfBase + b * Cfg::kSfCols);
+        tmem_st16(dst, rm);
+        if constexpr (Cfg::kSfN == 4) {
+          tmem_st16(dst + 16, rn);
+        } else {
+          static_assert(Cfg::kSfN == 4 || Cfg::kSfN == 8, "columns of the N side's exponents");
+          tmem_st32(dst + 16, rn);
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(st_full_bar(b));
+        b ^= 1;
+        if (b == 0) b_phase ^= 1u;
+      }
+    }
+  } else {
+    // ---------------- epilogue
+    const int quad = warp & 3;
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    for (int tile = blockIdx.x; tile < total_tiles; tile += gridDim.x) {
+      find_tile<kRows, kColsC>(tile, tile_start, row_start, group, t);
+      if (!mbar_wait(acc_full_bar(acc), acc_phase, abort_flag, p.err)) break;
+      tc_fence_after();
+      const uint32_t src = tmem + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>(acc * BN);
+      const int64_t bias0 = t.group * p.bias_stride;
+      for (int c0 = 0; c0 < BN; c0 += 16) {
+        uint32_t r[16];
+        tmem_ld16(src + static_cast<uint32_t>(c0), r);
+        tmem_ld_wait();
+        if constexpr (SWAP) {                       // lane = column of C, register = row
+          const int64_t col = t.n0 + quad * 32 + lane;
+          if (col < p.n) {
+            const float bias = p.bias ? load_float(p.bias, p.bias_dtype, bias0 + col) : 0.0f;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              const int64_t row = t.row0 + c0 + j;
+              if (row < t.row_end) store_out(p, row * p.ldo + col, __fadd_rn(__uint_as_float(r[j]), bias));
+            }
+          }
+        } else {                                    // lane = row, register = column
+          const int64_t row = t.row0 + quad * 32 + lane;
+          if (row < t.row_end) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              const int64_t col = t.n0 + c0 + j;
+              if (col < p.n)
+                store_out(p, row * p.ldo + col, __fadd_rn(__uint_as_float(r[j]), p.bias ? load_float(p.bias, p.bias_dtype, bias0 + col) : 0.0f));
+            }
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(acc_empty_bar(acc));
+      if (++acc == Cfg::kAccs) { acc = 0; acc_phase ^= 1u; }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, Cfg::kTmemCols);
+  }
+}
+
+struct MxOperand {
+  const uint8_t *codes, *scales;
+  int64_t code_stride, scale_stride, code_bs, scale_bs;   // bytes between rows and between matrices
+  int64_t rows, batch;
+};
+
+template <int BN, bool SWAP>
+int32_t launch_mx(const MxOperand &a, const MxOperand &b, int64_t k, const MxParams &p, int64_t max_tiles, cudaStream_t st) {
+  using Cfg = MxCfg<BN>;
+  const MxOperand &om = SWAP ? b : a, &on = SWAP ? a : b;
+  CUtensorMap tm, tn, tsm, tsn;
+  const uint64_t kb = static_cast<uint64_t>((k + 1) / 2), ks = static_cast<uint64_t>(ceil_div(k, 32));
+  if (!make_byte_tmap3(&tm, om.codes, kb, om.rows, om.batch, om.code_stride, om.code_bs, 128, kTileM, true) ||
+      !make_byte_tmap3(&tn, on.codes, kb, on.rows, on.batch, on.code_stride, on.code_bs, 128, BN, true) ||
+      !make_byte_tmap3(&tsm, om.scales, ks, om.rows, om.batch, om.scale_stride, om.scale_bs, 16, kTileM, false) ||
+      !make_byte_tmap3(&tsn, on.scales, ks, on.rows, on.batch, on.scale_stride, on.scale_bs, 16, BN, false))
+    return fail(BSIR_ERR_STRIDE, "matmul_mxfp4: the driver refuses a tensor map of these sizes and strides");
+  cudaFuncSetAttribute(mxfp4_gemm_kernel<BN, SWAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmem);
+  int64_t grid = device_info().sm_count > 0 ? device_info().sm_count : 148;
+  if (grid > max_tiles) grid = max_tiles;
+  launch_pdl(mxfp4_gemm_kernel<BN, SWAP>, dim3(static_cast<unsigned>(grid)), dim3(kThreads), Cfg::kSmem, st, tm, tn, tsm, tsn, p);
+  count_launch();
+  return check_launch("matmul_mxfp4");
+}
+
+}  // namespace
+}  // namespace bsir
+
+using namespace bsir;
+
+extern "C" int32_t bsir_matmul_mxfp4(const bsir_matmul_mxfp4_desc *d, void *stream) {
+  clear_error();
+  if (!d) return fail(BSIR_ERR_NULL, "matmul_mxfp4: null description");
+  if (!dtype_is_float(d->out_dtype)) return fail(BSIR_ERR_DTYPE, "matmul_mxfp4: out dtype %d (f32, f16, bf16)", d->out_dtype);
+  if (d->bias && !dtype_is_float(d->bias_dtype)) return fail(BSIR_ERR_DTYPE, "matmul_mxfp4: bias dtype %d (f32, f16, bf16)", d->bias_dtype);
+  constexpr int64_t kMax = int64_t{1} << 30;
+  if (d->m < 0 || d->n < 0 || d->k < 1 || d->m > kMax || d->n > kMax || d->k > kMax)
+    return fail(BSIR_ERR_SHAPE, "matmul_mxfp4: m %lld, n %lld, k %lld (k at least 1, none above 2^30)", (long long)d->m, (long long)d->n, (long long)d->k);
+  if (d->offsets ? (d->groups < 1 || d->groups > kMaxGroups) : d->groups > 1)
+    return fail(BSIR_ERR_SHAPE, "matmul_mxfp4: %lld groups (1 to %d with offsets, at most 1 without)", (long long)d->groups, kMaxGroups);
+  if (d->m == 0 || d->n == 0) return BSIR_OK;
+  if (!d->a || !d->scale_a || !d->b || !d->scale_b || !d->out) return fail(BSIR_ERR_NULL, "matmul_mxfp4: null pointer");
+  const int64_t groups = d->offsets ? d->groups : 1;
+  const int64_t kb = (d->k + 1) / 2, ks = ceil_div(d->k, 32);
+  const int64_t kb16 = ceil_div(kb, 16) * 16, ks16 = ceil_div(ks, 16) * 16;
+  MxOperand a{d->a, d->scale_a, d->lda, d->ldsa, 0, 0, d->m, 1}, b{d->b, d->scale_b, d->ldb, d->ldsb, d->batch_stride_b, d->batch_stride_sb, d->n, groups};
+  for (MxOperand *o : {&a, &b}) {
+    const char *name = o == &a ? "a" : "b";
+    if (o->rows == 1) { o->code_stride = kb16; o->scale_stride = ks16; }      // a lone row's pitch means nothing
+    if (o->batch == 1) { o->code_bs = o->rows * o->code_stride; o->scale_bs = o->rows * o->scale_stride; }
+    if (o->code_stride < kb || o->scale_stride < ks || o->code_stride % 16 || o->scale_stride % 16)
+      return fail(BSIR_ERR_STRIDE, "matmul_mxfp4: row strides of %s: codes %lld bytes (at least %lld), exponents %lld (at least %lld), multiples of 16", name,
+                  (long long)o->code_stride, (long long)kb, (long long)o->scale_stride, (long long)ks);
+    if (o->code_bs % 16 || o->scale_bs % 16 || o->code_bs < (o->rows - 1) * o->code_stride + kb || o->scale_bs < (o->rows - 1) * o->scale_stride + ks)
+      return fail(BSIR_ERR_STRIDE, "matmul_mxfp4: group strides of %s: codes %lld bytes, exponents %lld: multiples of 16 that hold a matrix", name,
+                  (long long)o->code_bs, (long long)o->scale_bs);
+    if (!aligned_to(o->codes, 16) || !aligned_to(o->scales, 16)) return fail(BSIR_ERR_ALIGN, "matmul_mxfp4: %s and its exponents want 16-byte aligned bases", name);
+  }
+  const int eb = dtype_bytes(d->out_dtype);
+  const int64_t ldo = d->m == 1 ? d->n : d->ldo;
+  if (ldo < d->n) return fail(BSIR_ERR_STRIDE, "matmul_mxfp4: row stride %lld of out for %lld columns", (long long)ldo, (long long)d->n);
+  if (!aligned_to(d->out, eb) || (d->offsets && !aligned_to(d->offsets, 4)) || (d->bias && !aligned_to(d->bias, dtype_bytes(d->bias_dtype))))
+    return fail(BSIR_ERR_ALIGN, "matmul_mxfp4: out, offsets or bias misaligned");
+  {
+    const char *o0 = static_cast<const char *>(d->out), *o1 = o0 + ((d->m - 1) * ldo + d->n) * eb;
+    const int64_t nbias = d->bias ? ((groups - 1) * d->bias_stride + d->n) * dtype_bytes(d->bias_dtype) : 0;
+    struct { const void *p; int64_t bytes; } in[6] = {
+        {a.codes, (a.rows - 1) * a.code_stride + kb}, {a.scales, (a.rows - 1) * a.scale_stride + ks},
+        {b.codes, (groups - 1) * b.code_bs + (b.rows - 1) * b.code_stride + kb}, {b.scales, (groups - 1) * b.scale_bs + (b.rows - 1) * b.scale_stride + ks},
+        {d->bias, nbias}, {d->offsets, d->offsets ? (groups + 1) * 4 : 0}};
+    for (const auto &i : in) {
+      const char *i0 = static_cast<const char *>(i.p);
+      if (i.bytes > 0 && i0 < o1 && o0 < i0 + i.bytes) return fail(BSIR_ERR_UNSUPPORTED, "matmul_mxfp4: out may not overlap an operand");
+    }
+  }
+  MxParams p{};
+  p.m = d->m; p.n = d->n; p.k_blocks = static_cast<int>(ceil_div(d->k, kStageK));
+  p.offsets = d->offsets; p.groups = static_cast<int>(groups);
+  p.bias = d->bias; p.bias_stride = d->bias_stride; p.bias_dtype = d->bias_dtype; p.out_dtype = d->out_dtype;
+  p.out = d->out; p.ldo = ldo;
+  p.err = device_error_word();
+  if (!p.err) return fail(BSIR_ERR_WORKSPACE, "matmul_mxfp4: no device error word");
+  cudaStream_t st = resolve_stream(stream);
+  // rows of a group that a tile should hold: all rows, or the groups' mean (their sizes are on the device)
+  const int64_t rows = ceil_div(d->m, groups);
+  auto tiles = [&](int64_t r, int64_t c) { return (d->m / r + groups) * ceil_div(d->n, c); };   // at most
+  if (rows <= 16) return launch_mx<16, true>(a, b, d->k, p, tiles(16, kTileM), st);
+  if (rows <= 64) return launch_mx<64, true>(a, b, d->k, p, tiles(64, kTileM), st);
+  return launch_mx<128, false>(a, b, d->k, p, tiles(kTileM, 128), st);
+}

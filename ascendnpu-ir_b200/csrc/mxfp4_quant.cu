@@ -1,0 +1,488 @@
+// mxfp4_quant.cu -- quantisation to and from microscaled 4-bit floats (the OCP MX format MXFP4): 32 consecutive
+// elements along the contracted axis share one exponent byte (E8M0: 2^(byte - 127), 255 = NaN), an element is e2m1
+// (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign), two to a byte with the even element in the lower half.
+//
+//   byte = clamp(floor(log2(max |x|)) - 2 + 127, 0, ..),   code = rne_e2m1(x * 2^(127 - byte)), stopped at +-6
+//
+// A power of two divides exactly, so every rounding but the element's own is avoided and the result does not depend on
+// how the work is cut: the exponent is read off the bits of the largest magnitude (its exponent field less 2), and
+// x * 2^(127 - byte) is exact wherever it could matter (only what rounds to zero anyway can fall under the normals).
+// A block that holds a NaN or an infinity gets the exponent byte 255 and codes 0.  Missing elements of a last block
+// are zeros, the unused half of a row's last byte is 0.
+//
+// Both directions of a matrix can come out of one read: blocks along the rows (what C = A * B^T contracts) and blocks
+// down the columns with the result transposed (what the products of a backward pass contract).
+#include "common.cuh"
+
+namespace bsir {
+namespace {
+
+constexpr int kBlock = 32;
+
+// index -> row without a division instruction: row = (i * magic) >> shift for i < 2^31 (round-up method; the divisor
+// of a vector index is the number of vectors in a padded row)
+struct FastDiv {
+  uint32_t d, magic, shift;
+};
+FastDiv make_fastdiv(uint32_t d) {
+  FastDiv f{d, 0, 0};
+  while ((1ull << f.shift) < d) ++f.shift;
+  f.magic = static_cast<uint32_t>(((1ull << 32) * ((1ull << f.shift) - d)) / d + 1);
+  return f;
+}
+__device__ __forceinline__ uint32_t fast_div(const FastDiv &f, uint32_t i) {
+  return (__umulhi(i, f.magic) + i) >> f.shift;   // i < 2^31 and the high product < i: the sum cannot wrap
+}
+
+// the largest magnitude's bits (NaN > infinity > numbers) -> exponent byte
+__device__ __forceinline__ uint32_t scale_byte(uint32_t abs_bits) {
+  const uint32_t e = abs_bits >> 23;
+  return e == 255u ? 255u : (e > 2u ? e - 2u : 0u);
+}
+// 2^(127 - byte) as float; byte <= 252 unless 255
+__device__ __forceinline__ float inv_scale(uint32_t byte) { return __uint_as_float((254u - (byte > 252u ? 252u : byte)) << 23); }
+
+// eight values -> eight codes, element 0 in the lowest half byte.  The conversion rounds to nearest even, stops at
+// +-6 and keeps the sign of what rounds to zero.
+__device__ __forceinline__ uint32_t pack_e2m1x8(const float *v) {
+  uint32_t r;
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n\t"
+      "mov.b32 %0, {b0, b1, b2, b3};\n\t}"
+      : "=r"(r)
+      : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
+  return r;
+}
+// eight codes -> eight values (exact in f16, hence in f32)
+__device__ __forceinline__ void unpack_e2m1x8(uint32_t q, float *v) {
+  uint32_t h[4];
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+      "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, b0;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, b2;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
+      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+      : "r"(q));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] = f16lo_to_f32(h[i]);
+    v[2 * i + 1] = f16hi_to_f32(h[i]);
+  }
+}
+
+template <int DT> __device__ __forceinline__ float load_elem(const void *x, int64_t i) {
+  if constexpr (DT == BSIR_F32) return static_cast<const float *>(x)[i];
+  else if constexpr (DT == BSIR_F16) return __half2float(__ushort_as_half(static_cast<const unsigned short *>(x)[i]));
+  else return __uint_as_float(static_cast<uint32_t>(static_cast<const unsigned short *>(x)[i]) << 16);
+}
+
+// eight consecutive elements of a row as floats; those at or behind `cols` are zeros
+template <int DT, bool VEC>
+__device__ __forceinline__ void load8(const void *x, int64_t row_at, int64_t c, int64_t cols, float *v) {
+  constexpr int kWords = 8 / FloatTraits<DT>::kPerWord;
+  if constexpr (VEC) {                 // cols % 8 == 0: a vector is all inside or all outside
+    if (c < cols) {
+      const char *src = static_cast<const char *>(x) + (row_at + c) * (4 / FloatTraits<DT>::kPerWord);
+#pragma unroll
+      for (int w = 0; w < kWords; w += 4) {
+        const Vec16 b = ld_stream(src + 4 * w);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) FloatTraits<DT>::unpack(b.w[i], v + (w + i) * FloatTraits<DT>::kPerWord);
+      }
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = c + i < cols ? load_elem<DT>(x, row_at + c + i) : 0.0f;
+  }
+}
+
+__device__ __forceinline__ uint32_t abs_max8(const float *v) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+  return m;
+}
+
+struct QuantParams {
+  int64_t rows, cols;
+  const void *x;
+  int64_t xs;                 // row stride of x, elements
+  uint8_t *q;                 // blocks along the rows, may be null
+  int64_t qs;
+  uint8_t *s;
+  int64_t ss;
+  uint8_t *qt;                // blocks down the columns, transposed, may be null
+  int64_t qts;
+  uint8_t *st;
+  int64_t sts;
+  FastDiv div;
+  uint32_t nvec;              // vectors of eight in all rows, rows padded to whole blocks
+  int q_words, qt_words;      // 4-byte / 16-byte stores of codes are aligned
+};
+
+__device__ __forceinline__ void store_codes(uint8_t *dst, uint32_t codes, int nbytes, bool words) {
+  if (words && nbytes >= 4) {
+    *reinterpret_cast<uint32_t *>(dst) = codes;
+  } else {
+    for (int i = 0; i < 4 && i < nbytes; ++i) dst[i] = static_cast<uint8_t>(codes >> (8 * i));
+  }
+}
+
+// Blocks along the rows: a lane takes eight elements (16 bytes of a 16-bit type), four lanes are a block and meet in
+// two shuffles; a warp's codes leave as 128 consecutive bytes.  Four vectors a thread are loaded before the first is
+// used.
+constexpr int kRowVecs = 4;
+template <int DT, bool VEC>
+__global__ void __launch_bounds__(256) mxfp4_rows_kernel(QuantParams p) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const uint32_t v0 = blockIdx.x * (256u * kRowVecs) + threadIdx.x;
+  float v[kRowVecs][8];
+  uint32_t row[kRowVecs], col[kRowVecs];
+#pragma unroll
+  for (int u = 0; u < kRowVecs; ++u) {
+    const uint32_t i = v0 + u * 256u;
+    row[u] = fast_div(p.div, i);
+    col[u] = (i - row[u] * p.div.d) * 8u;
+    load8<DT, VEC>(p.x, static_cast<int64_t>(row[u]) * p.xs, col[u], i < p.nvec ? p.cols : 0, v[u]);
+  }
+#pragma unroll
+  for (int u = 0; u < kRowVecs; ++u) {
+    uint32_t m = abs_max8(v[u]);
+    m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+    const uint32_t byte = scale_byte(m);
+    const float inv = inv_scale(byte);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[u][i] = __fmul_rn(v[u][i], inv);
+    const uint32_t codes = byte == 255u ? 0u : pack_e2m1x8(v[u]);
+    if (v0 + u * 256u < p.nvec && col[u] < p.cols) {
+      const int nbytes = static_cast<int>(min(static_cast<int64_t>(4), (p.cols - col[u] + 1) / 2));
+      store_codes(p.q + static_cast<int64_t>(row[u]) * p.qs + col[u] / 2, codes, nbytes, p.q_words);
+      if ((threadIdx.x & 3) == 0) p.s[static_cast<int64_t>(row[u]) * p.ss + col[u] / kBlock] = static_cast<uint8_t>(byte);
+    }
+  }
+}
+
+// Blocks down the columns, and along the rows as well when `q` is wanted: a CTA brings a tile of kTR rows x 64 columns
+// into shared memory (16-byte loads, 128 bytes of a row of a 16-bit type; the row-wise form is made from the registers
+// on the way), then a thread takes two neighbouring columns of a 32-row block -- a warp reads one row of the tile at a
+// time -- and its two blocks' codes (16 bytes each) go through shared memory so that a column's codes leave as kTR / 2
+// consecutive bytes.
+constexpr int kTC = 64;
+template <int DT> constexpr int kTR = DT == BSIR_F32 ? 128 : 256;
+template <int DT, bool VEC>
+__global__ void __launch_bounds__(256) mxfp4_cols_kernel(QuantParams p) {
+  constexpr int TR = kTR<DT>;
+  constexpr int EB = 4 / FloatTraits<DT>::kPerWord;
+  constexpr int kCodeRow = TR / 2 + 16;                  // bytes of a column's codes, padded against bank conflicts
+  extern __shared__ __align__(16) uint8_t tile[];        // [TR][kTC] elements, then [kTC][kCodeRow] codes
+  uint8_t *codes_s = tile + TR * kTC * EB;
+  __shared__ uint8_t scale_s[kTC][TR / kBlock];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int64_t r0 = static_cast<int64_t>(blockIdx.x) * TR;
+  const int64_t c0 = static_cast<int64_t>(blockIdx.y) * kTC;
+  const int tid = threadIdx.x;
+  constexpr int kPasses = TR * (kTC / 8) / 256;
+#pragma unroll
+  for (int u0 = 0; u0 < kPasses; u0 += 4) {
+    float v[4][8];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int i = (u0 + u) * 256 + tid, r = i >> 3, c = (i & 7) * 8;
+      load8<DT, VEC>(p.x, (r0 + r) * p.xs, c0 + c, r0 + r < p.rows ? p.cols : 0, v[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int i = (u0 + u) * 256 + tid, r = i >> 3, c = (i & 7) * 8;
+      uint32_t w[8 / FloatTraits<DT>::kPerWord];
+#pragma unroll
+      for (int j = 0; j < 8 / FloatTraits<DT>::kPerWord; ++j) w[j] = FloatTraits<DT>::pack(v[u] + j * FloatTraits<DT>::kPerWord);
+#pragma unroll
+      for (int j = 0; j < 8 / FloatTraits<DT>::kPerWord; j += 4)
+        *reinterpret_cast<uint4 *>(tile + (r * kTC + c) * EB + 4 * j) = make_uint4(w[j], w[j + 1], w[j + 2], w[j + 3]);
+      if (p.q) {
+        uint32_t m = abs_max8(v[u]);
+        m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+        m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+        const uint32_t byte = scale_byte(m);
+        const float inv = inv_scale(byte);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[u][j] = __fmul_rn(v[u][j], inv);
+        const uint32_t codes = byte == 255u ? 0u : pack_e2m1x8(v[u]);
+        const int64_t row = r0 + r, col = c0 + c;
+        if (row < p.rows && col < p.cols) {
+          const int nbytes = static_cast<int>(min(static_cast<int64_t>(4), (p.cols - col + 1) / 2));
+          store_codes(p.q + row * p.qs + col / 2, codes, nbytes, p.q_words);
+          if ((tid & 3) == 0) p.s[row * p.ss + col / kBlock] = static_cast<uint8_t>(byte);
+        }
+      }
+    }
+  }
+  __syncthreads();
+  const int lane = tid & 31;
+  for (int b = tid >> 5; b < TR / kBlock; b += 8) {      // this warp's 32-row block; lane = a pair of columns
+    uint32_t m0 = 0, m1 = 0;
+    float a[kBlock], c[kBlock];
+#pragma unroll
+    for (int r = 0; r < kBlock; ++r) {
+      const uint8_t *src = tile + ((b * kBlock + r) * kTC + 2 * lane) * EB;
+      if constexpr (DT == BSIR_F32) {
+        const float2 f = *reinterpret_cast<const float2 *>(src);
+        a[r] = f.x;
+        c[r] = f.y;
+      } else {
+        float f[2];
+        FloatTraits<DT>::unpack(*reinterpret_cast<const uint32_t *>(src), f);
+        a[r] = f[0];
+        c[r] = f[1];
+      }
+      m0 = max(m0, __float_as_uint(a[r]) & 0x7fffffffu);
+      m1 = max(m1, __float_as_uint(c[r]) & 0x7fffffffu);
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float *v = h ? c : a;
+      const uint32_t byte = scale_byte(h ? m1 : m0);
+      const float inv = inv_scale(byte);
+      uint32_t w[4];
+#pragma unroll
+      for (int r = 0; r < kBlock; ++r) v[r] = __fmul_rn(v[r], inv);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] = byte == 255u ? 0u : pack_e2m1x8(v + 8 * j);
+      *reinterpret_cast<uint4 *>(codes_s + (2 * lane + h) * kCodeRow + b * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+      scale_s[2 * lane + h][b] = static_cast<uint8_t>(byte);
+    }
+  }
+  __syncthreads();
+  constexpr int kPieces = TR / kBlock;                   // 16-byte pieces of a column's codes
+  const int64_t code_bytes = (p.rows + 1) / 2, blocks = (p.rows + kBlock - 1) / kBlock;
+  for (int i = tid; i < kTC * kPieces; i += 256) {
+    const int c = i / kPieces, b = i % kPieces;
+    const int64_t col = c0 + c, at = r0 / 2 + b * 16;
+    if (col >= p.cols || at >= code_bytes) continue;
+    uint8_t *dst = p.qt + col * p.qts + at;
+    const uint8_t *src = codes_s + c * kCodeRow + b * 16;
+    if (p.qt_words && at + 16 <= code_bytes) {
+      *reinterpret_cast<uint4 *>(dst) = *reinterpret_cast<const uint4 *>(src);
+    } else {
+      for (int j = 0; j < 16 && at + j < code_bytes; ++j) dst[j] = src[j];
+    }
+    if (r0 / kBlock + b < blocks) p.st[col * p.sts + r0 / kBlock + b] = scale_s[c][b];
+  }
+}
+
+// codes and exponents -> values: a lane takes eight codes (4 bytes in, 16 or 32 bytes out)
+struct DequantParams {
+  int64_t cols;
+  const uint8_t *q;
+  int64_t qs;
+  const uint8_t *s;
+  int64_t ss;
+  void *y;
+  int64_t ys;
+  FastDiv div;
+  uint32_t nvec;
+  int q_words;
+};
+template <int DT, bool VEC>
+__global__ void __launch_bounds__(256) mxfp4_dequant_kernel(DequantParams p) {
+  constexpr int kPer = FloatTraits<DT>::kPerWord;
+  pdl_launch_dependents();
+  pdl_wait();
+  const uint32_t v0 = blockIdx.x * (256u * kRowVecs) + threadIdx.x;
+  uint32_t codes[kRowVecs], byte[kRowVecs];
+#pragma unroll
+  for (int u = 0; u < kRowVecs; ++u) {
+    const uint32_t i = v0 + u * 256u;
+    codes[u] = byte[u] = 0;
+    if (i >= p.nvec) continue;
+    const uint32_t row = fast_div(p.div, i);
+    const int64_t col = static_cast<int64_t>(i - row * p.div.d) * 8;
+    if (col >= p.cols) continue;
+    const uint8_t *src = p.q + static_cast<int64_t>(row) * p.qs + col / 2;
+    const int nbytes = static_cast<int>(min(static_cast<int64_t>(4), (p.cols - col + 1) / 2));
+    if (p.q_words && nbytes == 4) {
+      codes[u] = *reinterpret_cast<const uint32_t *>(src);
+    } else {
+      for (int j = 0; j < 4 && j < nbytes; ++j) codes[u] |= static_cast<uint32_t>(src[j]) << (8 * j);
+    }
+    byte[u] = p.s[static_cast<int64_t>(row) * p.ss + col / kBlock];
+  }
+#pragma unroll
+  for (int u = 0; u < kRowVecs; ++u) {
+    const uint32_t i = v0 + u * 256u;
+    if (i >= p.nvec) continue;
+    const uint32_t row = fast_div(p.div, i);
+    const int64_t col = static_cast<int64_t>(i - row * p.div.d) * 8;
+    if (col >= p.cols) continue;
+    float v[8];
+    unpack_e2m1x8(codes[u], v);
+    // 2^(byte - 127): byte 0 is 2^-127, under f32's normals (bits 0x00400000); 255 is NaN
+    const float sc = byte[u] == 255u ? __uint_as_float(0x7fc00000u) : byte[u] == 0u ? __uint_as_float(0x00400000u) : __uint_as_float(byte[u] << 23);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = __fmul_rn(v[j], sc);
+    const int64_t at = static_cast<int64_t>(row) * p.ys + col;
+    uint32_t w[8 / kPer];
+#pragma unroll
+    for (int j = 0; j < 8 / kPer; ++j) w[j] = FloatTraits<DT>::pack(v + j * kPer);
+    if (VEC) {
+      char *dst = static_cast<char *>(p.y) + at * (4 / kPer);
+#pragma unroll
+      for (int j = 0; j < 8 / kPer; j += 4) st_stream(dst + 4 * j, Vec16{{w[j], w[j + 1], w[j + 2], w[j + 3]}});
+    } else {
+      for (int j = 0; j < 8 && col + j < p.cols; ++j) {
+        if constexpr (DT == BSIR_F32) static_cast<uint32_t *>(p.y)[at + j] = w[j];
+        else static_cast<uint16_t *>(p.y)[at + j] = static_cast<uint16_t>(w[j >> 1] >> (16 * (j & 1)));
+      }
+    }
+  }
+}
+
+template <int DT, bool VEC>
+int32_t launch_quant(QuantParams p, cudaStream_t st) {
+  if (p.qt) {
+    constexpr int TR = kTR<DT>;
+    constexpr size_t smem = TR * kTC * (DT == BSIR_F32 ? 4 : 2) + kTC * (TR / 2 + 16);
+    cudaFuncSetAttribute(mxfp4_cols_kernel<DT, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    const int64_t gx = ceil_div(p.rows, TR), gy = ceil_div(p.cols, kTC);
+    // the grid's y axis ends at 65535: wider matrices go in column strips (a strip starts at a whole block)
+    for (int64_t y0 = 0; y0 < gy; y0 += 65535) {
+      QuantParams s = p;
+      const int64_t c0 = y0 * kTC, ny = gy - y0 < 65535 ? gy - y0 : 65535;
+      s.x = static_cast<const char *>(p.x) + c0 * dtype_bytes(DT);
+      s.cols = p.cols - c0 < ny * kTC ? p.cols - c0 : ny * kTC;
+      if (p.q) { s.q = p.q + c0 / 2; s.s = p.s + c0 / kBlock; }
+      s.qt = p.qt + c0 * p.qts;
+      s.st = p.st + c0 * p.sts;
+      launch_pdl(mxfp4_cols_kernel<DT, VEC>, dim3(static_cast<unsigned>(gx), static_cast<unsigned>(ny)), dim3(256), smem, st, s);
+      count_launch();
+    }
+    return check_launch("quant_mxfp4");
+  }
+  const int64_t vpr = ceil_div(p.cols, kBlock) * 4;
+  const int64_t step = (int64_t{1} << 30) / vpr > 0 ? (int64_t{1} << 30) / vpr : 1;   // rows of one launch: 32-bit vector indices
+  for (int64_t r = 0; r < p.rows; r += step) {
+    QuantParams s = p;
+    s.rows = p.rows - r < step ? p.rows - r : step;
+    s.x = static_cast<const char *>(p.x) + r * p.xs * dtype_bytes(DT);
+    s.q = p.q + r * p.qs;
+    s.s = p.s + r * p.ss;
+    s.div = make_fastdiv(static_cast<uint32_t>(vpr));
+    s.nvec = static_cast<uint32_t>(s.rows * vpr);
+    launch_pdl(mxfp4_rows_kernel<DT, VEC>, dim3(static_cast<unsigned>(ceil_div(s.nvec, 256 * kRowVecs))), dim3(256), 0, st, s);
+    count_launch();
+  }
+  return check_launch("quant_mxfp4");
+}
+template <int DT, bool VEC>
+int32_t launch_dequant(DequantParams p, int64_t rows, cudaStream_t st) {
+  const int64_t vpr = ceil_div(p.cols, kBlock) * 4;
+  const int64_t step = (int64_t{1} << 30) / vpr > 0 ? (int64_t{1} << 30) / vpr : 1;
+  for (int64_t r = 0; r < rows; r += step) {
+    DequantParams s = p;
+    s.q = p.q + r * p.qs;
+    s.s = p.s + r * p.ss;
+    s.y = static_cast<char *>(p.y) + r * p.ys * dtype_bytes(DT);
+    s.div = make_fastdiv(static_cast<uint32_t>(vpr));
+    s.nvec = static_cast<uint32_t>((rows - r < step ? rows - r : step) * vpr);
+    launch_pdl(mxfp4_dequant_kernel<DT, VEC>, dim3(static_cast<unsigned>(ceil_div(s.nvec, 256 * kRowVecs))), dim3(256), 0, st, s);
+    count_launch();
+  }
+  return check_launch("dequant_mxfp4");
+}
+
+// [rows, cols] codes and exponents: strides and sizes (a 32-bit column index holds a row's vectors)
+int32_t check_codes(const char *what, int64_t rows, int64_t cols, const void *q, int64_t qs, const void *s, int64_t ss) {
+  if (!q || !s) return fail(BSIR_ERR_NULL, "%s: null pointer", what);
+  if (rows > 1 && (qs < (cols + 1) / 2 || ss < ceil_div(cols, kBlock)))
+    return fail(BSIR_ERR_STRIDE, "%s: row strides %lld / %lld bytes for %lld columns (codes take %lld, exponents %lld)", what, (long long)qs,
+                (long long)ss, (long long)cols, (long long)((cols + 1) / 2), (long long)ceil_div(cols, kBlock));
+  return BSIR_OK;
+}
+bool ranges_overlap(const void *a, int64_t na, const void *b, int64_t nb) {
+  const char *a0 = static_cast<const char *>(a), *b0 = static_cast<const char *>(b);
+  return a0 < b0 + nb && b0 < a0 + na;
+}
+
+}  // namespace
+}  // namespace bsir
+
+using namespace bsir;
+
+extern "C" int32_t bsir_quant_mxfp4(int32_t dtype, int64_t rows, int64_t cols, const void *x, int64_t x_row_stride, uint8_t *q,
+                                    int64_t q_row_stride, uint8_t *scale, int64_t scale_row_stride, uint8_t *qt, int64_t qt_row_stride,
+                                    uint8_t *scale_t, int64_t scale_t_row_stride, void *stream) {
+  clear_error();
+  if (!dtype_is_float(dtype)) return fail(BSIR_ERR_DTYPE, "quant_mxfp4: dtype %d (f32, f16, bf16)", dtype);
+  if (rows < 0 || cols < 0 || rows > (int64_t{1} << 31) || cols > (int64_t{1} << 31))
+    return fail(BSIR_ERR_SHAPE, "quant_mxfp4: [%lld, %lld] (at most 2^31 either way)", (long long)rows, (long long)cols);
+  if ((q == nullptr) != (scale == nullptr) || (qt == nullptr) != (scale_t == nullptr))
+    return fail(BSIR_ERR_NULL, "quant_mxfp4: codes and exponents of a direction come together");
+  if (rows == 0 || cols == 0) return BSIR_OK;
+  if (!x || (!q && !qt)) return fail(BSIR_ERR_NULL, "quant_mxfp4: null pointer");
+  const int eb = dtype_bytes(dtype);
+  if (rows > 1 && x_row_stride < cols) return fail(BSIR_ERR_STRIDE, "quant_mxfp4: row stride %lld of %lld columns", (long long)x_row_stride, (long long)cols);
+  if (!aligned_to(x, eb)) return fail(BSIR_ERR_ALIGN, "quant_mxfp4: misaligned");
+  if (rows == 1) { x_row_stride = cols; q_row_stride = (cols + 1) / 2; scale_row_stride = ceil_div(cols, kBlock); }
+  if (cols == 1) { qt_row_stride = (rows + 1) / 2; scale_t_row_stride = ceil_div(rows, kBlock); }
+  const int64_t x_bytes = ((rows - 1) * x_row_stride + cols) * eb;
+  for (int d = 0; d < 2; ++d) {
+    const void *cq = d ? qt : q, *cs = d ? scale_t : scale;
+    if (!cq) continue;
+    const int64_t r = d ? cols : rows, c = d ? rows : cols, qs = d ? qt_row_stride : q_row_stride, ss = d ? scale_t_row_stride : scale_row_stride;
+    if (int32_t rc = check_codes("quant_mxfp4", r, c, cq, qs, cs, ss)) return rc;
+    if (ranges_overlap(x, x_bytes, cq, (r - 1) * qs + (c + 1) / 2) || ranges_overlap(x, x_bytes, cs, (r - 1) * ss + ceil_div(c, kBlock)))
+      return fail(BSIR_ERR_UNSUPPORTED, "quant_mxfp4: a result may not overlap the source");
+  }
+  QuantParams p{};
+  p.rows = rows; p.cols = cols; p.x = x; p.xs = x_row_stride;
+  p.q = q; p.qs = q_row_stride; p.s = scale; p.ss = scale_row_stride;
+  p.qt = qt; p.qts = qt_row_stride; p.st = scale_t; p.sts = scale_t_row_stride;
+  p.q_words = q && aligned_to(q, 4) && q_row_stride % 4 == 0;
+  p.qt_words = qt && aligned_to(qt, 16) && qt_row_stride % 16 == 0;
+  const bool vec = cols % 8 == 0 && aligned_to(x, 16) && (x_row_stride * eb) % 16 == 0;
+  cudaStream_t st = resolve_stream(stream);
+  switch (dtype) {
+    case BSIR_F32: return vec ? launch_quant<BSIR_F32, true>(p, st) : launch_quant<BSIR_F32, false>(p, st);
+    case BSIR_F16: return vec ? launch_quant<BSIR_F16, true>(p, st) : launch_quant<BSIR_F16, false>(p, st);
+    default: return vec ? launch_quant<BSIR_BF16, true>(p, st) : launch_quant<BSIR_BF16, false>(p, st);
+  }
+}
+
+extern "C" int32_t bsir_dequant_mxfp4(int32_t dtype, int64_t rows, int64_t cols, const uint8_t *q, int64_t q_row_stride, const uint8_t *scale,
+                                      int64_t scale_row_stride, void *y, int64_t y_row_stride, void *stream) {
+  clear_error();
+  if (!dtype_is_float(dtype)) return fail(BSIR_ERR_DTYPE, "dequant_mxfp4: dtype %d (f32, f16, bf16)", dtype);
+  if (rows < 0 || cols < 0 || rows > (int64_t{1} << 31) || cols > (int64_t{1} << 31))
+    return fail(BSIR_ERR_SHAPE, "dequant_mxfp4: [%lld, %lld] (at most 2^31 either way)", (long long)rows, (long long)cols);
+  if (rows == 0 || cols == 0) return BSIR_OK;
+  if (!y) return fail(BSIR_ERR_NULL, "dequant_mxfp4: null pointer");
+  if (int32_t rc = check_codes("dequant_mxfp4", rows, cols, q, q_row_stride, scale, scale_row_stride)) return rc;
+  if (rows > 1 && y_row_stride < cols) return fail(BSIR_ERR_STRIDE, "dequant_mxfp4: row stride %lld of %lld columns", (long long)y_row_stride, (long long)cols);
+  const int eb = dtype_bytes(dtype);
+  if (!aligned_to(y, eb)) return fail(BSIR_ERR_ALIGN, "dequant_mxfp4: misaligned");
+  if (rows == 1) { q_row_stride = (cols + 1) / 2; scale_row_stride = ceil_div(cols, kBlock); y_row_stride = cols; }
+  const int64_t y_bytes = ((rows - 1) * y_row_stride + cols) * eb;
+  if (ranges_overlap(y, y_bytes, q, (rows - 1) * q_row_stride + (cols + 1) / 2) ||
+      ranges_overlap(y, y_bytes, scale, (rows - 1) * scale_row_stride + ceil_div(cols, kBlock)))
+    return fail(BSIR_ERR_UNSUPPORTED, "dequant_mxfp4: the result may not overlap the source");
+  DequantParams p{};
+  p.cols = cols; p.q = q; p.qs = q_row_stride; p.s = scale; p.ss = scale_row_stride; p.y = y; p.ys = y_row_stride;
+  p.q_words = aligned_to(q, 4) && q_row_stride % 4 == 0;
+  const bool vec = cols % 8 == 0 && aligned_to(y, 16) && (y_row_stride * eb) % 16 == 0;
+  cudaStream_t st = resolve_stream(stream);
+  switch (dtype) {
+    case BSIR_F32: return vec ? launch_dequant<BSIR_F32, true>(p, rows, st) : launch_dequant<BSIR_F32, false>(p, rows, st);
+    case BSIR_F16: return vec ? launch_dequant<BSIR_F16, true>(p, rows, st) : launch_dequant<BSIR_F16, false>(p, rows, st);
+    default: return vec ? launch_dequant<BSIR_BF16, true>(p, rows, st) : launch_dequant<BSIR_BF16, false>(p, rows, st);
+  }
+}

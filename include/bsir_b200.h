@@ -505,6 +505,88 @@ BSIR_API int32_t bsir_matmul_w4a16_peers(int64_t m, int64_t n, int64_t k, int64_
                                          int64_t ldo, void *stream);
 
 /* ------------------------------------------------------------------------ */
+/* microscaled 4-bit floats and mixtures of experts                          */
+/* ------------------------------------------------------------------------ */
+/* The reference has neither; both stand beside the int8 / int4 quantisers and GEMMs above.
+ *
+ * MXFP4 (OCP microscaling): 32 consecutive elements along the axis that a product contracts share an exponent byte,
+ * value 2^(byte - 127), 255 = NaN; elements are e2m1 (0, 0.5, 1, 1.5, 2, 3, 4, 6, top bit the sign), two to a byte, the
+ * even element in the lower half.  A [rows, cols] matrix has codes [rows, ceil(cols / 2)] and exponents
+ * [rows, ceil(cols / 32)], both uint8 with row strides in bytes.
+ *
+ * bsir_quant_mxfp4: byte = max(0, floor(log2(max |x|)) - 2 + 127), codes = x * 2^(127 - byte) rounded to nearest even,
+ * stopped at +-6; a block that holds a NaN or an infinity gets byte 255 and codes 0; elements that a last block lacks
+ * count as 0, and the unused half of a row's last byte is 0.  (q, scale): blocks along the rows.  (qt, scale_t): blocks
+ * down the columns, result transposed -- codes [cols, ceil(rows / 2)], exponents [cols, ceil(rows / 32)].  Either pair may
+ * be NULL; with both the source is read once.  The products of a linear layer's backward pass contract other axes than
+ * its forward product, so dY is wanted both ways, X and W down their columns.
+ * x: f32, f16 or bf16; at most 2^31 rows and columns; results may not overlap x. */
+BSIR_API int32_t bsir_quant_mxfp4(int32_t dtype, int64_t rows, int64_t cols, const void *x, int64_t x_row_stride, uint8_t *q,
+                                  int64_t q_row_stride, uint8_t *scale, int64_t scale_row_stride, uint8_t *qt,
+                                  int64_t qt_row_stride, uint8_t *scale_t, int64_t scale_t_row_stride, void *stream);
+/* y[r, c] = code * 2^(byte - 127) rounded to f32, f16 or bf16 (exact wherever y's type holds the value; what
+ * bsir_quant_mxfp4 made from that type always is). */
+BSIR_API int32_t bsir_dequant_mxfp4(int32_t dtype, int64_t rows, int64_t cols, const uint8_t *q, int64_t q_row_stride,
+                                    const uint8_t *scale, int64_t scale_row_stride, void *y, int64_t y_row_stride, void *stream);
+
+/* C[i, j] = cast_rint( sum_k A[i, k] * B[j, k] + bias[j] ) of MXFP4 matrices A [m, k] and B [n, k], accumulated in f32.
+ * With `offsets` (groups + 1 int32 on the device, not decreasing, within 0 .. m) rows offsets[g] .. offsets[g + 1] of A
+ * meet matrix g of B and bias g: the experts' products after bsir_expert_sort / _dispatch.  Rows of C that no group holds
+ * are left as they were; offsets outside 0 .. m are clamped.  The product's time follows the rows that the groups hold, so
+ * the call needs no size from the device and can be captured in a graph.
+ * Strides in bytes for codes and exponents (bases and strides multiples of 16; a row's exponents are padded to that),
+ * in elements for bias and out.  An odd k wants the unused half of a row's last byte 0 in one operand at least.
+ * 1 <= k; m, n, k <= 2^30; at most 1024 groups.  out: f32, f16 (no clamping: too large becomes infinite) or bf16; it may
+ * not overlap an operand. */
+typedef struct bsir_matmul_mxfp4_desc {
+  int32_t out_dtype;
+  int32_t bias_dtype;            /* BSIR_F32, BSIR_F16 or BSIR_BF16                                        */
+  int64_t m, n, k;
+  const uint8_t *a;              /* codes [m, ceil(k / 2)]                                                  */
+  int64_t lda;
+  const uint8_t *scale_a;        /* exponents [m, ceil(k / 32)]                                             */
+  int64_t ldsa;
+  const uint8_t *b;              /* codes [groups][n, ceil(k / 2)]                                          */
+  int64_t ldb, batch_stride_b;
+  const uint8_t *scale_b;        /* exponents [groups][n, ceil(k / 32)]                                     */
+  int64_t ldsb, batch_stride_sb;
+  const void *bias;              /* [groups][n] or NULL                                                     */
+  int64_t bias_stride;           /* elements between the groups' biases (0: one bias for all)               */
+  const int32_t *offsets;        /* [groups + 1] on the device, or NULL: one group of all m rows            */
+  int64_t groups;                /* 0 or 1 without offsets                                                  */
+  void *out;
+  int64_t ldo;
+} bsir_matmul_mxfp4_desc;
+BSIR_API int32_t bsir_matmul_mxfp4(const bsir_matmul_mxfp4_desc *desc, void *stream);
+
+/* Tokens sorted by expert.  ids [tokens, top_k] (int32 or int64): the expert of each choice; a number outside
+ * 0 .. experts - 1 names none (a padding token, an expert of another rank): such a choice is masked.
+ * offsets [experts + 1]: rows offsets[e] .. offsets[e + 1] belong to expert e.  slots [tokens, top_k]: the row of each
+ * choice, -1 for a masked one; rows of one expert keep the order of their choices.  experts <= 1024; more than 4096
+ * choices take the library's scratch (4 bytes x experts for each 4096 choices). */
+BSIR_API int32_t bsir_expert_sort(int32_t id_dtype, int64_t tokens, int64_t top_k, int64_t experts, const void *ids,
+                                  int32_t *offsets, int32_t *slots, void *stream);
+/* out[slots[t, j]] = x[t] for every choice that is not masked; other rows of out are left as they were.  Any element
+ * type (moved as bits: codes and exponents of a quantised x too).  No two choices may name one row (bsir_expert_sort's
+ * never do).  Here and below a slot outside -1 .. rows - 1 counts as masked and sets BSIR_DEVERR_GATHER_INDEX in the
+ * device error word. */
+BSIR_API int32_t bsir_expert_dispatch(int32_t dtype, int64_t tokens, int64_t top_k, int64_t cols, const void *x, int64_t x_row_stride,
+                                      const int32_t *slots, int64_t out_rows, void *out, int64_t out_row_stride, void *stream);
+/* out[t] = cast_rint( sum_j weights[t, j] * y[slots[t, j]] ), added in f32 in the order of j; masked choices add nothing
+ * (their weights and rows are not read), a token without choices gets zeros.  weights [tokens, top_k] contiguous, f32,
+ * f16 or bf16, or NULL for 1: then this is the gradient of bsir_expert_dispatch. */
+BSIR_API int32_t bsir_expert_combine(int32_t dtype, int64_t tokens, int64_t top_k, int64_t cols, int64_t y_rows, const void *y,
+                                     int64_t y_row_stride, const int32_t *slots, int32_t weight_dtype, const void *weights, void *out,
+                                     int64_t out_row_stride, void *stream);
+/* The gradient of bsir_expert_combine: dy[slots[t, j]] = cast_rint( weights[t, j] * dout[t] ),
+ * dweights[t, j] = sum_c dout[t, c] * y[slots[t, j], c] (f32; 0 for a masked choice).  Rows of dy that no choice names are
+ * left as they were; no two choices may name one row. */
+BSIR_API int32_t bsir_expert_combine_grad(int32_t dtype, int64_t tokens, int64_t top_k, int64_t cols, int64_t y_rows, const void *dout,
+                                          int64_t dout_row_stride, const void *y, int64_t y_row_stride, const int32_t *slots,
+                                          int32_t weight_dtype, const void *weights, void *dy, int64_t dy_row_stride, float *dweights,
+                                          void *stream);
+
+/* ------------------------------------------------------------------------ */
 /* B2: compiled-kernel ABI                                                   */
 /* ------------------------------------------------------------------------ */
 typedef enum {

@@ -1,0 +1,278 @@
+"""GPU: tokens sorted by expert and back, with weights and gradients, against plain loops in 64 bits; and a whole
+mixture-of-experts layer made of the library's calls."""
+import numpy as np
+import pytest
+import torch
+
+import mxfp4_reference as R
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def B():
+    import bsir
+    bsir.lib()
+    yield bsir
+    assert bsir.device_error() == 0
+
+
+def _ids(tokens, top_k, experts, seed, masked=0.2, skew=False):
+    g = torch.Generator().manual_seed(seed)
+    ids = torch.randint(0, experts, (tokens, top_k), generator=g)
+    if skew:
+        ids = torch.minimum(ids, torch.randint(0, experts, (tokens, top_k), generator=g) // 3)
+    drop = torch.rand(tokens, top_k, generator=g)
+    ids[drop < masked / 2] = -1
+    ids[drop > 1 - masked / 2] = experts + 3                           # another rank's
+    return ids
+
+
+SORTS = [(1, 1, 1), (1, 8, 256), (7, 3, 5), (32, 4, 64), (512, 8, 8), (513, 8, 60), (1000, 5, 1024), (4096, 1, 2), (9001, 6, 128), (70000, 8, 33)]
+
+
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("tokens,top_k,experts", SORTS)
+def test_sort(B, tokens, top_k, experts, wide):
+    ids = _ids(tokens, top_k, experts, tokens, skew=tokens > 1000)
+    wo, wsl = R.sort(ids.tolist(), experts)
+    off, slots = B.expert_sort(ids.cuda() if wide else ids.int().cuda(), experts)
+    assert np.array_equal(off.cpu().numpy(), wo) and np.array_equal(slots.cpu().numpy(), wsl)
+
+
+def test_sort_extremes(B):
+    off, slots = B.expert_sort(torch.full((5000, 2), -1, dtype=torch.int64, device="cuda"), 4)
+    assert (off == 0).all() and (slots == -1).all()
+    off, slots = B.expert_sort(torch.full((5000, 2), 3, dtype=torch.int32, device="cuda"), 4)
+    assert off.tolist() == [0, 0, 0, 0, 10000] and torch.equal(slots.flatten().cpu(), torch.arange(10000, dtype=torch.int32))
+    off, slots = B.expert_sort(torch.zeros((0, 2), dtype=torch.int32, device="cuda"), 3)
+    assert off.tolist() == [0, 0, 0, 0]
+    big = torch.tensor([[1 << 40, -(1 << 40), 1]], dtype=torch.int64, device="cuda")      # must not wrap into an expert
+    assert B.expert_sort(big, 2)[1].tolist() == [[-1, -1, 0]]
+
+
+CASES = [(1, 1, 1, 1), (1, 2, 4, 8), (3, 2, 4, 33), (40, 4, 8, 4096), (17, 8, 16, 1000), (65, 6, 7, 514), (300, 9, 40, 72), (5, 16, 64, 12288)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16, torch.uint8, torch.int64])
+@pytest.mark.parametrize("tokens,top_k,experts,cols", CASES)
+def test_dispatch(B, tokens, top_k, experts, cols, dtype):
+    _, slots = R.sort(_ids(tokens, top_k, experts, cols).tolist(), experts)
+    x = torch.randint(0, 200, (tokens, cols), generator=torch.Generator().manual_seed(1)).to(dtype)
+    rows = tokens * top_k
+    out = torch.full((rows + 1, cols), 77, dtype=dtype, device="cuda")
+    B.expert_dispatch(x.cuda(), torch.from_numpy(slots).cuda(), out=out)
+    want = torch.full((rows + 1, cols), 77, dtype=dtype)
+    for t in range(tokens):
+        for j in range(top_k):
+            if slots[t, j] >= 0:
+                want[slots[t, j]] = x[t]
+    assert torch.equal(out.cpu(), want)
+
+
+def _layer(tokens, top_k, experts, cols, dtype, wdtype, seed):
+    g = torch.Generator().manual_seed(seed)
+    _, slots = R.sort(_ids(tokens, top_k, experts, seed).tolist(), experts)
+    rows = tokens * top_k
+    y = torch.randn(rows, cols, generator=g).to(dtype)
+    used = set(slots[slots >= 0].tolist())
+    for r in range(rows):
+        if r not in used:
+            y[r] = float("nan")                                        # nobody's rows are not read
+    w = torch.randn(tokens, top_k, generator=g).to(wdtype)
+    w[torch.from_numpy(slots) < 0] = float("nan")                     # nor masked choices' weights
+    dout = torch.randn(tokens, cols, generator=g).to(dtype)
+    return slots, y, w, dout
+
+
+@pytest.mark.parametrize("wdtype", [torch.float32, torch.bfloat16, torch.float16, None])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("tokens,top_k,experts,cols", CASES)
+def test_combine_and_gradient(B, tokens, top_k, experts, cols, dtype, wdtype):
+    slots, y, w, dout = _layer(tokens, top_k, experts, cols, dtype, wdtype or torch.float32, cols + top_k)
+    rows = y.shape[0]
+    yd, gd = y.double().numpy(), dout.double().numpy()
+    wd = w.double().numpy() if wdtype else np.ones((tokens, top_k))
+    out, mag = np.zeros((tokens, cols)), np.zeros((tokens, cols))
+    dy, dw, dmag = np.full((rows, cols), 9.0), np.zeros((tokens, top_k)), np.zeros((tokens, top_k))
+    for t in range(tokens):
+        for j in range(top_k):
+            s = slots[t, j]
+            if s < 0:
+                continue
+            out[t] += wd[t, j] * yd[s]
+            mag[t] += np.abs(wd[t, j] * yd[s])
+            dy[s] = wd[t, j] * gd[t]
+            dw[t, j] = (gd[t] * yd[s]).sum()
+            dmag[t, j] = np.abs(gd[t] * yd[s]).sum()
+    half = torch.finfo(dtype).eps / 2
+    tiny = float(torch.finfo(dtype).smallest_normal)
+    sl = torch.from_numpy(slots).cuda()
+    wc = w.cuda() if wdtype else None
+    got = B.expert_combine(y.cuda(), sl, wc).cpu().double().numpy()
+    # one f32 rounding a term (2^-24 of a partial sum, at most the magnitudes' sum), then C's
+    assert (np.abs(got - out) <= top_k * 2.0 ** -24 * mag * 1.01 + half * np.abs(out) * 1.001 + tiny * half).all()
+    dy0 = torch.full((rows, cols), 9.0, dtype=dtype, device="cuda")
+    gy, gw = B.expert_combine_grad(dout.cuda(), y.cuda(), sl, wc, out=dy0)
+    # the f32 product's rounding, then dy's
+    assert (np.abs(gy.cpu().double().numpy() - dy) <= (half + 2.0 ** -24) * 1.001 * np.abs(dy) + tiny * half).all()
+    # a dot product of `cols` terms, each addition off by 2^-24 of at most the magnitudes' sum
+    assert (np.abs(gw.cpu().double().numpy() - dw) <= cols * 2.0 ** -24 * 1.01 * dmag).all()
+    assert (gw.cpu()[torch.from_numpy(slots) < 0] == 0).all()
+
+
+def test_dispatch_gradient_is_combine_without_weights(B):
+    """<dispatch(x), g> = <x, combine(g)> for integer data, hence by linearity its gradient; with differences of the former."""
+    tokens, top_k, experts, cols = 20, 3, 5, 64
+    _, slots = B.expert_sort(_ids(tokens, top_k, experts, 4).cuda(), experts)
+    g = torch.Generator().manual_seed(0)
+    x = torch.randint(-4, 5, (tokens, cols), generator=g).float().cuda()
+    gr = torch.randint(-4, 5, (tokens * top_k, cols), generator=g).float().cuda()
+    dx = B.expert_combine(gr, slots)
+    f = lambda v: (B.expert_dispatch(v, slots) * gr).sum().item()
+    assert f(x) == (x * dx).sum().item()
+    for t, c in ((0, 0), (7, 63), (19, 5)):
+        x1 = x.clone()
+        x1[t, c] += 1
+        assert f(x1) - f(x) == dx[t, c].item()
+
+
+def test_strided_and_unaligned_rows(B):
+    tokens, top_k, cols = 12, 2, 40
+    _, slots = B.expert_sort(_ids(tokens, top_k, 4, 9).cuda(), 4)
+    base = torch.randn(tokens, cols + 7, device="cuda").to(torch.bfloat16)
+    x = base[:, 3:3 + cols]
+    out = torch.zeros(tokens * top_k, cols + 5, dtype=torch.bfloat16, device="cuda")
+    B.expert_dispatch(x, slots, out=out[:, 1:1 + cols])
+    want = B.expert_dispatch(x.contiguous(), slots)
+    assert torch.equal(out[:, 1:1 + cols], want) and (out[:, 0] == 0).all() and (out[:, 1 + cols:] == 0).all()
+    w = torch.rand(tokens, top_k, device="cuda")
+    comb = torch.zeros(tokens, cols + 3, dtype=torch.bfloat16, device="cuda")
+    B.expert_combine(out[:, 1:1 + cols], slots, w, out=comb[:, 2:2 + cols])
+    assert torch.equal(comb[:, 2:2 + cols], B.expert_combine(want, slots, w)) and (comb[:, :2] == 0).all()
+    dy, dw = B.expert_combine_grad(x, out[:, 1:1 + cols], slots, w, out=torch.zeros_like(out)[:, 1:1 + cols])
+    dy2, dw2 = B.expert_combine_grad(x.contiguous(), want, slots, w)
+    assert torch.equal(dy, dy2)
+    assert (dw - dw2).abs().max() <= 2 * cols * 2.0 ** -24 * (x.float().abs().amax() * want.float().abs().amax() * cols)
+
+
+def test_bad_slots_are_masked_and_reported(B):
+    x = torch.ones(3, 8, device="cuda")
+    slots = torch.tensor([[0, 99], [-5, 1], [2, -1]], dtype=torch.int32, device="cuda")
+    out = B.expert_dispatch(x, slots, out=torch.zeros(4, 8, device="cuda"))
+    assert out.sum(1).tolist() == [8, 8, 8, 0]
+    assert B.device_error() == 0x100
+    assert B.expert_combine(out, slots).sum(1).tolist() == [8, 8, 8]
+    assert B.device_error() == 0x100
+    dy, dw = B.expert_combine_grad(x, out, slots)
+    assert dw.tolist() == [[8, 0], [0, 8], [8, 0]] and dy.sum(1).tolist() == [8, 8, 8, 0]
+    assert B.device_error() == 0x100
+
+
+def test_empty(B):
+    e = lambda *s: torch.zeros(*s, device="cuda")
+    no = torch.zeros(0, 2, dtype=torch.int32, device="cuda")
+    assert tuple(B.expert_dispatch(e(0, 8), no).shape) == (0, 8)
+    assert tuple(B.expert_combine(e(5, 8), no).shape) == (0, 8)
+    none = torch.full((3, 2), -1, dtype=torch.int32, device="cuda")
+    assert (B.expert_combine(e(0, 8), none) == 0).all()
+    dy, dw = B.expert_combine_grad(e(3, 8) + 1, e(6, 8) + 1, none)
+    assert (dy == 0).all() and (dw == 0).all()
+    assert tuple(B.expert_combine(e(4, 8), torch.zeros(3, 0, dtype=torch.int32, device="cuda")).shape) == (3, 8)
+
+
+def _moe(B, x, ids, w, w1, w2, experts, hidden):
+    """A feed-forward layer of experts: sort, quantise once per token, dispatch codes and exponents, product, relu,
+    quantise, product, combine."""
+    off, slots = B.expert_sort(ids, experts)
+    q, s = B.quant_mxfp4(x)
+    rows = ids.numel()
+    qr = torch.zeros(rows, q.stride(0), dtype=torch.uint8, device="cuda")[:, :q.shape[1]]
+    sr = torch.zeros(rows, s.stride(0), dtype=torch.uint8, device="cuda")[:, :s.shape[1]]
+    B.expert_dispatch(q, slots, out=qr)
+    B.expert_dispatch(s, slots, out=sr)
+    h = torch.zeros(rows, hidden, dtype=torch.bfloat16, device="cuda")
+    B.matmul_mxfp4(qr, sr, *w1, offsets=off, out=h)
+    h = B.elemwise_unary("relu", h)
+    hq, hs = B.quant_mxfp4(h)
+    y = torch.zeros(rows, x.shape[1], dtype=torch.bfloat16, device="cuda")
+    B.matmul_mxfp4(hq, hs, *w2, offsets=off, out=y)
+    return off, slots, qr, sr, h, y, B.expert_combine(y, slots, w)
+
+
+def _expert_weights(B, experts, n, k, seed):
+    g = torch.Generator().manual_seed(seed)
+    flat = (torch.randn(experts * n, k, generator=g) * 0.05).to(torch.bfloat16).cuda()
+    q, s = B.quant_mxfp4(flat)
+    cut = lambda t: t.as_strided((experts, n, t.shape[1]), (n * t.stride(0), t.stride(0), 1))
+    return flat, (cut(q), cut(s))
+
+
+@pytest.mark.parametrize("tokens,top_k,experts,cols,hidden", [(3, 2, 4, 256, 320), (64, 4, 8, 512, 288), (600, 2, 4, 320, 1024)])
+def test_layer(B, tokens, top_k, experts, cols, hidden):
+    g = torch.Generator().manual_seed(tokens)
+    x = torch.randn(tokens, cols, generator=g).to(torch.bfloat16).cuda()
+    ids = _ids(tokens, top_k, experts, tokens + 1).cuda()
+    w = torch.rand(tokens, top_k, generator=g).cuda()
+    _, w1 = _expert_weights(B, experts, hidden, cols, 1)
+    _, w2 = _expert_weights(B, experts, cols, hidden, 2)
+    off, slots, qr, sr, h, y, out = _moe(B, x, ids, w, w1, w2, experts, hidden)
+    wo, wsl = R.sort(ids.tolist(), experts)
+    assert np.array_equal(off.cpu().numpy(), wo) and np.array_equal(slots.cpu().numpy(), wsl)
+    xv = R.quant(x)[2]
+    half = torch.finfo(torch.bfloat16).eps / 2
+    for e in range(experts):
+        w1v = R.decode(w1[0][e], w1[1][e], cols)
+        w2v = R.decode(w2[0][e], w2[1][e], hidden)
+        for t, j in np.argwhere(ids.cpu().numpy() == e)[:40]:
+            r = wsl[t, j]
+            ref = xv[t] @ w1v.T
+            tol = R.product_tolerance(xv[t:t + 1], w1v, cols, torch.bfloat16)(ref[None])[0]
+            got = h[r].cpu().double().numpy()
+            assert (np.abs(got - np.maximum(ref, 0)) <= tol).all()
+            hv = R.quant(h[r:r + 1])[2]                                # from the layer's own intermediate, as rounded there
+            ref = hv @ w2v.T
+            assert (np.abs(y[r].cpu().double().numpy() - ref) <= R.product_tolerance(hv, w2v, hidden, torch.bfloat16)(ref)).all()
+    yd, wd = y.cpu().double().numpy(), w.cpu().double().numpy()
+    for t in range(tokens):
+        live = wsl[t] >= 0
+        terms = wd[t][live, None] * yd[wsl[t][live]]
+        ref = terms.sum(0)
+        assert (np.abs(out[t].cpu().double().numpy() - ref) <= half * np.abs(ref) * 1.001 + top_k * 2.0 ** -23 * np.abs(terms).sum(0)).all()
+
+
+def test_layer_captured_and_replayed(B):
+    tokens, top_k, experts, cols, hidden = 16, 2, 4, 256, 256
+    x = torch.randn(tokens, cols, device="cuda").to(torch.bfloat16)
+    ids = _ids(tokens, top_k, experts, 3).cuda()
+    w = torch.rand(tokens, top_k, device="cuda")
+    _, w1 = _expert_weights(B, experts, hidden, cols, 1)
+    _, w2 = _expert_weights(B, experts, cols, hidden, 2)
+    _moe(B, x, ids, w, w1, w2, experts, hidden)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        res = _moe(B, x, ids, w, w1, w2, experts, hidden)
+    for seed in (5, 6):
+        ids.copy_(_ids(tokens, top_k, experts, seed))
+        x.copy_(torch.randn(tokens, cols, generator=torch.Generator().manual_seed(seed)))
+        graph.replay()
+        got = [t.clone() for t in res]
+        want = _moe(B, x, ids, w, w1, w2, experts, hidden)
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+
+
+def test_two_streams_at_once(B):
+    """Long sorts take scratch: each stream its own."""
+    ids = [_ids(20000, 4, 64, s).cuda() for s in (1, 2)]
+    want = [R.sort(i.tolist(), 64) for i in ids]
+    streams = [torch.cuda.Stream() for _ in ids]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        got = []
+        for st, i in zip(streams, ids):
+            with torch.cuda.stream(st):
+                got.append(B.expert_sort(i, 64))
+        torch.cuda.synchronize()
+        for (o, s), (wo, ws) in zip(got, want):
+            assert np.array_equal(o.cpu().numpy(), wo) and np.array_equal(s.cpu().numpy(), ws)
