@@ -15,10 +15,14 @@
 //   warp 1      MMA issuer
 //   warps 2-5   epilogue: accumulator -> bias -> rounding -> C
 //   warps 6-9   exponents into tensor memory, two buffers
-// Few rows run with the operands swapped: 128 rows of B are the instruction's M side and BN rows of A its N side, so
-// that a tile of weights is streamed for as few as 16 rows of A.
-#include <mutex>
-
+// in three forms:
+//   kPair    256 rows of A x BN columns of C on two CTAs (cta_group::2): each holds its 128 rows of A and half of the
+//            tile's rows of B, so that an SM's shared memory is read and filled for B half as often;
+//   kSingle  128 rows x BN columns on one CTA, for groups that would leave much of a 256-row tile empty;
+//   kFew     operands swapped: 128 rows of B are the instruction's M side and BN rows of A its N side, so that weights
+//            are streamed for as few as 16 rows of A.  With few tiles a cluster of up to eight CTAs shares a tile's K:
+//            every CTA hands each other one that CTA's part of its partial tile through distributed shared memory,
+//            and the parts are added in the order of the CTAs (the same bits on every run).
 #include "tc_ptx.cuh"
 
 namespace bsir {
@@ -26,9 +30,9 @@ namespace {
 
 constexpr int kTileM = 128;
 constexpr int kStageK = 256;       // elements of K a stage: one 128-byte swizzle row of codes
-constexpr int kChunkK = 512;       // elements of K of a 16-byte piece of exponents
 constexpr int kThreads = 320;
 constexpr int kMaxGroups = 1024;
+enum MxMode { kSingle, kPair, kFew };
 
 struct MxParams {
   int64_t m, n;
@@ -41,36 +45,55 @@ struct MxParams {
   void *out;
   int64_t ldo;
   int *err;
+  int tma_out;                     // 1: C's rows can be written by TMA, 2: at least in 16-byte pieces, 0: neither
+  int split;                       // kFew: CTAs that share a tile's K (a cluster)
 };
 
-template <int BN>
+template <int BN, int MODE>
 struct MxCfg {
-  static constexpr int kStage = (kTileM + BN) * 128;
-  static constexpr int kStages = BN >= 256 ? 4 : BN >= 128 ? 6 : BN >= 64 ? 7 : 9;
+  static constexpr int kNRows = MODE == kPair ? BN / 2 : BN;         // rows of the N side's codes in this CTA
+  static constexpr int kStage = (kTileM + kNRows) * 128;
   static constexpr int kSfStage = (kTileM + BN) * 16;
-  static constexpr int kSfStages = 4;
-  static constexpr int kAccs = BN >= 256 ? 1 : 2;
+  static constexpr int kSfStages = 3;
+  static constexpr int kAccs = BN > 192 ? 1 : 2;
   // columns of tensor memory: accumulators, then two buffers of 4 x (4 + kSfN) cells of exponents
-  static constexpr int kSfN = BN >= 128 ? BN / 32 : 4;
+  static constexpr int kSfN = BN > 128 ? 8 : 4;
   static constexpr int kSfCols = 4 * (4 + kSfN);
   static constexpr int kSfBase = kAccs * BN;
   static constexpr int kCols = kSfBase + 2 * kSfCols;
   static constexpr int kTmemCols = kCols <= 128 ? 128 : kCols <= 256 ? 256 : 512;
+  // staging: two buffers of 32 rows x 128 bytes of C a warp, or the partial tiles of a cluster
+  static constexpr int kEpi = MODE == kFew ? BN * kTileM * 4 : 4 * 2 * 4096;
+  static constexpr int kTable = 2 * (kMaxGroups + 1) * 4;
+  static constexpr int kFixed = kSfStages * kSfStage + kEpi + 512 /*barriers*/ + kTable + 1024 /*alignment*/;
+  static constexpr int kFit = (227 * 1024 - kFixed) / kStage;
+  static constexpr int kStages = kFit > 9 ? 9 : kFit;
   static constexpr int kSfOff = kStages * kStage;
-  static constexpr int kBarOff = kSfOff + kSfStages * kSfStage;
-  static constexpr int kTableOff = kBarOff + 512;                    // tiles before a group; first row and end of each
-  static constexpr int kSmem = kTableOff + (3 * kMaxGroups + 1) * 4 + 1024 /*alignment*/;
+  static constexpr int kEpiOff = (kSfOff + kSfStages * kSfStage + 1023) / 1024 * 1024;    // 128-byte swizzle
+  static constexpr int kBarOff = kEpiOff + kEpi;
+  static constexpr int kTableOff = kBarOff + 512;                    // tiles before a group, first row of a group
+  static constexpr int kSmem = kTableOff + kTable + 1024;
   static_assert(kCols <= 512, "tensor memory");
-  static_assert(kSmem <= 227 * 1024, "shared memory");
+  static_assert(kStages >= 4 && kSmem <= 227 * 1024, "shared memory");
 };
 
+template <int MODE>
 __device__ __forceinline__ void mma_mxf4(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %6, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(tmem_d),
-      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
-      : "memory");
+  if constexpr (MODE == kPair) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(tmem_d),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        : "memory");
+  } else {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(tmem_d),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        : "memory");
+  }
 }
 // e2m1 x e2m1, exponents E8M0, both K-major; `sf_id` (0 or 2): which two of a cell's four bytes belong to these 64
 // elements of K
@@ -84,6 +107,16 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t *r) {
       "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
+__device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap *map, int x, int y, int z, uint32_t leader_bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(leader_bar)
+      : "memory");
+}
+__device__ __forceinline__ void st_cluster_f32(uint32_t cluster_addr, uint32_t bits) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr), "r"(bits) : "memory");
+}
+__device__ __forceinline__ void fence_cluster() { asm volatile("fence.acq_rel.cluster;" ::: "memory"); }
 
 __device__ __forceinline__ float load_float(const void *p, int32_t dtype, int64_t i) {
   if (dtype == BSIR_F32) return static_cast<const float *>(p)[i];
@@ -96,15 +129,15 @@ __device__ __forceinline__ void store_out(const MxParams &p, int64_t at, float f
   else static_cast<__nv_bfloat16 *>(p.out)[at] = __float2bfloat16_rn(f);
 }
 
-// Where a tile lies: `tile_start[g]` tiles come before group g; within a group the row tiles run fastest, so that
-// CTAs working at the same time share columns of B.
+// Where a tile lies: `tile_start[g]` tiles come before group g, whose rows begin at row_start[g]; within a group the
+// row tiles run fastest, so that CTAs working at the same time share rows of B.
 struct MxTile {
   int group, row0, row_end, n0;
 };
 template <int ROWS, int COLS>
 __device__ __forceinline__ void find_tile(int tile, const int *tile_start, const int *row_start, int &group, MxTile &t) {
   while (tile >= tile_start[group + 1]) ++group;            // a role's tiles only go up
-  const int first = row_start[2 * group], end = row_start[2 * group + 1];
+  const int first = row_start[group], end = row_start[group + 1];
   const int row_tiles = (end - first + ROWS - 1) / ROWS;
   const int local = tile - tile_start[group];
   t.group = group;
@@ -113,12 +146,102 @@ __device__ __forceinline__ void find_tile(int tile, const int *tile_start, const
   t.n0 = (local / row_tiles) * COLS;
 }
 
-template <int BN, bool SWAP>
+// One epilogue warp's 32 rows x BN columns of an accumulator -> C.  128 bytes of each row at a time are staged in
+// shared memory with the 128-byte swizzle and leave through a TMA store; where that cannot be (rows behind the group's
+// end in the box, C's rows not 16-byte aligned) the warp stores them itself, row by row.
+template <int BN>
+__device__ __forceinline__ void store_rows(const MxParams &p, const CUtensorMap *tmap_out, uint32_t acc, const MxTile &t, int row0, int lane,
+                                           uint8_t *stage, uint32_t stage_addr, uint32_t &nstores) {
+  const bool wide = p.out_dtype == BSIR_F32;
+  const int eb = wide ? 4 : 2, step = wide ? 32 : 64;        // columns of a 128-byte piece
+  const bool by_tma = p.tma_out == 1 && (row0 + 32 <= t.row_end || t.row_end == p.m);   // behind the last row nothing is written
+  const int rows = t.row_end - row0 < 32 ? t.row_end - row0 : 32;
+  for (int c0 = 0; c0 < BN; c0 += step) {
+    const int64_t col0 = t.n0 + c0;
+    if (col0 >= p.n) break;
+    const uint32_t b = nstores & 1u;
+    if (by_tma) {      // the store that read this buffer two pieces ago must have read it
+      if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+    }
+    __syncwarp();
+    uint8_t *buf = stage + b * 4096, *mine = buf + lane * 128;
+    const uint32_t sw = static_cast<uint32_t>(lane & 7);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {                            // 32 columns each
+      if (h == 1 && (wide || BN - c0 <= 32)) break;
+      uint32_t r[32];
+      tmem_ld32(acc + static_cast<uint32_t>(c0 + 32 * h), r);
+      tmem_ld_wait();
+      if (p.bias) {
+        const int64_t col = col0 + 32 * h + lane;
+        const float mine_b = col < p.n ? load_float(p.bias, p.bias_dtype, t.group * p.bias_stride + col) : 0.0f;
+#pragma unroll
+        for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__fadd_rn(__uint_as_float(r[j]), __shfl_sync(0xffffffffu, mine_b, j)));
+      }
+      if (wide) {
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+          *reinterpret_cast<uint4 *>(mine + ((c ^ sw) * 16)) = make_uint4(r[4 * c], r[4 * c + 1], r[4 * c + 2], r[4 * c + 3]);
+      } else {
+        uint32_t w[16];
+        if (p.out_dtype == BSIR_F16) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) w[j] = pack_f16x2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]));
+        } else {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) w[j] = pack_bf16x2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]));
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          *reinterpret_cast<uint4 *>(mine + (((4 * h + c) ^ sw) * 16)) = make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+      }
+    }
+    if (by_tma) {
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) tma_store_2d(tmap_out, static_cast<int>(col0) * eb, row0, stage_addr + b * 4096);
+      ++nstores;
+    } else {
+      __syncwarp();
+      const int64_t left = (p.n - col0) * eb;                // bytes of a row from here on
+      const int have = static_cast<int>(left < 128 ? left : 128) < (BN - c0) * eb ? static_cast<int>(left < 128 ? left : 128) : (BN - c0) * eb;
+      if (p.tma_out) {                                       // eight lanes a row, four rows at a time
+        const int piece = lane & 7;
+        for (int r = lane >> 3; r < rows; r += 4) {
+          const uint4 v = *reinterpret_cast<const uint4 *>(buf + r * 128 + ((piece ^ (r & 7)) * 16));
+          char *dst = static_cast<char *>(p.out) + ((row0 + r) * p.ldo + col0) * eb + piece * 16;
+          if (piece * 16 + 16 <= have) {
+            *reinterpret_cast<uint4 *>(dst) = v;
+          } else {
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+            for (int i = 0; i < 16 && piece * 16 + i < have; i += eb) {
+              if (wide) *reinterpret_cast<uint32_t *>(dst + i) = w[i / 4];
+              else *reinterpret_cast<uint16_t *>(dst + i) = static_cast<uint16_t>(w[i / 4] >> (8 * (i & 2)));
+            }
+          }
+        }
+      } else {
+        for (int r = 0; r < rows; ++r) {
+          char *dst = static_cast<char *>(p.out) + ((row0 + r) * p.ldo + col0) * eb;
+          for (int i = lane * eb; i < have; i += 32 * eb) {
+            const uint8_t *src = buf + r * 128 + (((i >> 4) ^ (r & 7)) * 16) + (i & 15);
+            if (wide) *reinterpret_cast<uint32_t *>(dst + i) = *reinterpret_cast<const uint32_t *>(src);
+            else *reinterpret_cast<uint16_t *>(dst + i) = *reinterpret_cast<const uint16_t *>(src);
+          }
+        }
+      }
+    }
+  }
+}
+
+template <int BN, int MODE>
 __global__ void __launch_bounds__(kThreads, 1)
     mxfp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_m, const __grid_constant__ CUtensorMap tmap_n,
-                      const __grid_constant__ CUtensorMap tmap_sm, const __grid_constant__ CUtensorMap tmap_sn, MxParams p) {
-  using Cfg = MxCfg<BN>;
-  constexpr int kRows = SWAP ? BN : kTileM;       // rows of A and columns of C (rows of B) a tile
+                      const __grid_constant__ CUtensorMap tmap_sm, const __grid_constant__ CUtensorMap tmap_sn,
+                      const __grid_constant__ CUtensorMap tmap_out, MxParams p) {
+  using Cfg = MxCfg<BN, MODE>;
+  constexpr bool SWAP = MODE == kFew, PAIR = MODE == kPair;
+  constexpr int kRows = SWAP ? BN : PAIR ? 2 * kTileM : kTileM;       // rows of A and columns of C (rows of B) a tile
   constexpr int kColsC = SWAP ? kTileM : BN;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
@@ -134,55 +257,68 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto st_empty_bar = [&](int b) { return bars + 8u * (kB2 + 2 + b); };
   auto acc_full_bar = [&](int b) { return bars + 8u * (kB2 + 4 + b); };
   auto acc_empty_bar = [&](int b) { return bars + 8u * (kB2 + 6 + b); };
-  static_assert(8 * (kB2 + 8) + 16 <= 512, "barriers");
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(gen + Cfg::kBarOff + 8 * (kB2 + 8));
+  const uint32_t red_full = bars + 8u * (kB2 + 8), red_empty = bars + 8u * (kB2 + 9);   // partial tiles of the cluster
+  static_assert(8 * (kB2 + 10) + 16 <= 512, "barriers");
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(gen + Cfg::kBarOff + 8 * (kB2 + 10));
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
   int *tile_start = reinterpret_cast<int *>(gen + Cfg::kTableOff);         // [groups + 1]
-  int *row_start = tile_start + kMaxGroups + 1;                            // [groups][2]: first row, end
+  int *row_start = tile_start + kMaxGroups + 1;                            // [groups + 1]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // CTAs that work on one tile: a pair (rows cut in two), a cluster that shares K, or one
+  const int team = PAIR ? 2 : SWAP ? p.split : 1;
+  const int rank = team > 1 ? static_cast<int>(cluster_rank()) : 0;
+  const int first_tile = blockIdx.x / team, tile_step = gridDim.x / team;
   pdl_launch_dependents();
   if (threadIdx.x == 0) {
     for (int s = 0; s < Cfg::kStages; ++s) { mbar_init(full_bar(s), 1); mbar_init(empty_bar(s), 1); }
     for (int s = 0; s < Cfg::kSfStages; ++s) { mbar_init(sf_full_bar(s), 1); mbar_init(sf_empty_bar(s), 4); }
     for (int b = 0; b < 2; ++b) {
-      mbar_init(st_full_bar(b), 4); mbar_init(st_empty_bar(b), 1);
-      mbar_init(acc_full_bar(b), 1); mbar_init(acc_empty_bar(b), 4);
+      mbar_init(st_full_bar(b), PAIR ? 8 : 4); mbar_init(st_empty_bar(b), 1);
+      mbar_init(acc_full_bar(b), 1); mbar_init(acc_empty_bar(b), PAIR ? 8 : 4);
     }
+    mbar_init(red_full, 4 * team);
+    mbar_init(red_empty, 4 * team);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     prefetch_tmap(&tmap_m); prefetch_tmap(&tmap_n); prefetch_tmap(&tmap_sm); prefetch_tmap(&tmap_sn);
   }
-  if (warp == 1) tmem_alloc(smem_u32(tmem_slot), Cfg::kTmemCols);
+  if (warp == 1) {
+    if constexpr (PAIR) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(Cfg::kTmemCols) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+      tmem_alloc(smem_u32(tmem_slot), Cfg::kTmemCols);
+    }
+  }
   pdl_wait();                       // no global memory is touched before this
-  if (warp == 2) {                  // the groups' rows (clamped to what exists) and tiles
+  if (warp == 2) {                  // the groups' first rows (clamped to what exists) and tiles
     const int col_tiles = static_cast<int>((p.n + kColsC - 1) / kColsC);
     int before = 0, reached = 0;
     for (int g0 = 0; g0 < p.groups; g0 += 32) {
       const int g = g0 + lane;
       // rows start where the largest offset so far says: groups never overlap, whatever the offsets hold
-      int64_t first = 0, end = p.m;
+      int first = 0, end = static_cast<int>(p.m);
       if (p.offsets) {
-        int64_t o = p.offsets[g < p.groups ? g : p.groups];
-        o = o < 0 ? 0 : o > p.m ? p.m : o;
-        int top = static_cast<int>(o);
+        auto offset = [&](int i) {
+          const int o = p.offsets[i < p.groups ? i : p.groups];
+          return o < 0 ? 0 : o > p.m ? static_cast<int>(p.m) : o;
+        };
+        first = offset(g);
 #pragma unroll
         for (int s = 1; s < 32; s <<= 1) {
-          const int up = __shfl_up_sync(0xffffffffu, top, s);
-          if (lane >= s) top = max(top, up);
+          const int up = __shfl_up_sync(0xffffffffu, first, s);
+          if (lane >= s) first = max(first, up);
         }
-        top = max(top, reached);
-        first = top;
-        int next = p.offsets[g + 1 < p.groups ? g + 1 : p.groups];
-        next = next < 0 ? 0 : next > p.m ? static_cast<int>(p.m) : next;
-        end = max(top, next);
-        reached = __shfl_sync(0xffffffffu, top, 31);
+        first = max(first, reached);
+        end = max(first, offset(g + 1));
+        reached = __shfl_sync(0xffffffffu, first, 31);
       }
       int tiles = 0;
       if (g < p.groups) {
-        row_start[2 * g] = static_cast<int>(first);
-        row_start[2 * g + 1] = static_cast<int>(end);
-        tiles = static_cast<int>((end - first + kRows - 1) / kRows) * col_tiles;
+        row_start[g] = first;
+        if (g == p.groups - 1) row_start[p.groups] = end;
+        tiles = ((end - first + kRows - 1) / kRows) * col_tiles;
       }
       int inc = tiles;
 #pragma unroll
@@ -197,10 +333,16 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   tc_fence_before();
   __syncthreads();
+  if (team > 1) cluster_sync_all();       // every CTA's barriers are initialised before anyone signals across
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   const int total_tiles = tile_start[p.groups];
-  const int chunks = (p.k_blocks + 1) / 2;
+  // this CTA's chunks of 512 elements of K
+  const int all_chunks = (p.k_blocks + 1) / 2;
+  const int per = SWAP ? (all_chunks + team - 1) / team : all_chunks;
+  const int chunk0 = SWAP ? rank * per : 0;
+  const int chunk1 = min(all_chunks, chunk0 + per);
+  const int kb0 = 2 * chunk0, kb1 = min(p.k_blocks, 2 * chunk1);
   int group = 0;
   MxTile t;
 
@@ -210,24 +352,32 @@ __global__ void __launch_bounds__(kThreads, 1)
       int stage = 0, sf = 0;
       uint32_t phase = 0, sf_phase = 0;
       bool ok = true;
-      for (int tile = blockIdx.x; tile < total_tiles && ok; tile += gridDim.x) {
+      for (int tile = first_tile; tile < total_tiles && ok; tile += tile_step) {
         find_tile<kRows, kColsC>(tile, tile_start, row_start, group, t);
-        const int m0 = SWAP ? t.n0 : t.row0, n0 = SWAP ? t.row0 : t.n0;
+        const int m0 = SWAP ? t.n0 : t.row0 + (PAIR ? rank * kTileM : 0);
+        const int n0 = SWAP ? t.row0 : t.n0 + (PAIR ? rank * Cfg::kNRows : 0);
         const int zm = SWAP ? t.group : 0, zn = SWAP ? 0 : t.group;
-        for (int kb = 0; kb < p.k_blocks; ++kb) {
+        for (int kb = kb0; kb < kb1; ++kb) {
           if ((kb & 1) == 0) {
             if (!mbar_wait(sf_empty_bar(sf), sf_phase ^ 1u, abort_flag, p.err)) { ok = false; break; }
             const uint32_t dst = base + Cfg::kSfOff + sf * Cfg::kSfStage;
             mbar_expect_tx(sf_full_bar(sf), Cfg::kSfStage);
             tma_load_3d(dst, &tmap_sm, kb * (kStageK / 32), m0, zm, sf_full_bar(sf));
-            tma_load_3d(dst + kTileM * 16, &tmap_sn, kb * (kStageK / 32), n0, zn, sf_full_bar(sf));
+            tma_load_3d(dst + kTileM * 16, &tmap_sn, kb * (kStageK / 32), SWAP ? t.row0 : t.n0, zn, sf_full_bar(sf));
             if (++sf == Cfg::kSfStages) { sf = 0; sf_phase ^= 1u; }
           }
           if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag, p.err)) { ok = false; break; }
           const uint32_t dst = base + stage * Cfg::kStage;
-          mbar_expect_tx(full_bar(stage), Cfg::kStage);
-          tma_load_3d(dst, &tmap_m, kb * 128, m0, zm, full_bar(stage));
-          tma_load_3d(dst + kTileM * 128, &tmap_n, kb * 128, n0, zn, full_bar(stage));
+          if constexpr (PAIR) {                       // both CTAs' bytes complete on the leader's barrier
+            const uint32_t leader = map_to_cta(full_bar(stage), 0);
+            if (rank == 0) mbar_expect_tx(full_bar(stage), 2 * Cfg::kStage);
+            tma_load_3d_pair(dst, &tmap_m, kb * 128, m0, zm, leader);
+            tma_load_3d_pair(dst + kTileM * 128, &tmap_n, kb * 128, n0, zn, leader);
+          } else {
+            mbar_expect_tx(full_bar(stage), Cfg::kStage);
+            tma_load_3d(dst, &tmap_m, kb * 128, m0, zm, full_bar(stage));
+            tma_load_3d(dst + kTileM * 128, &tmap_n, kb * 128, n0, zn, full_bar(stage));
+          }
           if (++stage == Cfg::kStages) { stage = 0; phase ^= 1u; }
         }
       }
@@ -241,39 +391,43 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
   } else if (warp == 1) {
-    // ---------------- MMA issuer
-    if (lane == 0) {
-      const uint32_t idesc0 = mx_idesc(BN, kTileM, 0), idesc2 = mx_idesc(BN, kTileM, 2);
+    // ---------------- MMA issuer (the pair's leader only)
+    if (lane == 0 && (!PAIR || rank == 0)) {
+      const uint32_t idesc0 = mx_idesc(BN, PAIR ? 256 : 128, 0), idesc2 = mx_idesc(BN, PAIR ? 256 : 128, 2);
+      auto commit = [&](uint32_t bar) {
+        if constexpr (PAIR) tc_commit_pair(bar);
+        else tc_commit(bar);
+      };
       int stage = 0, b = 0, acc = 0;
       uint32_t phase = 0, b_phase = 0, acc_phase = 0;
       bool ok = true;
-      for (int tile = blockIdx.x; tile < total_tiles && ok; tile += gridDim.x) {
+      for (int tile = first_tile; tile < total_tiles && ok; tile += tile_step) {
         if (!mbar_wait(acc_empty_bar(acc), acc_phase ^ 1u, abort_flag, p.err)) break;
         tc_fence_after();
         const uint32_t d = tmem + static_cast<uint32_t>(acc * BN);
-        for (int c = 0; c < chunks && ok; ++c) {
+        for (int c = chunk0; c < chunk1 && ok; ++c) {
           if (!mbar_wait(st_full_bar(b), b_phase, abort_flag, p.err)) { ok = false; break; }
           const uint32_t sf = tmem + static_cast<uint32_t>(Cfg::kSfBase + b * Cfg::kSfCols);
-          for (int h = 0; h < 2 && 2 * c + h < p.k_blocks; ++h) {
+          for (int h = 0; h < 2 && 2 * c + h < kb1; ++h) {
             if (!mbar_wait(full_bar(stage), phase, abort_flag, p.err)) { ok = false; break; }
             tc_fence_after();
             const uint32_t sm = base + stage * Cfg::kStage, sn = sm + kTileM * 128;
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk) {
               const uint32_t cell = static_cast<uint32_t>(2 * h + (kk >> 1));
-              mma_mxf4(d, make_desc(sm + kk * 32, 16, 1024), make_desc(sn + kk * 32, 16, 1024), (kk & 1) ? idesc2 : idesc0, sf + cell * 4,
-                       sf + 16 + cell * Cfg::kSfN, (c | h | kk) ? 1u : 0u);
+              mma_mxf4<MODE>(d, make_desc(sm + kk * 32, 16, 1024), make_desc(sn + kk * 32, 16, 1024), (kk & 1) ? idesc2 : idesc0, sf + cell * 4,
+                             sf + 16 + cell * Cfg::kSfN, (c > chunk0 || h > 0 || kk > 0) ? 1u : 0u);
             }
-            tc_commit(empty_bar(stage));
+            commit(empty_bar(stage));
             if (++stage == Cfg::kStages) { stage = 0; phase ^= 1u; }
           }
           if (!ok) break;
-          tc_commit(st_empty_bar(b));
+          commit(st_empty_bar(b));
           b ^= 1;
           if (b == 0) b_phase ^= 1u;
         }
         if (!ok) break;
-        tc_commit(acc_full_bar(acc));
+        commit(acc_full_bar(acc));
         if (++acc == Cfg::kAccs) { acc = 0; acc_phase ^= 1u; }
       }
     }
@@ -283,8 +437,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     int sf = 0, b = 0;
     uint32_t sf_phase = 0, b_phase = 0;
     bool ok = true;
-    for (int tile = blockIdx.x; tile < total_tiles && ok; tile += gridDim.x) {
-      for (int c = 0; c < chunks; ++c) {
+    for (int tile = first_tile; tile < total_tiles && ok; tile += tile_step) {
+      for (int c = chunk0; c < chunk1; ++c) {
         if (!mbar_wait(sf_full_bar(sf), sf_phase, abort_flag, p.err)) { ok = false; break; }
         const uint4 *src = reinterpret_cast<const uint4 *>(gen + Cfg::kSfOff + sf * Cfg::kSfStage);
         uint32_t rm[16], rn[4 * Cfg::kSfN];
@@ -295,8 +449,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
 #pragma unroll
         for (int j = 0; j < Cfg::kSfN; ++j) {
-          const bool have = j * 32 + lane < BN;
-          const uint4 w = have ? src[kTileM + j * 32 + lane] : make_uint4(0, 0, 0, 0);
+          const uint4 w = j * 32 + lane < BN ? src[kTileM + j * 32 + lane] : make_uint4(0, 0, 0, 0);
           rn[j] = w.x; rn[Cfg::kSfN + j] = w.y; rn[2 * Cfg::kSfN + j] = w.z; rn[3 * Cfg::kSfN + j] = w.w;
         }
         __syncwarp();
@@ -306,16 +459,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_after();
         const uint32_t dst = tmem + quad + static_cast<uint32_t>(Cfg::kSfBase + b * Cfg::kSfCols);
         tmem_st16(dst, rm);
-        if constexpr (Cfg::kSfN == 4) {
-          tmem_st16(dst + 16, rn);
-        } else {
-          static_assert(Cfg::kSfN == 4 || Cfg::kSfN == 8, "columns of the N side's exponents");
-          tmem_st32(dst + 16, rn);
-        }
+        if constexpr (Cfg::kSfN == 4) tmem_st16(dst + 16, rn);
+        else tmem_st32(dst + 16, rn);
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(st_full_bar(b));
+        if (lane == 0) {
+          if constexpr (PAIR) mbar_arrive_cluster(map_to_cta(st_full_bar(b), 0));
+          else mbar_arrive(st_full_bar(b));
+        }
         b ^= 1;
         if (b == 0) b_phase ^= 1u;
       }
@@ -323,51 +475,86 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else {
     // ---------------- epilogue
     const int quad = warp & 3;
+    uint8_t *stage = gen + Cfg::kEpiOff + (warp - 2) * 8192;
+    const uint32_t stage_addr = base + Cfg::kEpiOff + (warp - 2) * 8192;
     int acc = 0;
-    uint32_t acc_phase = 0;
-    for (int tile = blockIdx.x; tile < total_tiles; tile += gridDim.x) {
+    uint32_t acc_phase = 0, red_phase = 0, nstores = 0;
+    bool ok = true;
+    for (int tile = first_tile; tile < total_tiles && ok; tile += tile_step) {
       find_tile<kRows, kColsC>(tile, tile_start, row_start, group, t);
       if (!mbar_wait(acc_full_bar(acc), acc_phase, abort_flag, p.err)) break;
       tc_fence_after();
       const uint32_t src = tmem + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>(acc * BN);
-      const int64_t bias0 = t.group * p.bias_stride;
-      for (int c0 = 0; c0 < BN; c0 += 16) {
-        uint32_t r[16];
-        tmem_ld16(src + static_cast<uint32_t>(c0), r);
-        tmem_ld_wait();
-        if constexpr (SWAP) {                       // lane = column of C, register = row
-          const int64_t col = t.n0 + quad * 32 + lane;
-          if (col < p.n) {
-            const float bias = p.bias ? load_float(p.bias, p.bias_dtype, bias0 + col) : 0.0f;
+      if constexpr (SWAP) {                           // lane = column of C, register = row
+        const int64_t col = t.n0 + quad * 32 + lane;
+        const bool col_ok = col < p.n;
+        const float bias = p.bias && col_ok ? load_float(p.bias, p.bias_dtype, t.group * p.bias_stride + col) : 0.0f;
+        if (team == 1) {
+#pragma unroll 1
+          for (int c0 = 0; c0 < BN; c0 += 16) {
+            uint32_t r[16];
+            tmem_ld16(src + static_cast<uint32_t>(c0), r);
+            tmem_ld_wait();
+            if (!col_ok) continue;
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
               const int64_t row = t.row0 + c0 + j;
               if (row < t.row_end) store_out(p, row * p.ldo + col, __fadd_rn(__uint_as_float(r[j]), bias));
             }
           }
-        } else {                                    // lane = row, register = column
-          const int64_t row = t.row0 + quad * 32 + lane;
-          if (row < t.row_end) {
+        } else {
+          // this CTA's partial tile: row j goes to CTA j / own of the cluster, slot [rank][j % own][128]
+          const int own = BN / team;
+          const uint32_t red = base + Cfg::kEpiOff;
+          if (!mbar_wait(red_empty, red_phase ^ 1u, abort_flag, p.err)) break;
+#pragma unroll 1
+          for (int c0 = 0; c0 < BN; c0 += 16) {
+            uint32_t r[16];
+            tmem_ld16(src + static_cast<uint32_t>(c0), r);
+            tmem_ld_wait();
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
-              const int64_t col = t.n0 + c0 + j;
-              if (col < p.n)
-                store_out(p, row * p.ldo + col, __fadd_rn(__uint_as_float(r[j]), p.bias ? load_float(p.bias, p.bias_dtype, bias0 + col) : 0.0f));
+              const int to = (c0 + j) / own, slot = (c0 + j) - to * own;
+              st_cluster_f32(map_to_cta(red + static_cast<uint32_t>(((rank * own + slot) * kTileM + quad * 32 + lane) * 4), to), r[j]);
             }
           }
+          fence_cluster();
+          __syncwarp();
+          if (lane < team) mbar_arrive_cluster(map_to_cta(red_full, lane));
+          if (!mbar_wait(red_full, red_phase, abort_flag, p.err)) break;
+          fence_cluster();
+          const float *part = reinterpret_cast<const float *>(gen + Cfg::kEpiOff) + quad * 32 + lane;
+          for (int j = 0; j < own; ++j) {
+            float sum = part[j * kTileM];
+            for (int s = 1; s < team; ++s) sum += part[(s * own + j) * kTileM];
+            const int64_t row = t.row0 + rank * own + j;
+            if (col_ok && row < t.row_end) store_out(p, row * p.ldo + col, __fadd_rn(sum, bias));
+          }
+          __syncwarp();
+          if (lane < team) mbar_arrive_cluster(map_to_cta(red_empty, lane));
+          red_phase ^= 1u;
         }
+      } else {
+        const int row0 = t.row0 + (PAIR ? rank * kTileM : 0) + quad * 32;
+        if (row0 < t.row_end) store_rows<BN>(p, &tmap_out, src, t, row0, lane, stage, stage_addr, nstores);
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(acc_empty_bar(acc));
+      if (lane == 0) {
+        if constexpr (PAIR) mbar_arrive_cluster(map_to_cta(acc_empty_bar(acc), 0));
+        else mbar_arrive(acc_empty_bar(acc));
+      }
       if (++acc == Cfg::kAccs) { acc = 0; acc_phase ^= 1u; }
     }
+    if (!SWAP && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
   tc_fence_before();
   __syncthreads();
+  if (team > 1) cluster_sync_all();       // a peer may still signal into this CTA or read its shared memory
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, Cfg::kTmemCols);
+    if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Cfg::kTmemCols) : "memory");
+    else tmem_dealloc(tmem, Cfg::kTmemCols);
   }
 }
 
@@ -377,21 +564,27 @@ struct MxOperand {
   int64_t rows, batch;
 };
 
-template <int BN, bool SWAP>
-int32_t launch_mx(const MxOperand &a, const MxOperand &b, int64_t k, const MxParams &p, int64_t max_tiles, cudaStream_t st) {
-  using Cfg = MxCfg<BN>;
-  const MxOperand &om = SWAP ? b : a, &on = SWAP ? a : b;
-  CUtensorMap tm, tn, tsm, tsn;
+template <int BN, int MODE>
+int32_t launch_mx(const MxOperand &a, const MxOperand &b, int64_t k, MxParams p, int split, int64_t max_tiles, cudaStream_t st) {
+  using Cfg = MxCfg<BN, MODE>;
+  const MxOperand &om = MODE == kFew ? b : a, &on = MODE == kFew ? a : b;
+  CUtensorMap tm, tn, tsm, tsn, tout{};
   const uint64_t kb = static_cast<uint64_t>((k + 1) / 2), ks = static_cast<uint64_t>(ceil_div(k, 32));
+  const int eb = dtype_bytes(p.out_dtype);
   if (!make_byte_tmap3(&tm, om.codes, kb, om.rows, om.batch, om.code_stride, om.code_bs, 128, kTileM, true) ||
-      !make_byte_tmap3(&tn, on.codes, kb, on.rows, on.batch, on.code_stride, on.code_bs, 128, BN, true) ||
+      !make_byte_tmap3(&tn, on.codes, kb, on.rows, on.batch, on.code_stride, on.code_bs, 128, Cfg::kNRows, true) ||
       !make_byte_tmap3(&tsm, om.scales, ks, om.rows, om.batch, om.scale_stride, om.scale_bs, 16, kTileM, false) ||
-      !make_byte_tmap3(&tsn, on.scales, ks, on.rows, on.batch, on.scale_stride, on.scale_bs, 16, BN, false))
+      !make_byte_tmap3(&tsn, on.scales, ks, on.rows, on.batch, on.scale_stride, on.scale_bs, 16, BN, false) ||
+      (MODE != kFew && p.tma_out && !make_byte_tmap(&tout, p.out, p.n * eb, p.m, p.ldo * eb, 32)))
     return fail(BSIR_ERR_STRIDE, "matmul_mxfp4: the driver refuses a tensor map of these sizes and strides");
-  cudaFuncSetAttribute(mxfp4_gemm_kernel<BN, SWAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmem);
-  int64_t grid = device_info().sm_count > 0 ? device_info().sm_count : 148;
-  if (grid > max_tiles) grid = max_tiles;
-  launch_pdl(mxfp4_gemm_kernel<BN, SWAP>, dim3(static_cast<unsigned>(grid)), dim3(kThreads), Cfg::kSmem, st, tm, tn, tsm, tsn, p);
+  cudaFuncSetAttribute(mxfp4_gemm_kernel<BN, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmem);
+  const int team = MODE == kPair ? 2 : MODE == kFew ? split : 1;
+  p.split = team;
+  int64_t teams = (device_info().sm_count > 0 ? device_info().sm_count : 148) / team;
+  if (teams > max_tiles) teams = max_tiles;
+  const dim3 grid(static_cast<unsigned>(teams * team));
+  if (team > 1) launch_pdl_cluster(mxfp4_gemm_kernel<BN, MODE>, grid, dim3(kThreads), Cfg::kSmem, st, team, tm, tn, tsm, tsn, tout, p);
+  else launch_pdl(mxfp4_gemm_kernel<BN, MODE>, grid, dim3(kThreads), Cfg::kSmem, st, tm, tn, tsm, tsn, tout, p);
   count_launch();
   return check_launch("matmul_mxfp4");
 }
@@ -457,7 +650,24 @@ extern "C" int32_t bsir_matmul_mxfp4(const bsir_matmul_mxfp4_desc *d, void *stre
   // rows of a group that a tile should hold: all rows, or the groups' mean (their sizes are on the device)
   const int64_t rows = ceil_div(d->m, groups);
   auto tiles = [&](int64_t r, int64_t c) { return (d->m / r + groups) * ceil_div(d->n, c); };   // at most
-  if (rows <= 16) return launch_mx<16, true>(a, b, d->k, p, tiles(16, kTileM), st);
-  if (rows <= 64) return launch_mx<64, true>(a, b, d->k, p, tiles(64, kTileM), st);
-  return launch_mx<128, false>(a, b, d->k, p, tiles(kTileM, 128), st);
+  p.tma_out = aligned_to(d->out, 16) && (ldo * eb) % 16 == 0;
+  const int mode = std::getenv("MX_MODE") ? atoi(std::getenv("MX_MODE")) : -1;
+  const int sms = device_info().sm_count > 0 ? device_info().sm_count : 148;
+  auto split_of = [&](int64_t nt) {
+    if (std::getenv("MX_SPLIT")) return atoi(std::getenv("MX_SPLIT"));
+    const int chunks = (p.k_blocks + 1) / 2;
+    int s = 1;
+    while (s < 8 && nt * s * 2 <= sms && ceil_div(chunks, 2 * s) * (2 * s - 1) < chunks) s *= 2;
+    return s;
+  };
+  if (mode == 0) return launch_mx<128, kSingle>(a, b, d->k, p, 1, tiles(kTileM, 128), st);
+  if (mode == 1) return launch_mx<192, kPair>(a, b, d->k, p, 1, tiles(256, 192), st);
+  if (mode == 2) return launch_mx<256, kPair>(a, b, d->k, p, 1, tiles(256, 256), st);
+  if (mode == 3) return launch_mx<192, kSingle>(a, b, d->k, p, 1, tiles(128, 192), st);
+  if (mode == 4) return launch_mx<32, kFew>(a, b, d->k, p, split_of(tiles(32, kTileM)), tiles(32, kTileM), st);
+  if (mode == 5) return launch_mx<128, kPair>(a, b, d->k, p, 1, tiles(256, 128), st);
+  if (rows <= 16) return launch_mx<16, kFew>(a, b, d->k, p, split_of(tiles(16, kTileM)), tiles(16, kTileM), st);
+  if (rows <= 64) return launch_mx<64, kFew>(a, b, d->k, p, split_of(tiles(64, kTileM)), tiles(64, kTileM), st);
+  if (rows >= 512) return launch_mx<192, kPair>(a, b, d->k, p, 1, tiles(256, 192), st);
+  return launch_mx<128, kSingle>(a, b, d->k, p, 1, tiles(kTileM, 128), st);
 }
