@@ -8,13 +8,16 @@
 // (a 128-byte row is 256 elements of K); the exponents have to lie in tensor memory: row r of an operand tile at lane
 // r % 32, column r / 32, four bytes (128 elements of K) a cell, the same in all four lane quadrants.  The exponent
 // matrices keep the plain [rows, K / 32] layout, so groups may start at any row: TMA brings [rows x 16 bytes] (512
-// elements of K), and four warps, one a quadrant, move them shared memory -> registers -> tensor memory.
+// elements of K), a warp per 128 rows turns them in shared memory from a row's four words into a lane's four rows, and
+// the MMA issuer copies them to tensor memory with tcgen05.cp ahead of the instructions that use them.  (Warps storing
+// them to tensor memory themselves were the first form: next to cta_group::2 instructions such a store took 1400
+// cycles, and a chunk of 512 elements of K is 1024 of multiplication.)
 //
-// A persistent kernel, one CTA per SM, 320 threads:
+// A persistent kernel, one CTA per SM, 288 threads:
 //   warp 0      TMA producer of codes (a ring of stages of 256 elements of K) and exponents (a ring of 512)
-//   warp 1      MMA issuer
+//   warp 1      issuer of tcgen05.cp and tcgen05.mma
 //   warps 2-5   epilogue: accumulator -> bias -> rounding -> C
-//   warps 6-9   exponents into tensor memory, two buffers
+//   warps 6-8   exponents: rows of four words -> lanes of four rows, 128 rows a warp
 // in three forms:
 //   kPair    256 rows of A x BN columns of C on two CTAs (cta_group::2): each holds its 128 rows of A and half of the
 //            tile's rows of B, so that an SM's shared memory is read and filled for B half as often;
@@ -30,7 +33,7 @@ namespace {
 
 constexpr int kTileM = 128;
 constexpr int kStageK = 256;       // elements of K a stage: one 128-byte swizzle row of codes
-constexpr int kThreads = 320;
+constexpr int kThreads = 288;
 constexpr int kMaxGroups = 1024;
 enum MxMode { kSingle, kPair, kFew };
 
@@ -53,15 +56,16 @@ template <int BN, int MODE>
 struct MxCfg {
   static constexpr int kNRows = MODE == kPair ? BN / 2 : BN;         // rows of the N side's codes in this CTA
   static constexpr int kStage = (kTileM + kNRows) * 128;
-  static constexpr int kSfStage = (kTileM + BN) * 16;
+  static constexpr int kSfBlocks = 1 + (BN + 127) / 128;             // blocks of 128 rows of exponents: M side, N side
+  static constexpr int kSfStage = kSfBlocks * 2048;
   static constexpr int kSfStages = 3;
   static constexpr int kAccs = BN > 192 ? 1 : 2;
-  // columns of tensor memory: accumulators, then two buffers of 4 x (4 + kSfN) cells of exponents
-  static constexpr int kSfN = BN > 128 ? 8 : 4;
-  static constexpr int kSfCols = 4 * (4 + kSfN);
+  // columns of tensor memory: accumulators, then two buffers of exponents, 4 x 4 columns a block (512 elements of K)
+  static constexpr int kSfCols = kSfBlocks * 16;
   static constexpr int kSfBase = kAccs * BN;
-  static constexpr int kCols = kSfBase + 2 * kSfCols;
-  static constexpr int kTmemCols = kCols <= 128 ? 128 : kCols <= 256 ? 256 : 512;
+  static constexpr int kSfBufs = 2;
+  static constexpr int kCols = kSfBase + kSfBufs * kSfCols;
+  static constexpr int kTmemCols = kCols <= 64 ? 64 : kCols <= 128 ? 128 : kCols <= 256 ? 256 : 512;
   // staging: two buffers of 32 rows x 128 bytes of C a warp, or the partial tiles of a cluster
   static constexpr int kEpi = MODE == kFew ? BN * kTileM * 4 : 4 * 2 * 4096;
   static constexpr int kTable = 2 * (kMaxGroups + 1) * 4;
@@ -69,7 +73,7 @@ struct MxCfg {
   static constexpr int kFit = (227 * 1024 - kFixed) / kStage;
   static constexpr int kStages = kFit > 9 ? 9 : kFit;
   static constexpr int kSfOff = kStages * kStage;
-  static constexpr int kEpiOff = (kSfOff + kSfStages * kSfStage + 1023) / 1024 * 1024;    // 128-byte swizzle
+  static constexpr int kEpiOff = kSfOff + kSfStages * kSfStage;    // 128-byte swizzle
   static constexpr int kBarOff = kEpiOff + kEpi;
   static constexpr int kTableOff = kBarOff + 512;                    // tiles before a group, first row of a group
   static constexpr int kSmem = kTableOff + kTable + 1024;
@@ -77,35 +81,70 @@ struct MxCfg {
   static_assert(kStages >= 4 && kSmem <= 227 * 1024, "shared memory");
 };
 
+// The issuing warp's instructions.  All 32 lanes execute them and the predicate of one elected lane lets them through:
+// without a branch around them their operands are warp-uniform values, and one issues every 68 to 73 cycles, under the
+// 96 to 128 that the tensor core takes for N = 192 to 256; behind a branch (one lane of the warp, elected or lane 0)
+// it was 97 to 167.  Shared-memory descriptors come as their low words (address / 16); the high word is the same for
+// every K-major tile with the 128-byte swizzle (8-row groups 1024 bytes apart, version 1).
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_lo(uint32_t saddr) { return (saddr >> 4) | (1u << 16); }
 template <int MODE>
-__device__ __forceinline__ void mma_mxf4(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
+__device__ __forceinline__ void mma_mxf4(uint32_t elected, uint32_t tmem_d, uint32_t adesc, uint32_t bdesc, uint32_t idesc, uint32_t sfa, uint32_t sfb,
+                                         uint32_t accumulate) {
   if constexpr (MODE == kPair) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(tmem_d),
-        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        "{\n\t.reg .pred p, e;\n\t.reg .b64 a, b;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\tsetp.ne.b32 e, %8, 0;\n\t"
+        "mov.b64 a, {%1, %7};\n\tmov.b64 b, {%2, %7};\n\t"
+        "@e tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], a, b, %3, [%4], [%5], p;\n\t}" ::"r"(tmem_d),
+        "r"(adesc), "r"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate), "n"(kDescHi), "r"(elected)
         : "memory");
   } else {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(tmem_d),
-        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        "{\n\t.reg .pred p, e;\n\t.reg .b64 a, b;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\tsetp.ne.b32 e, %8, 0;\n\t"
+        "mov.b64 a, {%1, %7};\n\tmov.b64 b, {%2, %7};\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], a, b, %3, [%4], [%5], p;\n\t}" ::"r"(tmem_d),
+        "r"(adesc), "r"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate), "n"(kDescHi), "r"(elected)
         : "memory");
   }
+}
+// 32 lanes x 16 bytes of shared memory (no swizzle, 8 rows of 16 bytes 128 bytes apart) -> four columns of tensor
+// memory, repeated in the four lane quadrants; cta_group::2: in both CTAs, each from its own shared memory
+constexpr uint32_t kCopyDescHi = (128u >> 4) | (1u << 14);
+template <int MODE>
+__device__ __forceinline__ void tmem_copy(uint32_t elected, uint32_t taddr, uint32_t saddr) {
+  if constexpr (MODE == kPair)
+    asm volatile(
+        "{\n\t.reg .pred e;\n\t.reg .b64 a;\n\tsetp.ne.b32 e, %2, 0;\n\tmov.b64 a, {%1, %3};\n\t"
+        "@e tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], a;\n\t}" ::"r"(taddr),
+        "r"(saddr >> 4), "r"(elected), "n"(kCopyDescHi)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred e;\n\t.reg .b64 a;\n\tsetp.ne.b32 e, %2, 0;\n\tmov.b64 a, {%1, %3};\n\t"
+        "@e tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], a;\n\t}" ::"r"(taddr),
+        "r"(saddr >> 4), "r"(elected), "n"(kCopyDescHi)
+        : "memory");
+}
+template <int MODE>
+__device__ __forceinline__ void commit_to(uint32_t elected, uint32_t bar) {   // kPair: the barrier of both CTAs
+  if constexpr (MODE == kPair)
+    asm volatile(
+        "{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %1, 0;\n\t"
+        "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %2;\n\t}" ::"r"(bar),
+        "r"(elected), "h"(static_cast<uint16_t>(3))
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %1, 0;\n\t"
+        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar), "r"(elected)
+        : "memory");
 }
 // e2m1 x e2m1, exponents E8M0, both K-major; `sf_id` (0 or 2): which two of a cell's four bytes belong to these 64
 // elements of K
 __device__ __forceinline__ uint32_t mx_idesc(int n, int m, uint32_t sf_id) {
   return (sf_id << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n >> 3) << 17) | (1u << 23) | (static_cast<uint32_t>(m >> 7) << 27) | (sf_id << 29);
-}
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t *r) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
-      "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-      : "memory");
 }
 __device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap *map, int x, int y, int z, uint32_t leader_bar) {
   asm volatile(
@@ -113,10 +152,29 @@ __device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(leader_bar)
       : "memory");
 }
+// Arrival on a barrier of the pair's leader by a thread that hands over nothing but its own CTA's shared memory (made
+// visible to the tensor core by fence.proxy.async) or tensor memory (ordered by tcgen05.fence): no release at cluster
+// scope, which took about 1400 cycles next to running copies.
+__device__ __forceinline__ void mbar_arrive_leader(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
 __device__ __forceinline__ void st_cluster_f32(uint32_t cluster_addr, uint32_t bits) {
   asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr), "r"(bits) : "memory");
 }
 __device__ __forceinline__ void fence_cluster() { asm volatile("fence.acq_rel.cluster;" ::: "memory"); }
+
+// column (from a buffer's first) of word w (128 elements of K) of block b's exponents: the M side's four columns a
+// word, then the N side's, whose blocks lie side by side
+template <int BN>
+__device__ constexpr uint32_t sf_column(int b, int w) {
+  constexpr int nb = (BN + 127) / 128;
+  return b == 0 ? w * 4 : 16 + (w * nb + b - 1) * 4;
+}
+__device__ __forceinline__ uint32_t elect_one() {       // 1 in one lane of the (whole) warp
+  uint32_t one;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+  return one;
+}
 
 __device__ __forceinline__ float load_float(const void *p, int32_t dtype, int64_t i) {
   if (dtype == BSIR_F32) return static_cast<const float *>(p)[i];
@@ -253,13 +311,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto sf_full_bar = [&](int s) { return bars + 8u * (2 * Cfg::kStages + s); };
   auto sf_empty_bar = [&](int s) { return bars + 8u * (2 * Cfg::kStages + Cfg::kSfStages + s); };
   constexpr int kB2 = 2 * Cfg::kStages + 2 * Cfg::kSfStages;
-  auto st_full_bar = [&](int b) { return bars + 8u * (kB2 + b); };        // exponents in tensor memory
-  auto st_empty_bar = [&](int b) { return bars + 8u * (kB2 + 2 + b); };
-  auto acc_full_bar = [&](int b) { return bars + 8u * (kB2 + 4 + b); };
-  auto acc_empty_bar = [&](int b) { return bars + 8u * (kB2 + 6 + b); };
-  const uint32_t red_full = bars + 8u * (kB2 + 8), red_empty = bars + 8u * (kB2 + 9);   // partial tiles of the cluster
-  static_assert(8 * (kB2 + 10) + 16 <= 512, "barriers");
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(gen + Cfg::kBarOff + 8 * (kB2 + 10));
+  auto sf_ready_bar = [&](int s) { return bars + 8u * (kB2 + s); };                       // exponents turned
+  auto sf_used_bar = [&](int b) { return bars + 8u * (kB2 + Cfg::kSfStages + b); };       // a buffer's instructions are done
+  constexpr int kB3 = kB2 + Cfg::kSfStages + Cfg::kSfBufs;
+  auto acc_full_bar = [&](int b) { return bars + 8u * (kB3 + b); };
+  auto acc_empty_bar = [&](int b) { return bars + 8u * (kB3 + 2 + b); };
+  const uint32_t red_full = bars + 8u * (kB3 + 4), red_empty = bars + 8u * (kB3 + 5);   // partial tiles of the cluster
+  static_assert(8 * (kB3 + 6) + 16 <= 512, "barriers");
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(gen + Cfg::kBarOff + 8 * (kB3 + 6));
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
   int *tile_start = reinterpret_cast<int *>(gen + Cfg::kTableOff);         // [groups + 1]
   int *row_start = tile_start + kMaxGroups + 1;                            // [groups + 1]
@@ -272,9 +331,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   pdl_launch_dependents();
   if (threadIdx.x == 0) {
     for (int s = 0; s < Cfg::kStages; ++s) { mbar_init(full_bar(s), 1); mbar_init(empty_bar(s), 1); }
-    for (int s = 0; s < Cfg::kSfStages; ++s) { mbar_init(sf_full_bar(s), 1); mbar_init(sf_empty_bar(s), 4); }
+    for (int s = 0; s < Cfg::kSfStages; ++s) {
+      mbar_init(sf_full_bar(s), 1); mbar_init(sf_empty_bar(s), 1); mbar_init(sf_ready_bar(s), Cfg::kSfBlocks * (PAIR ? 2 : 1));
+    }
+    for (int b = 0; b < Cfg::kSfBufs; ++b) mbar_init(sf_used_bar(b), 1);
     for (int b = 0; b < 2; ++b) {
-      mbar_init(st_full_bar(b), PAIR ? 8 : 4); mbar_init(st_empty_bar(b), 1);
       mbar_init(acc_full_bar(b), 1); mbar_init(acc_empty_bar(b), PAIR ? 8 : 4);
     }
     mbar_init(red_full, 4 * team);
@@ -361,7 +422,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if ((kb & 1) == 0) {
             if (!mbar_wait(sf_empty_bar(sf), sf_phase ^ 1u, abort_flag, p.err)) { ok = false; break; }
             const uint32_t dst = base + Cfg::kSfOff + sf * Cfg::kSfStage;
-            mbar_expect_tx(sf_full_bar(sf), Cfg::kSfStage);
+            mbar_expect_tx(sf_full_bar(sf), (kTileM + BN) * 16);
             tma_load_3d(dst, &tmap_sm, kb * (kStageK / 32), m0, zm, sf_full_bar(sf));
             tma_load_3d(dst + kTileM * 16, &tmap_sn, kb * (kStageK / 32), SWAP ? t.row0 : t.n0, zn, sf_full_bar(sf));
             if (++sf == Cfg::kSfStages) { sf = 0; sf_phase ^= 1u; }
@@ -392,84 +453,73 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp == 1) {
     // ---------------- MMA issuer (the pair's leader only)
-    if (lane == 0 && (!PAIR || rank == 0)) {
+    if (!PAIR || rank == 0) {
       const uint32_t idesc0 = mx_idesc(BN, PAIR ? 256 : 128, 0), idesc2 = mx_idesc(BN, PAIR ? 256 : 128, 2);
-      auto commit = [&](uint32_t bar) {
-        if constexpr (PAIR) tc_commit_pair(bar);
-        else tc_commit(bar);
-      };
-      int stage = 0, b = 0, acc = 0;
-      uint32_t phase = 0, b_phase = 0, acc_phase = 0;
+      const uint32_t elected = elect_one();
+      int stage = 0, sf = 0, b = 0, acc = 0;
+      uint32_t phase = 0, sf_phase = 0, b_phase = 0, acc_phase = 0;
       bool ok = true;
       for (int tile = first_tile; tile < total_tiles && ok; tile += tile_step) {
         if (!mbar_wait(acc_empty_bar(acc), acc_phase ^ 1u, abort_flag, p.err)) break;
-        tc_fence_after();
         const uint32_t d = tmem + static_cast<uint32_t>(acc * BN);
-        for (int c = chunk0; c < chunk1 && ok; ++c) {
-          if (!mbar_wait(st_full_bar(b), b_phase, abort_flag, p.err)) { ok = false; break; }
-          const uint32_t sf = tmem + static_cast<uint32_t>(Cfg::kSfBase + b * Cfg::kSfCols);
-          for (int h = 0; h < 2 && 2 * c + h < kb1; ++h) {
-            if (!mbar_wait(full_bar(stage), phase, abort_flag, p.err)) { ok = false; break; }
-            tc_fence_after();
-            const uint32_t sm = base + stage * Cfg::kStage, sn = sm + kTileM * 128;
-#pragma unroll
-            for (int kk = 0; kk < 4; ++kk) {
-              const uint32_t cell = static_cast<uint32_t>(2 * h + (kk >> 1));
-              mma_mxf4<MODE>(d, make_desc(sm + kk * 32, 16, 1024), make_desc(sn + kk * 32, 16, 1024), (kk & 1) ? idesc2 : idesc0, sf + cell * 4,
-                             sf + 16 + cell * Cfg::kSfN, (c > chunk0 || h > 0 || kk > 0) ? 1u : 0u);
-            }
-            commit(empty_bar(stage));
-            if (++stage == Cfg::kStages) { stage = 0; phase ^= 1u; }
+        for (int kb = kb0; kb < kb1; ++kb) {
+          const bool first_half = (kb & 1) == 0, last_half = !first_half || kb + 1 == kb1;
+          const uint32_t sfb = tmem + static_cast<uint32_t>(Cfg::kSfBase + b * Cfg::kSfCols);
+          if (first_half) {      // this chunk's exponents are turned, and the buffer's last instructions have read it
+            if (!mbar_wait(sf_ready_bar(sf), sf_phase, abort_flag, p.err)) { ok = false; break; }
+            if (!mbar_wait(sf_used_bar(b), b_phase ^ 1u, abort_flag, p.err)) { ok = false; break; }
           }
-          if (!ok) break;
-          commit(st_empty_bar(b));
-          b ^= 1;
-          if (b == 0) b_phase ^= 1u;
+          if (!mbar_wait(full_bar(stage), phase, abort_flag, p.err)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t sm = desc_lo(base) + static_cast<uint32_t>(stage) * (Cfg::kStage >> 4), sn = sm + kTileM * 8;
+          const uint32_t sfs = base + Cfg::kSfOff + sf * Cfg::kSfStage;
+          const uint32_t half = first_half ? 0u : 2u;
+          if (first_half) {
+#pragma unroll
+            for (int i = 0; i < 4 * Cfg::kSfBlocks; ++i) tmem_copy<MODE>(elected, sfb + sf_column<BN>(i / 4, i % 4), sfs + i * 512);
+            commit_to<MODE>(elected, sf_empty_bar(sf));
+          }
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk) {
+            const uint32_t cell = half + (kk >> 1);
+            mma_mxf4<MODE>(elected, d, sm + kk * 2, sn + kk * 2, (kk & 1) ? idesc2 : idesc0, sfb + cell * 4, sfb + 16 + cell * (Cfg::kSfBlocks - 1) * 4,
+                           (kb > kb0 || kk > 0) ? 1u : 0u);
+          }
+          commit_to<MODE>(elected, empty_bar(stage));
+          if (last_half) commit_to<MODE>(elected, sf_used_bar(b));
+          if (kb + 1 == kb1) commit_to<MODE>(elected, acc_full_bar(acc));
+          if (++stage == Cfg::kStages) { stage = 0; phase ^= 1u; }
+          if (first_half && ++sf == Cfg::kSfStages) { sf = 0; sf_phase ^= 1u; }
+          if (last_half && ++b == Cfg::kSfBufs) { b = 0; b_phase ^= 1u; }
         }
-        if (!ok) break;
-        commit(acc_full_bar(acc));
         if (++acc == Cfg::kAccs) { acc = 0; acc_phase ^= 1u; }
       }
     }
   } else if (warp >= 6) {
-    // ---------------- exponents: shared memory -> registers -> this warp's quadrant of tensor memory
-    const uint32_t quad = static_cast<uint32_t>(warp & 3) * 32u << 16;
-    int sf = 0, b = 0;
-    uint32_t sf_phase = 0, b_phase = 0;
-    bool ok = true;
-    for (int tile = first_tile; tile < total_tiles && ok; tile += tile_step) {
-      for (int c = chunk0; c < chunk1; ++c) {
-        if (!mbar_wait(sf_full_bar(sf), sf_phase, abort_flag, p.err)) { ok = false; break; }
-        const uint4 *src = reinterpret_cast<const uint4 *>(gen + Cfg::kSfOff + sf * Cfg::kSfStage);
-        uint32_t rm[16], rn[4 * Cfg::kSfN];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint4 w = src[j * 32 + lane];
-          rm[j] = w.x; rm[4 + j] = w.y; rm[8 + j] = w.z; rm[12 + j] = w.w;
+    // ---------------- exponents: this warp's block of 128 rows, turned in place: row r's words w -> lane r % 32 of word w
+    const int block = warp - 6;
+    if (block < Cfg::kSfBlocks) {
+      int sf = 0;
+      uint32_t sf_phase = 0;
+      bool ok = true;
+      for (int tile = first_tile; tile < total_tiles && ok; tile += tile_step) {
+        for (int c = chunk0; c < chunk1; ++c) {
+          if (!mbar_wait(sf_full_bar(sf), sf_phase, abort_flag, p.err)) { ok = false; break; }
+          uint4 *rows = reinterpret_cast<uint4 *>(gen + Cfg::kSfOff + sf * Cfg::kSfStage + block * 2048);
+          const uint4 r0 = rows[lane], r1 = rows[32 + lane], r2 = rows[64 + lane], r3 = rows[96 + lane];
+          __syncwarp();
+          rows[lane] = make_uint4(r0.x, r1.x, r2.x, r3.x);
+          rows[32 + lane] = make_uint4(r0.y, r1.y, r2.y, r3.y);
+          rows[64 + lane] = make_uint4(r0.z, r1.z, r2.z, r3.z);
+          rows[96 + lane] = make_uint4(r0.w, r1.w, r2.w, r3.w);
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) {
+            if constexpr (PAIR) mbar_arrive_leader(map_to_cta(sf_ready_bar(sf), 0));
+            else mbar_arrive(sf_ready_bar(sf));
+          }
+          if (++sf == Cfg::kSfStages) { sf = 0; sf_phase ^= 1u; }
         }
-#pragma unroll
-        for (int j = 0; j < Cfg::kSfN; ++j) {
-          const uint4 w = j * 32 + lane < BN ? src[kTileM + j * 32 + lane] : make_uint4(0, 0, 0, 0);
-          rn[j] = w.x; rn[Cfg::kSfN + j] = w.y; rn[2 * Cfg::kSfN + j] = w.z; rn[3 * Cfg::kSfN + j] = w.w;
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(sf_empty_bar(sf));
-        if (++sf == Cfg::kSfStages) { sf = 0; sf_phase ^= 1u; }
-        if (!mbar_wait(st_empty_bar(b), b_phase ^ 1u, abort_flag, p.err)) { ok = false; break; }
-        tc_fence_after();
-        const uint32_t dst = tmem + quad + static_cast<uint32_t>(Cfg::kSfBase + b * Cfg::kSfCols);
-        tmem_st16(dst, rm);
-        if constexpr (Cfg::kSfN == 4) tmem_st16(dst + 16, rn);
-        else tmem_st32(dst + 16, rn);
-        tmem_st_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) {
-          if constexpr (PAIR) mbar_arrive_cluster(map_to_cta(st_full_bar(b), 0));
-          else mbar_arrive(st_full_bar(b));
-        }
-        b ^= 1;
-        if (b == 0) b_phase ^= 1u;
       }
     }
   } else {
@@ -541,7 +591,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {
-        if constexpr (PAIR) mbar_arrive_cluster(map_to_cta(acc_empty_bar(acc), 0));
+        if constexpr (PAIR) mbar_arrive_leader(map_to_cta(acc_empty_bar(acc), 0));
         else mbar_arrive(acc_empty_bar(acc));
       }
       if (++acc == Cfg::kAccs) { acc = 0; acc_phase ^= 1u; }
