@@ -48,7 +48,7 @@ struct MxParams {
   void *out;
   int64_t ldo;
   int *err;
-  int tma_out;                     // 1: C's rows can be written by TMA, 2: at least in 16-byte pieces, 0: neither
+  int tma_out;                     // 1: C's rows start 16-byte aligned (TMA stores, 16-byte pieces)
   int split;                       // kFew: CTAs that share a tile's K (a cluster)
 };
 
@@ -60,18 +60,21 @@ struct MxCfg {
   static constexpr int kSfStage = kSfBlocks * 2048;
   static constexpr int kSfStages = 3;
   static constexpr int kAccs = BN > 192 ? 1 : 2;
-  // columns of tensor memory: accumulators, then two buffers of exponents, 4 x 4 columns a block (512 elements of K)
-  static constexpr int kSfCols = kSfBlocks * 16;
+  // columns of tensor memory: accumulators, then each stage's exponents: two words (128 elements of K each) of four
+  // columns a block, the N side's first
+  static constexpr int kSfN = (kSfBlocks - 1) * 4;
+  static constexpr int kSfCols = 2 * (kSfN + 4);
   static constexpr int kSfBase = kAccs * BN;
-  static constexpr int kSfBufs = 2;
-  static constexpr int kCols = kSfBase + kSfBufs * kSfCols;
-  static constexpr int kTmemCols = kCols <= 64 ? 64 : kCols <= 128 ? 128 : kCols <= 256 ? 256 : 512;
+  static constexpr int kSfBufs = (512 - kSfBase) / kSfCols;
   // staging: two buffers of 32 rows x 128 bytes of C a warp, or the partial tiles of a cluster
   static constexpr int kEpi = MODE == kFew ? BN * kTileM * 4 : 4 * 2 * 4096;
   static constexpr int kTable = 2 * (kMaxGroups + 1) * 4;
   static constexpr int kFixed = kSfStages * kSfStage + kEpi + 512 /*barriers*/ + kTable + 1024 /*alignment*/;
   static constexpr int kFit = (227 * 1024 - kFixed) / kStage;
-  static constexpr int kStages = kFit > 9 ? 9 : kFit;
+  static constexpr int kMost = kSfBufs < 9 ? kSfBufs : 9;
+  static constexpr int kStages = kFit > kMost ? kMost : kFit;
+  static constexpr int kCols = kSfBase + kStages * kSfCols;
+  static constexpr int kTmemCols = kCols <= 64 ? 64 : kCols <= 128 ? 128 : kCols <= 256 ? 256 : 512;
   static constexpr int kSfOff = kStages * kStage;
   static constexpr int kEpiOff = kSfOff + kSfStages * kSfStage;    // 128-byte swizzle
   static constexpr int kBarOff = kEpiOff + kEpi;
@@ -141,6 +144,11 @@ __device__ __forceinline__ void commit_to(uint32_t elected, uint32_t bar) {   //
         "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar), "r"(elected)
         : "memory");
 }
+__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {      // without waiting
+  uint32_t done;
+  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+  return done != 0;
+}
 // e2m1 x e2m1, exponents E8M0, both K-major; `sf_id` (0 or 2): which two of a cell's four bytes belong to these 64
 // elements of K
 __device__ __forceinline__ uint32_t mx_idesc(int n, int m, uint32_t sf_id) {
@@ -163,13 +171,6 @@ __device__ __forceinline__ void st_cluster_f32(uint32_t cluster_addr, uint32_t b
 }
 __device__ __forceinline__ void fence_cluster() { asm volatile("fence.acq_rel.cluster;" ::: "memory"); }
 
-// column (from a buffer's first) of word w (128 elements of K) of block b's exponents: the M side's four columns a
-// word, then the N side's, whose blocks lie side by side
-template <int BN>
-__device__ constexpr uint32_t sf_column(int b, int w) {
-  constexpr int nb = (BN + 127) / 128;
-  return b == 0 ? w * 4 : 16 + (w * nb + b - 1) * 4;
-}
 __device__ __forceinline__ uint32_t elect_one() {       // 1 in one lane of the (whole) warp
   uint32_t one;
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
@@ -204,91 +205,141 @@ __device__ __forceinline__ void find_tile(int tile, const int *tile_start, const
   t.n0 = (local / row_tiles) * COLS;
 }
 
-// One epilogue warp's 32 rows x BN columns of an accumulator -> C.  128 bytes of each row at a time are staged in
-// shared memory with the 128-byte swizzle and leave through a TMA store; where that cannot be (rows behind the group's
-// end in the box, C's rows not 16-byte aligned) the warp stores them itself, row by row.
-template <int BN>
-__device__ __forceinline__ void store_rows(const MxParams &p, const CUtensorMap *tmap_out, uint32_t acc, const MxTile &t, int row0, int lane,
-                                           uint8_t *stage, uint32_t stage_addr, uint32_t &nstores) {
-  const bool wide = p.out_dtype == BSIR_F32;
-  const int eb = wide ? 4 : 2, step = wide ? 32 : 64;        // columns of a 128-byte piece
-  const bool by_tma = p.tma_out == 1 && (row0 + 32 <= t.row_end || t.row_end == p.m);   // behind the last row nothing is written
-  const int rows = t.row_end - row0 < 32 ? t.row_end - row0 : 32;
-  for (int c0 = 0; c0 < BN; c0 += step) {
-    const int64_t col0 = t.n0 + c0;
-    if (col0 >= p.n) break;
-    const uint32_t b = nstores & 1u;
-    if (by_tma) {      // the store that read this buffer two pieces ago must have read it
-      if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
-    }
+// 32 columns of an epilogue warp's 32 rows from tensor memory, bias added
+__device__ __forceinline__ void load_columns(const MxParams &p, uint32_t acc, int group, int64_t col0, int lane, uint32_t *r) {
+  tmem_ld32(acc, r);
+  tmem_ld_wait();
+  if (p.bias) {
+    const int64_t col = col0 + lane;
+    const float mine = col < p.n ? load_float(p.bias, p.bias_dtype, group * p.bias_stride + col) : 0.0f;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__fadd_rn(__uint_as_float(r[j]), __shfl_sync(0xffffffffu, mine, j)));
+  }
+}
+__device__ __forceinline__ void round_columns(const MxParams &p, const uint32_t *r, uint32_t *w) {
+  if (p.out_dtype == BSIR_F16) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) w[j] = pack_f16x2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]));
+  } else {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) w[j] = pack_bf16x2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]));
+  }
+}
+// 64 bytes (half of a 128-byte piece) of this lane's row into the staging buffer, 128-byte swizzle
+__device__ __forceinline__ void stage_half(uint8_t *row, int lane, int half, const uint32_t *w) {
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+    *reinterpret_cast<uint4 *>(row + (((4 * half + c) ^ (lane & 7)) * 16)) = make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+}
+
+// An epilogue warp's 32 rows of C, 128 bytes a row at a time: staged in shared memory and sent by a TMA store; where
+// that cannot be (rows behind the group's end in the box, C's rows not 16-byte aligned) the warp stores them itself,
+// row by row.
+struct RowWriter {
+  const MxParams &p;
+  const CUtensorMap *tmap_out;
+  const MxTile &t;
+  int row0, lane, eb, rows;
+  bool by_tma;
+  uint8_t *stage;
+  uint32_t stage_addr;
+  uint32_t &nstores;
+  __device__ __forceinline__ RowWriter(const MxParams &p_, const CUtensorMap *m, const MxTile &t_, int row0_, int lane_, uint8_t *stage_, uint32_t addr, uint32_t &n)
+      : p(p_), tmap_out(m), t(t_), row0(row0_), lane(lane_), stage(stage_), stage_addr(addr), nstores(n) {
+    eb = p.out_dtype == BSIR_F32 ? 4 : 2;
+    rows = t.row_end - row0 < 32 ? t.row_end - row0 : 32;
+    by_tma = p.tma_out && (rows == 32 || t.row_end == p.m);     // behind the last row of C nothing is written
+  }
+  // the buffer for the next piece: this lane's row of it
+  __device__ __forceinline__ uint8_t *begin() {
+    if (by_tma && lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");   // the store of two pieces ago has read it
     __syncwarp();
-    uint8_t *buf = stage + b * 4096, *mine = buf + lane * 128;
-    const uint32_t sw = static_cast<uint32_t>(lane & 7);
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {                            // 32 columns each
-      if (h == 1 && (wide || BN - c0 <= 32)) break;
-      uint32_t r[32];
-      tmem_ld32(acc + static_cast<uint32_t>(c0 + 32 * h), r);
-      tmem_ld_wait();
-      if (p.bias) {
-        const int64_t col = col0 + 32 * h + lane;
-        const float mine_b = col < p.n ? load_float(p.bias, p.bias_dtype, t.group * p.bias_stride + col) : 0.0f;
-#pragma unroll
-        for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__fadd_rn(__uint_as_float(r[j]), __shfl_sync(0xffffffffu, mine_b, j)));
-      }
-      if (wide) {
-#pragma unroll
-        for (int c = 0; c < 8; ++c)
-          *reinterpret_cast<uint4 *>(mine + ((c ^ sw) * 16)) = make_uint4(r[4 * c], r[4 * c + 1], r[4 * c + 2], r[4 * c + 3]);
-      } else {
-        uint32_t w[16];
-        if (p.out_dtype == BSIR_F16) {
-#pragma unroll
-          for (int j = 0; j < 16; ++j) w[j] = pack_f16x2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]));
-        } else {
-#pragma unroll
-          for (int j = 0; j < 16; ++j) w[j] = pack_bf16x2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]));
-        }
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-          *reinterpret_cast<uint4 *>(mine + (((4 * h + c) ^ sw) * 16)) = make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
-      }
-    }
+    return stage + (nstores & 1u) * 4096 + lane * 128;
+  }
+  __device__ __forceinline__ void send(int64_t col0, int cols) {     // `cols` of C from col0 on, at most 128 bytes
+    uint8_t *buf = stage + (nstores & 1u) * 4096;
     if (by_tma) {
       fence_proxy_async();
       __syncwarp();
-      if (lane == 0) tma_store_2d(tmap_out, static_cast<int>(col0) * eb, row0, stage_addr + b * 4096);
+      if (lane == 0) tma_store_2d(tmap_out, static_cast<int>(col0) * eb, row0, stage_addr + (nstores & 1u) * 4096);
       ++nstores;
-    } else {
-      __syncwarp();
-      const int64_t left = (p.n - col0) * eb;                // bytes of a row from here on
-      const int have = static_cast<int>(left < 128 ? left : 128) < (BN - c0) * eb ? static_cast<int>(left < 128 ? left : 128) : (BN - c0) * eb;
-      if (p.tma_out) {                                       // eight lanes a row, four rows at a time
-        const int piece = lane & 7;
-        for (int r = lane >> 3; r < rows; r += 4) {
-          const uint4 v = *reinterpret_cast<const uint4 *>(buf + r * 128 + ((piece ^ (r & 7)) * 16));
-          char *dst = static_cast<char *>(p.out) + ((row0 + r) * p.ldo + col0) * eb + piece * 16;
-          if (piece * 16 + 16 <= have) {
-            *reinterpret_cast<uint4 *>(dst) = v;
-          } else {
-            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-            for (int i = 0; i < 16 && piece * 16 + i < have; i += eb) {
-              if (wide) *reinterpret_cast<uint32_t *>(dst + i) = w[i / 4];
-              else *reinterpret_cast<uint16_t *>(dst + i) = static_cast<uint16_t>(w[i / 4] >> (8 * (i & 2)));
-            }
-          }
+      return;
+    }
+    __syncwarp();
+    const int have = static_cast<int>(p.n - col0 < cols ? p.n - col0 : cols) * eb;    // bytes of a row
+    if (p.tma_out) {                                       // eight lanes a row, four rows at a time
+      const int piece = lane & 7;
+      for (int r = lane >> 3; r < rows; r += 4) {
+        const uint4 v = *reinterpret_cast<const uint4 *>(buf + r * 128 + ((piece ^ (r & 7)) * 16));
+        char *dst = static_cast<char *>(p.out) + ((row0 + r) * p.ldo + col0) * eb + piece * 16;
+        if (piece * 16 + 16 <= have) {
+          *reinterpret_cast<uint4 *>(dst) = v;
+        } else {
+          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (piece * 16 + 2 * i < have) reinterpret_cast<uint16_t *>(dst)[i] = static_cast<uint16_t>(w[i / 2] >> (16 * (i & 1)));
         }
-      } else {
-        for (int r = 0; r < rows; ++r) {
-          char *dst = static_cast<char *>(p.out) + ((row0 + r) * p.ldo + col0) * eb;
-          for (int i = lane * eb; i < have; i += 32 * eb) {
-            const uint8_t *src = buf + r * 128 + (((i >> 4) ^ (r & 7)) * 16) + (i & 15);
-            if (wide) *reinterpret_cast<uint32_t *>(dst + i) = *reinterpret_cast<const uint32_t *>(src);
-            else *reinterpret_cast<uint16_t *>(dst + i) = *reinterpret_cast<const uint16_t *>(src);
-          }
+      }
+    } else {
+      for (int r = 0; r < rows; ++r) {
+        char *dst = static_cast<char *>(p.out) + ((row0 + r) * p.ldo + col0) * eb;
+        for (int i = lane * eb; i < have; i += 32 * eb) {
+          const uint8_t *src = buf + r * 128 + (((i >> 4) ^ (r & 7)) * 16) + (i & 15);
+          if (eb == 4) *reinterpret_cast<uint32_t *>(dst + i) = *reinterpret_cast<const uint32_t *>(src);
+          else *reinterpret_cast<uint16_t *>(dst + i) = *reinterpret_cast<const uint16_t *>(src);
         }
       }
     }
+    __syncwarp();
+  }
+};
+
+// One accumulator -> C.  `release()` hands the accumulator back to the issuer.  With a second accumulator the issuer is
+// busy meanwhile and the columns go out as they come; with one (BN = 256) it is waiting: 16-bit results are first taken
+// into registers whole.
+template <int BN, bool kDrain, class Release>
+__device__ __forceinline__ void store_rows(const MxParams &p, RowWriter &out, uint32_t acc, const MxTile &t, int lane, Release release) {
+  if (p.out_dtype == BSIR_F32) {
+    for (int c0 = 0; c0 < BN && t.n0 + c0 < p.n; c0 += 32) {
+      uint32_t r[32];
+      load_columns(p, acc + static_cast<uint32_t>(c0), t.group, t.n0 + c0, lane, r);
+      uint8_t *row = out.begin();
+      stage_half(row, lane, 0, r);
+      stage_half(row, lane, 1, r + 16);
+      out.send(t.n0 + c0, 32);
+    }
+    release();
+  } else if constexpr (kDrain) {
+    uint32_t w[BN / 2];
+#pragma unroll
+    for (int c = 0; c < BN / 32; ++c) {
+      uint32_t r[32];
+      load_columns(p, acc + static_cast<uint32_t>(32 * c), t.group, t.n0 + 32 * c, lane, r);
+      round_columns(p, r, w + 16 * c);
+    }
+    release();
+#pragma unroll
+    for (int c = 0; c < BN / 64; ++c) {
+      if (t.n0 + 64 * c >= p.n) break;
+      uint8_t *row = out.begin();
+      stage_half(row, lane, 0, w + 32 * c);
+      stage_half(row, lane, 1, w + 32 * c + 16);
+      out.send(t.n0 + 64 * c, 64);
+    }
+  } else {
+    for (int c0 = 0; c0 < BN && t.n0 + c0 < p.n; c0 += 64) {
+      uint32_t r[32], w[16];
+      load_columns(p, acc + static_cast<uint32_t>(c0), t.group, t.n0 + c0, lane, r);
+      round_columns(p, r, w);
+      uint8_t *row = out.begin();
+      stage_half(row, lane, 0, w);
+      load_columns(p, acc + static_cast<uint32_t>(c0 + 32), t.group, t.n0 + c0 + 32, lane, r);
+      round_columns(p, r, w);
+      stage_half(row, lane, 1, w);
+      out.send(t.n0 + c0, 64);
+    }
+    release();
   }
 }
 
@@ -312,8 +363,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto sf_empty_bar = [&](int s) { return bars + 8u * (2 * Cfg::kStages + Cfg::kSfStages + s); };
   constexpr int kB2 = 2 * Cfg::kStages + 2 * Cfg::kSfStages;
   auto sf_ready_bar = [&](int s) { return bars + 8u * (kB2 + s); };                       // exponents turned
-  auto sf_used_bar = [&](int b) { return bars + 8u * (kB2 + Cfg::kSfStages + b); };       // a buffer's instructions are done
-  constexpr int kB3 = kB2 + Cfg::kSfStages + Cfg::kSfBufs;
+  constexpr int kB3 = kB2 + Cfg::kSfStages;
   auto acc_full_bar = [&](int b) { return bars + 8u * (kB3 + b); };
   auto acc_empty_bar = [&](int b) { return bars + 8u * (kB3 + 2 + b); };
   const uint32_t red_full = bars + 8u * (kB3 + 4), red_empty = bars + 8u * (kB3 + 5);   // partial tiles of the cluster
@@ -334,7 +384,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int s = 0; s < Cfg::kSfStages; ++s) {
       mbar_init(sf_full_bar(s), 1); mbar_init(sf_empty_bar(s), 1); mbar_init(sf_ready_bar(s), Cfg::kSfBlocks * (PAIR ? 2 : 1));
     }
-    for (int b = 0; b < Cfg::kSfBufs; ++b) mbar_init(sf_used_bar(b), 1);
     for (int b = 0; b < 2; ++b) {
       mbar_init(acc_full_bar(b), 1); mbar_init(acc_empty_bar(b), PAIR ? 8 : 4);
     }
@@ -403,7 +452,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int per = SWAP ? (all_chunks + team - 1) / team : all_chunks;
   const int chunk0 = SWAP ? rank * per : 0;
   const int chunk1 = min(all_chunks, chunk0 + per);
-  const int kb0 = 2 * chunk0, kb1 = min(p.k_blocks, 2 * chunk1);
+  const int kb0 = 2 * chunk0, kb1 = min(p.k_blocks, 2 * chunk1);       // its stages
   int group = 0;
   MxTile t;
 
@@ -456,41 +505,40 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (!PAIR || rank == 0) {
       const uint32_t idesc0 = mx_idesc(BN, PAIR ? 256 : 128, 0), idesc2 = mx_idesc(BN, PAIR ? 256 : 128, 2);
       const uint32_t elected = elect_one();
-      int stage = 0, sf = 0, b = 0, acc = 0;
-      uint32_t phase = 0, sf_phase = 0, b_phase = 0, acc_phase = 0;
-      bool ok = true;
+      int stage = 0, sf = 0, acc = 0;
+      uint32_t phase = 0, sf_phase = 0, acc_phase = 0;
+      bool ok = true, here = false, sf_here = false;
       for (int tile = first_tile; tile < total_tiles && ok; tile += tile_step) {
         if (!mbar_wait(acc_empty_bar(acc), acc_phase ^ 1u, abort_flag, p.err)) break;
         const uint32_t d = tmem + static_cast<uint32_t>(acc * BN);
         for (int kb = kb0; kb < kb1; ++kb) {
-          const bool first_half = (kb & 1) == 0, last_half = !first_half || kb + 1 == kb1;
-          const uint32_t sfb = tmem + static_cast<uint32_t>(Cfg::kSfBase + b * Cfg::kSfCols);
-          if (first_half) {      // this chunk's exponents are turned, and the buffer's last instructions have read it
-            if (!mbar_wait(sf_ready_bar(sf), sf_phase, abort_flag, p.err)) { ok = false; break; }
-            if (!mbar_wait(sf_used_bar(b), b_phase ^ 1u, abort_flag, p.err)) { ok = false; break; }
-          }
-          if (!mbar_wait(full_bar(stage), phase, abort_flag, p.err)) { ok = false; break; }
+          const uint32_t half = static_cast<uint32_t>(kb & 1);          // of the chunk
+          // the next barriers were looked at while the last stage's instructions went out
+          if (half == 0 && !sf_here && !mbar_wait(sf_ready_bar(sf), sf_phase, abort_flag, p.err)) { ok = false; break; }
+          if (!here && !mbar_wait(full_bar(stage), phase, abort_flag, p.err)) { ok = false; break; }
           tc_fence_after();
+          // the stage's codes have landed, so the instructions that used its columns of exponents before are done
+          const uint32_t sfb = tmem + static_cast<uint32_t>(Cfg::kSfBase + stage * Cfg::kSfCols), sfa = sfb + 2 * Cfg::kSfN;
+          const uint32_t sfs = base + Cfg::kSfOff + sf * Cfg::kSfStage + half * 1024;
           const uint32_t sm = desc_lo(base) + static_cast<uint32_t>(stage) * (Cfg::kStage >> 4), sn = sm + kTileM * 8;
-          const uint32_t sfs = base + Cfg::kSfOff + sf * Cfg::kSfStage;
-          const uint32_t half = first_half ? 0u : 2u;
-          if (first_half) {
 #pragma unroll
-            for (int i = 0; i < 4 * Cfg::kSfBlocks; ++i) tmem_copy<MODE>(elected, sfb + sf_column<BN>(i / 4, i % 4), sfs + i * 512);
-            commit_to<MODE>(elected, sf_empty_bar(sf));
+          for (int w = 0; w < 2; ++w) {
+            tmem_copy<MODE>(elected, sfa + w * 4, sfs + w * 512);
+#pragma unroll
+            for (int i = 1; i < Cfg::kSfBlocks; ++i) tmem_copy<MODE>(elected, sfb + w * Cfg::kSfN + (i - 1) * 4, sfs + i * 2048 + w * 512);
           }
+          const bool sf_done = half == 1 || kb + 1 == kb1;
+          if (sf_done) commit_to<MODE>(elected, sf_empty_bar(sf));
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk) {
-            const uint32_t cell = half + (kk >> 1);
-            mma_mxf4<MODE>(elected, d, sm + kk * 2, sn + kk * 2, (kk & 1) ? idesc2 : idesc0, sfb + cell * 4, sfb + 16 + cell * (Cfg::kSfBlocks - 1) * 4,
+          for (int kk = 0; kk < 4; ++kk)
+            mma_mxf4<MODE>(elected, d, sm + kk * 2, sn + kk * 2, (kk & 1) ? idesc2 : idesc0, sfa + (kk >> 1) * 4, sfb + (kk >> 1) * Cfg::kSfN,
                            (kb > kb0 || kk > 0) ? 1u : 0u);
-          }
           commit_to<MODE>(elected, empty_bar(stage));
-          if (last_half) commit_to<MODE>(elected, sf_used_bar(b));
           if (kb + 1 == kb1) commit_to<MODE>(elected, acc_full_bar(acc));
           if (++stage == Cfg::kStages) { stage = 0; phase ^= 1u; }
-          if (first_half && ++sf == Cfg::kSfStages) { sf = 0; sf_phase ^= 1u; }
-          if (last_half && ++b == Cfg::kSfBufs) { b = 0; b_phase ^= 1u; }
+          if (sf_done && ++sf == Cfg::kSfStages) { sf = 0; sf_phase ^= 1u; }
+          here = mbar_test(full_bar(stage), phase);
+          sf_here = sf_done && mbar_test(sf_ready_bar(sf), sf_phase);
         }
         if (++acc == Cfg::kAccs) { acc = 0; acc_phase ^= 1u; }
       }
@@ -535,6 +583,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!mbar_wait(acc_full_bar(acc), acc_phase, abort_flag, p.err)) break;
       tc_fence_after();
       const uint32_t src = tmem + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>(acc * BN);
+      auto release = [&]() {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if constexpr (PAIR) mbar_arrive_leader(map_to_cta(acc_empty_bar(acc), 0));
+          else mbar_arrive(acc_empty_bar(acc));
+        }
+      };
       if constexpr (SWAP) {                           // lane = column of C, register = row
         const int64_t col = t.n0 + quad * 32 + lane;
         const bool col_ok = col < p.n;
@@ -584,15 +640,15 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (lane < team) mbar_arrive_cluster(map_to_cta(red_empty, lane));
           red_phase ^= 1u;
         }
+        release();
       } else {
         const int row0 = t.row0 + (PAIR ? rank * kTileM : 0) + quad * 32;
-        if (row0 < t.row_end) store_rows<BN>(p, &tmap_out, src, t, row0, lane, stage, stage_addr, nstores);
-      }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        if constexpr (PAIR) mbar_arrive_leader(map_to_cta(acc_empty_bar(acc), 0));
-        else mbar_arrive(acc_empty_bar(acc));
+        if (row0 < t.row_end) {
+          RowWriter out(p, &tmap_out, t, row0, lane, stage, stage_addr, nstores);
+          store_rows<BN, Cfg::kAccs == 1>(p, out, src, t, lane, release);
+        } else {
+          release();
+        }
       }
       if (++acc == Cfg::kAccs) { acc = 0; acc_phase ^= 1u; }
     }
