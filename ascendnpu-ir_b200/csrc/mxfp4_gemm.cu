@@ -7,17 +7,17 @@
 // into the f32 accumulator, four times the rate of a 16-bit product.  Codes come by TMA into 128-byte-swizzled tiles
 // (a 128-byte row is 256 elements of K); the exponents have to lie in tensor memory: row r of an operand tile at lane
 // r % 32, column r / 32, four bytes (128 elements of K) a cell, the same in all four lane quadrants.  The exponent
-// matrices keep the plain [rows, K / 32] layout, so groups may start at any row: TMA brings [rows x 16 bytes] (512
-// elements of K), a warp per 128 rows turns them in shared memory from a row's four words into a lane's four rows, and
+// matrices keep the plain [rows, K / 32] layout, so groups may start at any row: TMA brings [rows x 32 bytes] (1024
+// elements of K), a warp per 128 rows turns them in shared memory from a row's eight words into a lane's four rows, and
 // the MMA issuer copies them to tensor memory with tcgen05.cp ahead of the instructions that use them.  (Warps storing
 // them to tensor memory themselves were the first form: next to cta_group::2 instructions such a store took 1400
 // cycles, and a chunk of 512 elements of K is 1024 of multiplication.)
 //
 // A persistent kernel, one CTA per SM, 288 threads:
-//   warp 0      TMA producer of codes (a ring of stages of 256 elements of K) and exponents (a ring of 512)
+//   warp 0      TMA producer of codes (a ring of stages of 256 elements of K) and exponents (a ring of 1024)
 //   warp 1      issuer of tcgen05.cp and tcgen05.mma
 //   warps 2-5   epilogue: accumulator -> bias -> rounding -> C
-//   warps 6-8   exponents: rows of four words -> lanes of four rows, 128 rows a warp
+//   warps 6-8   exponents: rows of eight words -> lanes of four rows, 128 rows a warp
 // in three forms:
 //   kPair    256 rows of A x BN columns of C on two CTAs (cta_group::2): each holds its 128 rows of A and half of the
 //            tile's rows of B, so that an SM's shared memory is read and filled for B half as often;
@@ -33,6 +33,7 @@ namespace {
 
 constexpr int kTileM = 128;
 constexpr int kStageK = 256;       // elements of K a stage: one 128-byte swizzle row of codes
+constexpr int kChunk = 4;           // stages that a piece of exponents lasts: 32 bytes (a sector) of each row
 constexpr int kThreads = 288;
 constexpr int kMaxGroups = 1024;
 enum MxMode { kSingle, kPair, kFew };
@@ -57,8 +58,8 @@ struct MxCfg {
   static constexpr int kNRows = MODE == kPair ? BN / 2 : BN;         // rows of the N side's codes in this CTA
   static constexpr int kStage = (kTileM + kNRows) * 128;
   static constexpr int kSfBlocks = 1 + (BN + 127) / 128;             // blocks of 128 rows of exponents: M side, N side
-  static constexpr int kSfStage = kSfBlocks * 2048;
-  static constexpr int kSfStages = 3;
+  static constexpr int kSfStage = kSfBlocks * 4096;
+  static constexpr int kSfStages = 2;
   static constexpr int kAccs = BN > 192 ? 1 : 2;
   // columns of tensor memory: accumulators, then each stage's exponents: two words (128 elements of K each) of four
   // columns a block, the N side's first
@@ -447,12 +448,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   const int total_tiles = tile_start[p.groups];
-  // this CTA's chunks of 512 elements of K
-  const int all_chunks = (p.k_blocks + 1) / 2;
+  // this CTA's chunks of kChunk stages
+  const int all_chunks = (p.k_blocks + kChunk - 1) / kChunk;
   const int per = SWAP ? (all_chunks + team - 1) / team : all_chunks;
   const int chunk0 = SWAP ? rank * per : 0;
   const int chunk1 = min(all_chunks, chunk0 + per);
-  const int kb0 = 2 * chunk0, kb1 = min(p.k_blocks, 2 * chunk1);       // its stages
+  const int kb0 = kChunk * chunk0, kb1 = min(p.k_blocks, kChunk * chunk1);       // its stages
   int group = 0;
   MxTile t;
 
@@ -468,12 +469,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int n0 = SWAP ? t.row0 : t.n0 + (PAIR ? rank * Cfg::kNRows : 0);
         const int zm = SWAP ? t.group : 0, zn = SWAP ? 0 : t.group;
         for (int kb = kb0; kb < kb1; ++kb) {
-          if ((kb & 1) == 0) {
+          if (kb % kChunk == 0) {
             if (!mbar_wait(sf_empty_bar(sf), sf_phase ^ 1u, abort_flag, p.err)) { ok = false; break; }
             const uint32_t dst = base + Cfg::kSfOff + sf * Cfg::kSfStage;
-            mbar_expect_tx(sf_full_bar(sf), (kTileM + BN) * 16);
+            mbar_expect_tx(sf_full_bar(sf), (kTileM + BN) * 32);
             tma_load_3d(dst, &tmap_sm, kb * (kStageK / 32), m0, zm, sf_full_bar(sf));
-            tma_load_3d(dst + kTileM * 16, &tmap_sn, kb * (kStageK / 32), SWAP ? t.row0 : t.n0, zn, sf_full_bar(sf));
+            tma_load_3d(dst + kTileM * 32, &tmap_sn, kb * (kStageK / 32), SWAP ? t.row0 : t.n0, zn, sf_full_bar(sf));
             if (++sf == Cfg::kSfStages) { sf = 0; sf_phase ^= 1u; }
           }
           if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag, p.err)) { ok = false; break; }
@@ -512,22 +513,22 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!mbar_wait(acc_empty_bar(acc), acc_phase ^ 1u, abort_flag, p.err)) break;
         const uint32_t d = tmem + static_cast<uint32_t>(acc * BN);
         for (int kb = kb0; kb < kb1; ++kb) {
-          const uint32_t half = static_cast<uint32_t>(kb & 1);          // of the chunk
+          const uint32_t part = static_cast<uint32_t>(kb) % kChunk;          // of the chunk
           // the next barriers were looked at while the last stage's instructions went out
-          if (half == 0 && !sf_here && !mbar_wait(sf_ready_bar(sf), sf_phase, abort_flag, p.err)) { ok = false; break; }
+          if (part == 0 && !sf_here && !mbar_wait(sf_ready_bar(sf), sf_phase, abort_flag, p.err)) { ok = false; break; }
           if (!here && !mbar_wait(full_bar(stage), phase, abort_flag, p.err)) { ok = false; break; }
           tc_fence_after();
           // the stage's codes have landed, so the instructions that used its columns of exponents before are done
           const uint32_t sfb = tmem + static_cast<uint32_t>(Cfg::kSfBase + stage * Cfg::kSfCols), sfa = sfb + 2 * Cfg::kSfN;
-          const uint32_t sfs = base + Cfg::kSfOff + sf * Cfg::kSfStage + half * 1024;
+          const uint32_t sfs = base + Cfg::kSfOff + sf * Cfg::kSfStage + part * 1024;
           const uint32_t sm = desc_lo(base) + static_cast<uint32_t>(stage) * (Cfg::kStage >> 4), sn = sm + kTileM * 8;
 #pragma unroll
           for (int w = 0; w < 2; ++w) {
             tmem_copy<MODE>(elected, sfa + w * 4, sfs + w * 512);
 #pragma unroll
-            for (int i = 1; i < Cfg::kSfBlocks; ++i) tmem_copy<MODE>(elected, sfb + w * Cfg::kSfN + (i - 1) * 4, sfs + i * 2048 + w * 512);
+            for (int i = 1; i < Cfg::kSfBlocks; ++i) tmem_copy<MODE>(elected, sfb + w * Cfg::kSfN + (i - 1) * 4, sfs + i * 4096 + w * 512);
           }
-          const bool sf_done = half == 1 || kb + 1 == kb1;
+          const bool sf_done = part == kChunk - 1 || kb + 1 == kb1;
           if (sf_done) commit_to<MODE>(elected, sf_empty_bar(sf));
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk)
@@ -553,13 +554,22 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int tile = first_tile; tile < total_tiles && ok; tile += tile_step) {
         for (int c = chunk0; c < chunk1; ++c) {
           if (!mbar_wait(sf_full_bar(sf), sf_phase, abort_flag, p.err)) { ok = false; break; }
-          uint4 *rows = reinterpret_cast<uint4 *>(gen + Cfg::kSfOff + sf * Cfg::kSfStage + block * 2048);
-          const uint4 r0 = rows[lane], r1 = rows[32 + lane], r2 = rows[64 + lane], r3 = rows[96 + lane];
+          uint4 *rows = reinterpret_cast<uint4 *>(gen + Cfg::kSfOff + sf * Cfg::kSfStage + block * 4096);
+          uint4 lo[4], hi[4];                          // rows lane, 32 + lane, ..: words 0-3 and 4-7
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            lo[j] = rows[2 * (32 * j + lane)];
+            hi[j] = rows[2 * (32 * j + lane) + 1];
+          }
           __syncwarp();
-          rows[lane] = make_uint4(r0.x, r1.x, r2.x, r3.x);
-          rows[32 + lane] = make_uint4(r0.y, r1.y, r2.y, r3.y);
-          rows[64 + lane] = make_uint4(r0.z, r1.z, r2.z, r3.z);
-          rows[96 + lane] = make_uint4(r0.w, r1.w, r2.w, r3.w);
+          rows[lane] = make_uint4(lo[0].x, lo[1].x, lo[2].x, lo[3].x);
+          rows[32 + lane] = make_uint4(lo[0].y, lo[1].y, lo[2].y, lo[3].y);
+          rows[64 + lane] = make_uint4(lo[0].z, lo[1].z, lo[2].z, lo[3].z);
+          rows[96 + lane] = make_uint4(lo[0].w, lo[1].w, lo[2].w, lo[3].w);
+          rows[128 + lane] = make_uint4(hi[0].x, hi[1].x, hi[2].x, hi[3].x);
+          rows[160 + lane] = make_uint4(hi[0].y, hi[1].y, hi[2].y, hi[3].y);
+          rows[192 + lane] = make_uint4(hi[0].z, hi[1].z, hi[2].z, hi[3].z);
+          rows[224 + lane] = make_uint4(hi[0].w, hi[1].w, hi[2].w, hi[3].w);
           fence_proxy_async();
           __syncwarp();
           if (lane == 0) {
@@ -679,8 +689,8 @@ int32_t launch_mx(const MxOperand &a, const MxOperand &b, int64_t k, MxParams p,
   const int eb = dtype_bytes(p.out_dtype);
   if (!make_byte_tmap3(&tm, om.codes, kb, om.rows, om.batch, om.code_stride, om.code_bs, 128, kTileM, true) ||
       !make_byte_tmap3(&tn, on.codes, kb, on.rows, on.batch, on.code_stride, on.code_bs, 128, Cfg::kNRows, true) ||
-      !make_byte_tmap3(&tsm, om.scales, ks, om.rows, om.batch, om.scale_stride, om.scale_bs, 16, kTileM, false) ||
-      !make_byte_tmap3(&tsn, on.scales, ks, on.rows, on.batch, on.scale_stride, on.scale_bs, 16, BN, false) ||
+      !make_byte_tmap3(&tsm, om.scales, ks, om.rows, om.batch, om.scale_stride, om.scale_bs, 32, kTileM, false) ||
+      !make_byte_tmap3(&tsn, on.scales, ks, on.rows, on.batch, on.scale_stride, on.scale_bs, 32, BN, false) ||
       (MODE != kFew && p.tma_out && !make_byte_tmap(&tout, p.out, p.n * eb, p.m, p.ldo * eb, 32)))
     return fail(BSIR_ERR_STRIDE, "matmul_mxfp4: the driver refuses a tensor map of these sizes and strides");
   cudaFuncSetAttribute(mxfp4_gemm_kernel<BN, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmem);
@@ -761,7 +771,7 @@ extern "C" int32_t bsir_matmul_mxfp4(const bsir_matmul_mxfp4_desc *d, void *stre
   const int sms = device_info().sm_count > 0 ? device_info().sm_count : 148;
   auto split_of = [&](int64_t nt) {
     if (std::getenv("MX_SPLIT")) return atoi(std::getenv("MX_SPLIT"));
-    const int chunks = (p.k_blocks + 1) / 2;
+    const int chunks = static_cast<int>(ceil_div(p.k_blocks, kChunk));
     int s = 1;
     while (s < 8 && nt * s * 2 <= sms && ceil_div(chunks, 2 * s) * (2 * s - 1) < chunks) s *= 2;
     return s;
