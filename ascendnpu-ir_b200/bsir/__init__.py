@@ -105,6 +105,15 @@ def lib() -> C.CDLL:
         L.bsir_reduce_with_index_workspace_bytes.restype = C.c_int64
         L.bsir_matmul_w8a8_workspace_bytes.restype = C.c_int64
         L.bsir_fused_elementwise_source.restype = C.c_int64
+        # functions that take plain Python numbers and addresses
+        i, n, p = C.c_int32, C.c_int64, C.c_void_p
+        L.bsir_quant_mxfp4.argtypes = (i, n, n, p, n, p, n, p, n, p, n, p, n, p)
+        L.bsir_dequant_mxfp4.argtypes = (i, n, n, p, n, p, n, p, n, p)
+        L.bsir_matmul_mxfp4.argtypes = (p, p)
+        L.bsir_expert_sort.argtypes = (i, n, n, n, p, p, p, p)
+        L.bsir_expert_dispatch.argtypes = (i, n, n, n, p, n, p, n, p, n, p)
+        L.bsir_expert_combine.argtypes = (i, n, n, n, n, p, n, p, i, p, p, n, p)
+        L.bsir_expert_combine_grad.argtypes = (i, n, n, n, n, p, n, p, n, p, i, p, p, n, p, p)
         _lib = L
     return _lib
 
@@ -115,7 +124,8 @@ def _check(rc: int) -> None:
 
 
 def _stream() -> C.c_void_p:
-    return C.c_void_p(torch.cuda.current_stream().cuda_stream)
+    # the raw handle of torch's current stream; torch.cuda.current_stream() builds a Stream object around it (3.4 us)
+    return C.c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
 
 
 def _dt(t: torch.Tensor) -> int:
@@ -489,9 +499,11 @@ class FusedChain:
 def _rows(x: torch.Tensor):
     if x.dim() != 2:
         raise BsirError(-2, "expected a 2-D tensor")
-    if x.shape[1] > 1 and x.stride(1) != 1:
+    rows, cols = x.shape
+    pitch, inner = x.stride()
+    if cols > 1 and inner != 1:
         raise BsirError(-3, "innermost dimension must be unit-stride")
-    return x.shape[0], x.shape[1], (x.stride(0) if x.shape[0] > 1 else max(x.shape[1], 1))
+    return rows, cols, (pitch if rows > 1 else max(cols, 1))
 
 
 def reduce(kind: str, x: torch.Tensor, dim: int = 1, out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -748,28 +760,34 @@ def matmul_w4a16(a: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, z
 
 
 # ---------------------------------------------------------------------------- microscaled 4-bit floats (MXFP4)
-def _on_device(*ts: Optional[torch.Tensor]) -> None:
-    """The operands must live on the current CUDA device, whose stream the call goes to."""
-    cur = torch.cuda.current_device()
+def _current(*ts: Optional[torch.Tensor]) -> int:
+    """The current stream's handle; the operands must live on the current CUDA device, whose stream the call goes to."""
+    dev = ts[0].get_device()                 # -1: not a CUDA tensor
     for t in ts:
-        if t is not None and (not t.is_cuda or t.device.index != cur):
-            raise BsirError(-9, f"an operand is on {t.device}, the current device is cuda:{cur}")
+        if t is not None and t.get_device() != dev:
+            raise BsirError(-9, f"operands on {ts[0].device} and {t.device}")
+    if dev < 0 or dev != torch._C._cuda_getDevice():
+        raise BsirError(-9, f"the operands are on {ts[0].device}, which is not the current CUDA device")
+    return torch._C._cuda_getCurrentRawStream(dev)
 
 
-def _code_rows(rows: int, cols: int, device) -> torch.Tensor:
+def _code_rows(rows: int, cols: int, like: torch.Tensor) -> torch.Tensor:
     """uint8 [rows, cols] with 16-byte aligned rows, as the products want codes and exponents."""
-    return torch.empty((rows, (cols + 15) // 16 * 16), dtype=torch.uint8, device=device)[:, :cols]
+    if cols % 16 == 0:
+        return like.new_empty((rows, cols), dtype=torch.uint8)
+    return like.new_empty((rows, (cols + 15) // 16 * 16), dtype=torch.uint8)[:, :cols]
 
 
 def _byte_rows(t: torch.Tensor, rows: int, cols: int, what: str) -> int:
     """Row stride of a uint8 [rows, cols] tensor with contiguous rows."""
     if t.dtype != torch.uint8:
         raise BsirError(-4, f"{what}: expected uint8, got {t.dtype}")
-    if tuple(t.shape) != (rows, cols):
+    if t.shape != (rows, cols):
         raise BsirError(-2, f"{what}: expected [{rows}, {cols}], got {list(t.shape)}")
-    if cols > 1 and t.stride(1) != 1:
+    st = t.stride()
+    if cols > 1 and st[1] != 1:
         raise BsirError(-3, f"{what}: innermost dimension must be unit-stride")
-    return t.stride(0) if rows > 1 else max(cols, 1)
+    return st[0] if rows > 1 else max(cols, 1)
 
 
 def _quant_mxfp4(x: torch.Tensor, along: bool, down: bool, outs: Sequence[Optional[torch.Tensor]]):
@@ -777,15 +795,15 @@ def _quant_mxfp4(x: torch.Tensor, along: bool, down: bool, outs: Sequence[Option
     res, args = [], []
     for want, r, c, q, s in ((along, rows, cols, outs[0], outs[1]), (down, cols, rows, outs[2], outs[3])):
         if not want:
-            args += [C.c_void_p(0), C.c_int64(0), C.c_void_p(0), C.c_int64(0)]
+            args += (None, 0, None, 0)
             continue
-        q = _code_rows(r, (c + 1) // 2, x.device) if q is None else q
-        s = _code_rows(r, (c + 31) // 32, x.device) if s is None else s
-        args += [_ptr(q), C.c_int64(_byte_rows(q, r, (c + 1) // 2, "quant_mxfp4: codes")),
-                 _ptr(s), C.c_int64(_byte_rows(s, r, (c + 31) // 32, "quant_mxfp4: exponents"))]
-        res += [q, s]
-    _on_device(x, *res)
-    _check(lib().bsir_quant_mxfp4(_dt(x), C.c_int64(rows), C.c_int64(cols), _ptr(x), C.c_int64(rs), *args, _stream()))
+        qc, sc = (c + 1) // 2, (c + 31) // 32
+        q = _code_rows(r, qc, x) if q is None else q
+        s = _code_rows(r, sc, x) if s is None else s
+        args += (q.data_ptr(), _byte_rows(q, r, qc, "quant_mxfp4: codes"), s.data_ptr(), _byte_rows(s, r, sc, "quant_mxfp4: exponents"))
+        res += (q, s)
+    stream = _current(x, *res)
+    _check(lib().bsir_quant_mxfp4(_dt(x), rows, cols, x.data_ptr(), rs, *args, stream))
     return tuple(res)
 
 
@@ -822,9 +840,8 @@ def dequant_mxfp4(q: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype = tor
     orows, ocols, os_ = _rows(out)
     if (orows, ocols) != (rows, cols):
         raise BsirError(-2, f"dequant_mxfp4: out {list(out.shape)} for [{rows}, {cols}]")
-    _on_device(q, scale, out)
-    _check(lib().bsir_dequant_mxfp4(_dt(out), C.c_int64(rows), C.c_int64(cols), _ptr(q), C.c_int64(qs), _ptr(scale), C.c_int64(ss),
-                                    _ptr(out), C.c_int64(os_), _stream()))
+    stream = _current(q, scale, out)
+    _check(lib().bsir_dequant_mxfp4(_dt(out), rows, cols, q.data_ptr(), qs, scale.data_ptr(), ss, out.data_ptr(), os_, stream))
     return out
 
 
@@ -851,36 +868,39 @@ def matmul_mxfp4(a: torch.Tensor, scale_a: torch.Tensor, b: torch.Tensor, scale_
     m, kb = a.shape
     n, groups = b.shape[-2], b.shape[0] if offsets is not None else 1
     ks = (2 * kb + 31) // 32
-    d = MatmulMxfp4Desc()
-    d.lda = _byte_rows(a, m, kb, "matmul_mxfp4: a")
-    d.ldsa = _byte_rows(scale_a, m, ks, "matmul_mxfp4: scale_a")
-    if b.shape[-1] != kb or tuple(scale_b.shape) != (*b.shape[:-1], ks):
+    lda = _byte_rows(a, m, kb, "matmul_mxfp4: a")
+    ldsa = _byte_rows(scale_a, m, ks, "matmul_mxfp4: scale_a")
+    if b.shape[-1] != kb or scale_b.shape != (*b.shape[:-1], ks):
         raise BsirError(-2, f"matmul_mxfp4: b {list(b.shape)} and scale_b {list(scale_b.shape)} for {kb} bytes of codes and {ks} exponents a row")
-    b2, s2 = (b, scale_b) if offsets is None else (b[0], scale_b[0]) if groups else (b.reshape(0, kb), scale_b.reshape(0, ks))
-    d.ldb = _byte_rows(b2, n, kb, "matmul_mxfp4: b")
-    d.ldsb = _byte_rows(s2, n, ks, "matmul_mxfp4: scale_b")
+    if b.dtype != torch.uint8 or scale_b.dtype != torch.uint8:
+        raise BsirError(-4, f"matmul_mxfp4: b is {b.dtype}, scale_b {scale_b.dtype}, expected uint8")
+    bst, sbst = b.stride(), scale_b.stride()
+    if (kb > 1 and bst[-1] != 1) or (ks > 1 and sbst[-1] != 1):
+        raise BsirError(-3, "matmul_mxfp4: innermost dimension of b and scale_b must be unit-stride")
+    ldb, ldsb = (bst[-2], sbst[-2]) if n > 1 else (max(kb, 1), max(ks, 1))
     if out is None:
-        out = torch.empty((m, n), dtype=out_dtype or torch.bfloat16, device=a.device)
+        out = a.new_empty((m, n), dtype=out_dtype or torch.bfloat16)
     elif out_dtype is not None and out.dtype != out_dtype:
         raise BsirError(-4, f"matmul_mxfp4: out is {out.dtype}, out_dtype {out_dtype}")
-    orows, ocols, d.ldo = _rows(out)
+    orows, ocols, ldo = _rows(out)
     if (orows, ocols) != (m, n):
         raise BsirError(-2, f"matmul_mxfp4: out {list(out.shape)} for [{m}, {n}]")
+    bsb = bssb = bias_stride = 0
     if offsets is not None:
-        if offsets.dtype != torch.int32 or offsets.dim() != 1 or offsets.shape[0] != groups + 1 or not offsets.is_contiguous():
+        if offsets.dtype != torch.int32 or offsets.shape != (groups + 1,) or not offsets.is_contiguous():
             raise BsirError(-2, f"matmul_mxfp4: offsets must be contiguous int32 [{groups + 1}]")
-        d.offsets, d.groups = offsets.data_ptr(), groups
-        d.batch_stride_b, d.batch_stride_sb = b.stride(0), scale_b.stride(0)
+        bsb, bssb = bst[0], sbst[0]
     if bias is not None:
         if bias.shape[-1] != n or bias.dim() not in (1, 2) or (bias.dim() == 2 and (offsets is None or bias.shape[0] != groups)):
             raise BsirError(-2, f"matmul_mxfp4: bias {list(bias.shape)} for {n} columns")
         if n > 1 and bias.stride(-1) != 1:
             raise BsirError(-3, "matmul_mxfp4: innermost dimension of bias must be unit-stride")
-        d.bias, d.bias_dtype, d.bias_stride = bias.data_ptr(), _dt(bias), (bias.stride(0) if bias.dim() == 2 else 0)
-    _on_device(a, scale_a, b, scale_b, out, bias, offsets)
-    d.out_dtype, d.m, d.n, d.k = _dt(out), m, n, 2 * kb
-    d.a, d.scale_a, d.b, d.scale_b, d.out = a.data_ptr(), scale_a.data_ptr(), b.data_ptr(), scale_b.data_ptr(), out.data_ptr()
-    _check(lib().bsir_matmul_mxfp4(C.byref(d), _stream()))
+        bias_stride = bias.stride(0) if bias.dim() == 2 else 0
+    stream = _current(a, scale_a, b, scale_b, out, bias, offsets)
+    d = MatmulMxfp4Desc(_dt(out), F32 if bias is None else _dt(bias), m, n, 2 * kb, a.data_ptr(), lda, scale_a.data_ptr(), ldsa,
+                        b.data_ptr(), ldb, bsb, scale_b.data_ptr(), ldsb, bssb, None if bias is None else bias.data_ptr(), bias_stride,
+                        None if offsets is None else offsets.data_ptr(), groups, out.data_ptr(), ldo)
+    _check(lib().bsir_matmul_mxfp4(C.byref(d), stream))
     return out
 
 
@@ -909,9 +929,8 @@ def expert_sort(ids: torch.Tensor, experts: int, offsets: Optional[torch.Tensor]
         raise BsirError(-2, f"expert_sort: offsets must be contiguous int32 [{experts + 1}]")
     if _choices(slots, "expert_sort") != ids.shape:
         raise BsirError(-2, f"expert_sort: slots {list(slots.shape)} for ids {list(ids.shape)}")
-    _on_device(ids, offsets, slots)
-    _check(lib().bsir_expert_sort(_dt(ids), C.c_int64(tokens), C.c_int64(top_k), C.c_int64(experts), _ptr(ids), _ptr(offsets), _ptr(slots),
-                                  _stream()))
+    stream = _current(ids, offsets, slots)
+    _check(lib().bsir_expert_sort(_dt(ids), tokens, top_k, experts, ids.data_ptr(), offsets.data_ptr(), slots.data_ptr(), stream))
     return offsets, slots
 
 
@@ -926,9 +945,8 @@ def expert_dispatch(x: torch.Tensor, slots: torch.Tensor, out: Optional[torch.Te
     orows, ocols, os_ = _rows(out)
     if ocols != cols or out.dtype != x.dtype:
         raise BsirError(-2, f"expert_dispatch: out {list(out.shape)} {out.dtype} for {cols} columns of {x.dtype}")
-    _on_device(x, slots, out)
-    _check(lib().bsir_expert_dispatch(_dt(x), C.c_int64(tokens), C.c_int64(top_k), C.c_int64(cols), _ptr(x), C.c_int64(rs), _ptr(slots),
-                                      C.c_int64(orows), _ptr(out), C.c_int64(os_), _stream()))
+    stream = _current(x, slots, out)
+    _check(lib().bsir_expert_dispatch(_dt(x), tokens, top_k, cols, x.data_ptr(), rs, slots.data_ptr(), orows, out.data_ptr(), os_, stream))
     return out
 
 
@@ -943,9 +961,9 @@ def expert_combine(y: torch.Tensor, slots: torch.Tensor, weights: Optional[torch
     orows, ocols, os_ = _rows(out)
     if (orows, ocols) != (tokens, cols) or out.dtype != y.dtype:
         raise BsirError(-2, f"expert_combine: out {list(out.shape)} {out.dtype} for [{tokens}, {cols}] of {y.dtype}")
-    _on_device(y, slots, weights, out)
-    _check(lib().bsir_expert_combine(_dt(y), C.c_int64(tokens), C.c_int64(top_k), C.c_int64(cols), C.c_int64(rows), _ptr(y), C.c_int64(ys),
-                                     _ptr(slots), wdt, _ptr(weights), _ptr(out), C.c_int64(os_), _stream()))
+    stream = _current(y, slots, weights, out)
+    _check(lib().bsir_expert_combine(_dt(y), tokens, top_k, cols, rows, y.data_ptr(), ys, slots.data_ptr(), wdt,
+                                     None if weights is None else weights.data_ptr(), out.data_ptr(), os_, stream))
     return out
 
 
@@ -967,10 +985,9 @@ def expert_combine_grad(dout: torch.Tensor, y: torch.Tensor, slots: torch.Tensor
         raise BsirError(-2, f"expert_combine_grad: out {list(dy.shape)} {dy.dtype} for [{rows}, {cols}] of {y.dtype}")
     if dw.dtype != torch.float32 or dw.shape != slots.shape or not dw.is_contiguous():
         raise BsirError(-2, f"expert_combine_grad: dweights must be contiguous f32 {list(slots.shape)}")
-    _on_device(dout, y, slots, weights, dy, dw)
-    _check(lib().bsir_expert_combine_grad(_dt(y), C.c_int64(tokens), C.c_int64(top_k), C.c_int64(cols), C.c_int64(rows), _ptr(dout),
-                                          C.c_int64(ds), _ptr(y), C.c_int64(ys), _ptr(slots), wdt, _ptr(weights), _ptr(dy), C.c_int64(dys),
-                                          _ptr(dw), _stream()))
+    stream = _current(dout, y, slots, weights, dy, dw)
+    _check(lib().bsir_expert_combine_grad(_dt(y), tokens, top_k, cols, rows, dout.data_ptr(), ds, y.data_ptr(), ys, slots.data_ptr(), wdt,
+                                          None if weights is None else weights.data_ptr(), dy.data_ptr(), dys, dw.data_ptr(), stream))
     return dy, dw
 
 
