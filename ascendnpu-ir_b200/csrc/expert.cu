@@ -168,20 +168,35 @@ struct RowParams {
   float *dw;
   int *err;
 };
-// slot of choice j, -1 when masked; numbers that name no row are masked too and reported
-__device__ __forceinline__ int64_t load_slot(const RowParams &p, int64_t t, int j) {
-  const int32_t s = p.slots[t * p.top_k + j];
-  if (s >= 0 && s < p.rows) return s;
-  if (s != -1 && threadIdx.x == 0) atomicOr(p.err, BSIR_DEVERR_GATHER_INDEX);
-  return -1;
-}
-__device__ __forceinline__ float load_weight(const RowParams &p, int64_t t, int j) {
-  if (!p.w) return 1.0f;
-  const int64_t i = t * p.top_k + j;
-  if (p.w_dtype == BSIR_F32) return static_cast<const float *>(p.w)[i];
-  const unsigned short h = static_cast<const unsigned short *>(p.w)[i];
-  return p.w_dtype == BSIR_F16 ? __half2float(__ushort_as_half(h)) : __uint_as_float(static_cast<uint32_t>(h) << 16);
-}
+// The choices of a token, 32 at a time: lane j holds the slot (-1: masked; so is a number that names no row, which is
+// reported) and the weight of choice j0 + j, loaded before the rows they lead to and handed round by shuffles.
+struct Choices {
+  int32_t slot;
+  float weight;
+  __device__ __forceinline__ void load(const RowParams &p, int64_t t, int j0) {
+    const int lane = threadIdx.x & 31;
+    slot = -1;
+    weight = 1.0f;
+    if (j0 + lane >= p.top_k) return;
+    const int64_t i = t * p.top_k + j0 + lane;
+    const int32_t s = p.slots[i];
+    if (s >= 0 && s < p.rows) {
+      slot = s;
+      if (p.w) {
+        if (p.w_dtype == BSIR_F32) {
+          weight = static_cast<const float *>(p.w)[i];
+        } else {
+          const unsigned short h = static_cast<const unsigned short *>(p.w)[i];
+          weight = p.w_dtype == BSIR_F16 ? __half2float(__ushort_as_half(h)) : __uint_as_float(static_cast<uint32_t>(h) << 16);
+        }
+      }
+    } else if (s != -1) {
+      atomicOr(p.err, BSIR_DEVERR_GATHER_INDEX);
+    }
+  }
+  __device__ __forceinline__ int32_t slot_of(int j) const { return __shfl_sync(0xffffffffu, slot, j); }
+  __device__ __forceinline__ float weight_of(int j) const { return __shfl_sync(0xffffffffu, weight, j); }
+};
 
 // Rows as pieces of type T (16 bytes where everything is aligned to it): a thread holds four pieces of the token's row
 // and stores them to each of its rows.
@@ -192,6 +207,8 @@ __global__ void __launch_bounds__(kMoveThreads) expert_dispatch_kernel(RowParams
   pdl_wait();
   for (int64_t t = blockIdx.x; t < p.tokens; t += gridDim.x) {
     const T *src = static_cast<const T *>(p.x) + t * p.xs;
+    Choices ch;
+    ch.load(p, t, 0);
     for (int64_t c0 = static_cast<int64_t>(blockIdx.y) * (kMoveThreads * 4); c0 < p.cols; c0 += static_cast<int64_t>(gridDim.y) * (kMoveThreads * 4)) {
       T v[4];
       const int64_t c = c0 + threadIdx.x;
@@ -199,7 +216,8 @@ __global__ void __launch_bounds__(kMoveThreads) expert_dispatch_kernel(RowParams
       for (int u = 0; u < 4; ++u)
         if (c + u * kMoveThreads < p.cols) v[u] = src[c + u * kMoveThreads];
       for (int j = 0; j < p.top_k; ++j) {
-        const int64_t s = load_slot(p, t, j);
+        if (p.top_k > 32 && j % 32 == 0) ch.load(p, t, j);
+        const int64_t s = ch.slot_of(j % 32);
         if (s < 0) continue;
         T *dst = static_cast<T *>(p.out) + s * p.os;
 #pragma unroll
@@ -210,7 +228,7 @@ __global__ void __launch_bounds__(kMoveThreads) expert_dispatch_kernel(RowParams
   }
 }
 
-// A thread takes kE elements (16 bytes when kE > 1) of a token's row and runs over its choices, four of y's rows in
+// A thread takes kE elements (16 bytes when kE > 1) of a token's row and runs over its choices, eight of y's rows in
 // flight at a time.
 template <int DT, bool VEC> struct RowVec {
   static constexpr int kPer = FloatTraits<DT>::kPerWord;
@@ -260,69 +278,76 @@ __global__ void __launch_bounds__(kMoveThreads) expert_combine_kernel(RowParams 
   pdl_launch_dependents();
   pdl_wait();
   for (int64_t t = blockIdx.x; t < p.tokens; t += gridDim.x) {
-    for (int64_t c = (static_cast<int64_t>(blockIdx.y) * kMoveThreads + threadIdx.x) * kE; c < p.cols;
-         c += static_cast<int64_t>(gridDim.y) * kMoveThreads * kE) {
+    Choices ch;
+    ch.load(p, t, 0);
+    // the warp stays together for the shuffles: lanes behind the row's end go along without loading
+    for (int64_t c0 = static_cast<int64_t>(blockIdx.y) * kMoveThreads * kE; c0 < p.cols; c0 += static_cast<int64_t>(gridDim.y) * kMoveThreads * kE) {
+      const int64_t c = c0 + threadIdx.x * kE;
+      const bool in = c < p.cols;
       float acc[kE];
 #pragma unroll
       for (int i = 0; i < kE; ++i) acc[i] = 0.0f;
-      for (int j0 = 0; j0 < p.top_k; j0 += 4) {
-        V v[4];
-        float w[4];
-        bool live[4];
+      for (int j0 = 0; j0 < p.top_k; j0 += 8) {
+        if (p.top_k > 32 && j0 % 32 == 0) ch.load(p, t, j0);
+        V v[8];
+        uint32_t live = 0;
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int64_t s = j0 + u < p.top_k ? load_slot(p, t, j0 + u) : -1;
-          live[u] = s >= 0;
-          if (live[u]) {
-            w[u] = load_weight(p, t, j0 + u);
-            v[u].load(p.y, s * p.ys + c);
+        for (int u = 0; u < 8; ++u) {
+          const int64_t s = ch.slot_of((j0 + u) % 32);      // lanes behind the last choice hold -1
+          if (s >= 0) {
+            live |= 1u << u;
+            if (in) v[u].load(p.y, s * p.ys + c);
           }
         }
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          if (!live[u]) continue;
+        for (int u = 0; u < 8; ++u) {
+          const float w = ch.weight_of((j0 + u) % 32);
+          if (!(live >> u & 1u) || !in) continue;
           float f[kE];
           v[u].get(f);
 #pragma unroll
-          for (int i = 0; i < kE; ++i) acc[i] = __fmaf_rn(w[u], f[i], acc[i]);
+          for (int i = 0; i < kE; ++i) acc[i] = __fmaf_rn(w, f[i], acc[i]);
         }
       }
-      V::store(p.out, t * p.os + c, acc);
+      if (in) V::store(p.out, t * p.os + c, acc);
     }
   }
 }
 
-// One CTA per token: dout's row stays in registers for four choices at a time, y's rows are read once, dy's written
-// once; the dot products meet across the warps in a fixed order.
-constexpr int kGradThreads = 256;
+// One CTA per token, four choices at a time (eight took 120 registers and 267 us where four take 190): y's rows are
+// read once, dy's written once, dout's once for the four; the dot products meet across the warps in a fixed order.
+constexpr int kGradThreads = 128;
+constexpr int kGradChoices = 4;
 template <int DT, bool VEC>
 __global__ void __launch_bounds__(kGradThreads) expert_combine_grad_kernel(RowParams p) {
   using V = RowVec<DT, VEC>;
   constexpr int kE = V::kE;
-  __shared__ float part[4][kGradThreads / 32];
+  __shared__ float part[kGradChoices][kGradThreads / 32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   pdl_launch_dependents();
   pdl_wait();
   for (int64_t t = blockIdx.x; t < p.tokens; t += gridDim.x) {
-    for (int j0 = 0; j0 < p.top_k; j0 += 4) {
-      int64_t s[4];
-      float w[4], dot[4];
+    Choices ch;
+    for (int j0 = 0; j0 < p.top_k; j0 += kGradChoices) {
+      if (j0 % 32 == 0) ch.load(p, t, j0);
+      int32_t s[kGradChoices];
+      float w[kGradChoices], dot[kGradChoices];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        s[u] = j0 + u < p.top_k ? load_slot(p, t, j0 + u) : -1;
-        w[u] = s[u] >= 0 ? load_weight(p, t, j0 + u) : 0.0f;
+      for (int u = 0; u < kGradChoices; ++u) {
+        s[u] = ch.slot_of((j0 + u) % 32);
+        w[u] = ch.weight_of((j0 + u) % 32);
         dot[u] = 0.0f;
       }
       for (int64_t c = static_cast<int64_t>(threadIdx.x) * kE; c < p.cols; c += static_cast<int64_t>(kGradThreads) * kE) {
-        V g, y[4];
+        V g, y[kGradChoices];
         g.load(p.x, t * p.xs + c);
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
+        for (int u = 0; u < kGradChoices; ++u)
           if (s[u] >= 0) y[u].load(p.y, s[u] * p.ys + c);
         float gf[kE];
         g.get(gf);
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
+        for (int u = 0; u < kGradChoices; ++u) {
           if (s[u] < 0) continue;
           float yf[kE], o[kE];
           y[u].get(yf);
@@ -335,12 +360,12 @@ __global__ void __launch_bounds__(kGradThreads) expert_combine_grad_kernel(RowPa
         }
       }
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
+      for (int u = 0; u < kGradChoices; ++u) {
         dot[u] = warp_sum(dot[u]);
         if (lane == 0) part[u][warp] = dot[u];
       }
       __syncthreads();
-      if (threadIdx.x < 4 && j0 + static_cast<int>(threadIdx.x) < p.top_k) {
+      if (threadIdx.x < kGradChoices && j0 + static_cast<int>(threadIdx.x) < p.top_k) {
         float sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < kGradThreads / 32; ++i) sum += part[threadIdx.x][i];

@@ -74,40 +74,88 @@ __device__ __forceinline__ void unpack_e2m1x8(uint32_t q, float *v) {
   }
 }
 
+// Two 16-bit floats at once.  Magnitudes compare like unsigned numbers, so the largest one of a block is found on packed
+// bits; a bf16 times a power of two is exact, so pairs are scaled before they are widened (the power and its product
+// with anything that does not round to zero are bf16 numbers; f16's exponent range is too short for that).
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+// magnitude bits of a 16-bit float as those of the f32 of the same value (NaN and infinity stay what they are)
+template <int DT> __device__ __forceinline__ uint32_t widen_abs(uint32_t h) {
+  if constexpr (DT == BSIR_BF16) return h << 16;
+  else return __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(h))));
+}
+// eight elements as they lie in memory -> codes and the block's exponent byte, by the four lanes that hold the block
+template <int DT>
+__device__ __forceinline__ uint32_t quant8(const uint32_t *w, uint32_t *byte_out) {
+  constexpr int kPer = FloatTraits<DT>::kPerWord;
+  uint32_t m;
+  if constexpr (DT == BSIR_F32) {
+    m = w[0] & 0x7fffffffu;
+#pragma unroll
+    for (int i = 1; i < 8; ++i) m = max(m, w[i] & 0x7fffffffu);
+    m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+  } else {
+    uint32_t h = max_u16x2(max_u16x2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu), max_u16x2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
+    h = max_u16x2(h, __shfl_xor_sync(0xffffffffu, h, 1));
+    h = max_u16x2(h, __shfl_xor_sync(0xffffffffu, h, 2));
+    m = widen_abs<DT>(max(h & 0xffffu, h >> 16));
+  }
+  const uint32_t byte = scale_byte(m);
+  const float inv = inv_scale(byte);
+  float v[8];
+  if constexpr (DT == BSIR_BF16) {
+    const uint32_t inv2 = __float_as_uint(inv) | (__float_as_uint(inv) >> 16);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) FloatTraits<DT>::unpack(mul_bf16x2(w[i], inv2), v + 2 * i);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8 / kPer; ++i) FloatTraits<DT>::unpack(w[i], v + i * kPer);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __fmul_rn(v[i], inv);
+  }
+  *byte_out = byte;
+  return byte == 255u ? 0u : pack_e2m1x8(v);
+}
+
 template <int DT> __device__ __forceinline__ float load_elem(const void *x, int64_t i) {
   if constexpr (DT == BSIR_F32) return static_cast<const float *>(x)[i];
   else if constexpr (DT == BSIR_F16) return __half2float(__ushort_as_half(static_cast<const unsigned short *>(x)[i]));
   else return __uint_as_float(static_cast<uint32_t>(static_cast<const unsigned short *>(x)[i]) << 16);
 }
 
-// eight consecutive elements of a row as floats; those at or behind `cols` are zeros
+// eight consecutive elements of a row as they lie in memory; those at or behind `cols` are zeros
 template <int DT, bool VEC>
-__device__ __forceinline__ void load8(const void *x, int64_t row_at, int64_t c, int64_t cols, float *v) {
-  constexpr int kWords = 8 / FloatTraits<DT>::kPerWord;
+__device__ __forceinline__ void load8(const void *x, int64_t row_at, int64_t c, int64_t cols, uint32_t *w) {
+  constexpr int kPer = FloatTraits<DT>::kPerWord, kWords = 8 / kPer;
   if constexpr (VEC) {                 // cols % 8 == 0: a vector is all inside or all outside
     if (c < cols) {
-      const char *src = static_cast<const char *>(x) + (row_at + c) * (4 / FloatTraits<DT>::kPerWord);
+      const char *src = static_cast<const char *>(x) + (row_at + c) * (4 / kPer);
 #pragma unroll
-      for (int w = 0; w < kWords; w += 4) {
-        const Vec16 b = ld_stream(src + 4 * w);
+      for (int i = 0; i < kWords; i += 4) {
+        const Vec16 b = ld_stream(src + 4 * i);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) FloatTraits<DT>::unpack(b.w[i], v + (w + i) * FloatTraits<DT>::kPerWord);
+        for (int k = 0; k < 4; ++k) w[i + k] = b.w[k];
       }
       return;
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+    for (int i = 0; i < kWords; ++i) w[i] = 0u;
   } else {
+    float v[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = c + i < cols ? load_elem<DT>(x, row_at + c + i) : 0.0f;
-  }
-}
-
-__device__ __forceinline__ uint32_t abs_max8(const float *v) {
-  uint32_t m = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
-  return m;
+    for (int i = 0; i < kWords; ++i) w[i] = FloatTraits<DT>::pack(v + i * kPer);
+  }
 }
 
 struct QuantParams {
@@ -137,36 +185,59 @@ __device__ __forceinline__ void store_codes(uint8_t *dst, uint32_t codes, int nb
 
 // Blocks along the rows: a lane takes eight elements (16 bytes of a 16-bit type), four lanes are a block and meet in
 // two shuffles; a warp's codes leave as 128 consecutive bytes.  Four vectors a thread are loaded before the first is
-// used.
+// used.  FLAT: rows of whole blocks that follow one another without gaps in x, codes and exponents, so that a vector's
+// number is all the addressing it takes.
 constexpr int kRowVecs = 4;
-template <int DT, bool VEC>
+template <int DT, bool VEC, bool FLAT>
 __global__ void __launch_bounds__(256) mxfp4_rows_kernel(QuantParams p) {
+  constexpr int kWords = 8 / FloatTraits<DT>::kPerWord;
   pdl_launch_dependents();
   pdl_wait();
   const uint32_t v0 = blockIdx.x * (256u * kRowVecs) + threadIdx.x;
-  float v[kRowVecs][8];
-  uint32_t row[kRowVecs], col[kRowVecs];
+  uint32_t w[kRowVecs][kWords];
+  if constexpr (FLAT) {
+    const char *src = static_cast<const char *>(p.x) + static_cast<uint64_t>(v0) * (4 * kWords);
 #pragma unroll
-  for (int u = 0; u < kRowVecs; ++u) {
-    const uint32_t i = v0 + u * 256u;
-    row[u] = fast_div(p.div, i);
-    col[u] = (i - row[u] * p.div.d) * 8u;
-    load8<DT, VEC>(p.x, static_cast<int64_t>(row[u]) * p.xs, col[u], i < p.nvec ? p.cols : 0, v[u]);
-  }
+    for (int u = 0; u < kRowVecs; ++u) {
 #pragma unroll
-  for (int u = 0; u < kRowVecs; ++u) {
-    uint32_t m = abs_max8(v[u]);
-    m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-    m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-    const uint32_t byte = scale_byte(m);
-    const float inv = inv_scale(byte);
+      for (int i = 0; i < kWords; ++i) w[u][i] = 0u;
+      if (v0 + u * 256u < p.nvec) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[u][i] = __fmul_rn(v[u][i], inv);
-    const uint32_t codes = byte == 255u ? 0u : pack_e2m1x8(v[u]);
-    if (v0 + u * 256u < p.nvec && col[u] < p.cols) {
-      const int nbytes = static_cast<int>(min(static_cast<int64_t>(4), (p.cols - col[u] + 1) / 2));
-      store_codes(p.q + static_cast<int64_t>(row[u]) * p.qs + col[u] / 2, codes, nbytes, p.q_words);
-      if ((threadIdx.x & 3) == 0) p.s[static_cast<int64_t>(row[u]) * p.ss + col[u] / kBlock] = static_cast<uint8_t>(byte);
+        for (int i = 0; i < kWords; i += 4) {
+          const Vec16 b = ld_stream(src + u * 256 * 4 * kWords + 4 * i);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) w[u][i + k] = b.w[k];
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kRowVecs; ++u) {
+      uint32_t byte;
+      const uint32_t codes = quant8<DT>(w[u], &byte);
+      const uint32_t i = v0 + u * 256u;
+      if (i < p.nvec) {
+        reinterpret_cast<uint32_t *>(p.q)[i] = codes;
+        if ((threadIdx.x & 3) == 0) p.s[i >> 2] = static_cast<uint8_t>(byte);
+      }
+    }
+  } else {
+    uint32_t row[kRowVecs], col[kRowVecs];
+#pragma unroll
+    for (int u = 0; u < kRowVecs; ++u) {
+      const uint32_t i = v0 + u * 256u;
+      row[u] = fast_div(p.div, i);
+      col[u] = (i - row[u] * p.div.d) * 8u;
+      load8<DT, VEC>(p.x, static_cast<int64_t>(row[u]) * p.xs, col[u], i < p.nvec ? p.cols : 0, w[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < kRowVecs; ++u) {
+      uint32_t byte;
+      const uint32_t codes = quant8<DT>(w[u], &byte);
+      if (v0 + u * 256u < p.nvec && col[u] < p.cols) {
+        const int nbytes = static_cast<int>(min(static_cast<int64_t>(4), (p.cols - col[u] + 1) / 2));
+        store_codes(p.q + static_cast<int64_t>(row[u]) * p.qs + col[u] / 2, codes, nbytes, p.q_words);
+        if ((threadIdx.x & 3) == 0) p.s[static_cast<int64_t>(row[u]) * p.ss + col[u] / kBlock] = static_cast<uint8_t>(byte);
+      }
     }
   }
 }
@@ -177,47 +248,40 @@ __global__ void __launch_bounds__(256) mxfp4_rows_kernel(QuantParams p) {
 // time -- and its two blocks' codes (16 bytes each) go through shared memory so that a column's codes leave as kTR / 2
 // consecutive bytes.
 constexpr int kTC = 64;
-template <int DT> constexpr int kTR = DT == BSIR_F32 ? 128 : 256;
+constexpr int kTR = 128;
+constexpr int kColThreads = 128;
 template <int DT, bool VEC>
-__global__ void __launch_bounds__(256) mxfp4_cols_kernel(QuantParams p) {
-  constexpr int TR = kTR<DT>;
+__global__ void __launch_bounds__(kColThreads) mxfp4_cols_kernel(QuantParams p) {
+  constexpr int TR = kTR;
   constexpr int EB = 4 / FloatTraits<DT>::kPerWord;
+  constexpr int kWords = 8 / FloatTraits<DT>::kPerWord;
   constexpr int kCodeRow = TR / 2 + 16;                  // bytes of a column's codes, padded against bank conflicts
   extern __shared__ __align__(16) uint8_t tile[];        // [TR][kTC] elements, then [kTC][kCodeRow] codes
   uint8_t *codes_s = tile + TR * kTC * EB;
   __shared__ uint8_t scale_s[kTC][TR / kBlock];
   pdl_launch_dependents();
   pdl_wait();
-  const int64_t r0 = static_cast<int64_t>(blockIdx.x) * TR;
-  const int64_t c0 = static_cast<int64_t>(blockIdx.y) * kTC;
+  const int64_t r0 = static_cast<int64_t>(blockIdx.y) * TR;
+  const int64_t c0 = static_cast<int64_t>(blockIdx.x) * kTC;
   const int tid = threadIdx.x;
-  constexpr int kPasses = TR * (kTC / 8) / 256;
+  constexpr int kPasses = TR * (kTC / 8) / kColThreads;
 #pragma unroll
   for (int u0 = 0; u0 < kPasses; u0 += 4) {
-    float v[4][8];
+    uint32_t w[4][kWords];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      const int i = (u0 + u) * 256 + tid, r = i >> 3, c = (i & 7) * 8;
-      load8<DT, VEC>(p.x, (r0 + r) * p.xs, c0 + c, r0 + r < p.rows ? p.cols : 0, v[u]);
+      const int i = (u0 + u) * kColThreads + tid, r = i >> 3, c = (i & 7) * 8;
+      load8<DT, VEC>(p.x, (r0 + r) * p.xs, c0 + c, r0 + r < p.rows ? p.cols : 0, w[u]);
     }
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      const int i = (u0 + u) * 256 + tid, r = i >> 3, c = (i & 7) * 8;
-      uint32_t w[8 / FloatTraits<DT>::kPerWord];
+      const int i = (u0 + u) * kColThreads + tid, r = i >> 3, c = (i & 7) * 8;
 #pragma unroll
-      for (int j = 0; j < 8 / FloatTraits<DT>::kPerWord; ++j) w[j] = FloatTraits<DT>::pack(v[u] + j * FloatTraits<DT>::kPerWord);
-#pragma unroll
-      for (int j = 0; j < 8 / FloatTraits<DT>::kPerWord; j += 4)
-        *reinterpret_cast<uint4 *>(tile + (r * kTC + c) * EB + 4 * j) = make_uint4(w[j], w[j + 1], w[j + 2], w[j + 3]);
+      for (int j = 0; j < kWords; j += 4)
+        *reinterpret_cast<uint4 *>(tile + (r * kTC + c) * EB + 4 * j) = make_uint4(w[u][j], w[u][j + 1], w[u][j + 2], w[u][j + 3]);
       if (p.q) {
-        uint32_t m = abs_max8(v[u]);
-        m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-        m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-        const uint32_t byte = scale_byte(m);
-        const float inv = inv_scale(byte);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[u][j] = __fmul_rn(v[u][j], inv);
-        const uint32_t codes = byte == 255u ? 0u : pack_e2m1x8(v[u]);
+        uint32_t byte;
+        const uint32_t codes = quant8<DT>(w[u], &byte);
         const int64_t row = r0 + r, col = c0 + c;
         if (row < p.rows && col < p.cols) {
           const int nbytes = static_cast<int>(min(static_cast<int64_t>(4), (p.cols - col + 1) / 2));
@@ -229,43 +293,75 @@ __global__ void __launch_bounds__(256) mxfp4_cols_kernel(QuantParams p) {
   }
   __syncthreads();
   const int lane = tid & 31;
-  for (int b = tid >> 5; b < TR / kBlock; b += 8) {      // this warp's 32-row block; lane = a pair of columns
-    uint32_t m0 = 0, m1 = 0;
-    float a[kBlock], c[kBlock];
+  for (int b = tid >> 5; b < TR / kBlock; b += kColThreads / 32) {      // this warp's 32-row block; lane = a pair of columns
+    uint32_t byte[2];
+    uint4 *dst0 = reinterpret_cast<uint4 *>(codes_s + 2 * lane * kCodeRow + b * 16);
+    uint4 *dst1 = reinterpret_cast<uint4 *>(codes_s + (2 * lane + 1) * kCodeRow + b * 16);
+    uint32_t q0[4], q1[4];
+    const uint8_t *src = tile + (b * kBlock * kTC + 2 * lane) * EB;
+    if constexpr (DT == BSIR_F32) {
+      uint32_t m0 = 0, m1 = 0;
+      float2 x[kBlock];
 #pragma unroll
-    for (int r = 0; r < kBlock; ++r) {
-      const uint8_t *src = tile + ((b * kBlock + r) * kTC + 2 * lane) * EB;
-      if constexpr (DT == BSIR_F32) {
-        const float2 f = *reinterpret_cast<const float2 *>(src);
-        a[r] = f.x;
-        c[r] = f.y;
-      } else {
-        float f[2];
-        FloatTraits<DT>::unpack(*reinterpret_cast<const uint32_t *>(src), f);
-        a[r] = f[0];
-        c[r] = f[1];
+      for (int r = 0; r < kBlock; ++r) {
+        x[r] = *reinterpret_cast<const float2 *>(src + r * kTC * EB);
+        m0 = max(m0, __float_as_uint(x[r].x) & 0x7fffffffu);
+        m1 = max(m1, __float_as_uint(x[r].y) & 0x7fffffffu);
       }
-      m0 = max(m0, __float_as_uint(a[r]) & 0x7fffffffu);
-      m1 = max(m1, __float_as_uint(c[r]) & 0x7fffffffu);
+      byte[0] = scale_byte(m0);
+      byte[1] = scale_byte(m1);
+      const float i0 = inv_scale(byte[0]), i1 = inv_scale(byte[1]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float v[8], y[8];
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+          v[r] = __fmul_rn(x[8 * j + r].x, i0);
+          y[r] = __fmul_rn(x[8 * j + r].y, i1);
+        }
+        q0[j] = pack_e2m1x8(v);
+        q1[j] = pack_e2m1x8(y);
+      }
+    } else {
+      uint32_t x[kBlock], m = 0;
+#pragma unroll
+      for (int r = 0; r < kBlock; ++r) {
+        x[r] = *reinterpret_cast<const uint32_t *>(src + r * kTC * EB);
+        m = max_u16x2(m, x[r] & 0x7fff7fffu);
+      }
+      byte[0] = scale_byte(widen_abs<DT>(m & 0xffffu));
+      byte[1] = scale_byte(widen_abs<DT>(m >> 16));
+      const float i0 = inv_scale(byte[0]), i1 = inv_scale(byte[1]);
+      const uint32_t inv2 = (__float_as_uint(i0) >> 16) | __float_as_uint(i1);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float v[8], y[8];
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+          float f[2];
+          if constexpr (DT == BSIR_BF16) {
+            FloatTraits<DT>::unpack(mul_bf16x2(x[8 * j + r], inv2), f);
+          } else {
+            FloatTraits<DT>::unpack(x[8 * j + r], f);
+            f[0] = __fmul_rn(f[0], i0);
+            f[1] = __fmul_rn(f[1], i1);
+          }
+          v[r] = f[0];
+          y[r] = f[1];
+        }
+        q0[j] = pack_e2m1x8(v);
+        q1[j] = pack_e2m1x8(y);
+      }
     }
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      float *v = h ? c : a;
-      const uint32_t byte = scale_byte(h ? m1 : m0);
-      const float inv = inv_scale(byte);
-      uint32_t w[4];
-#pragma unroll
-      for (int r = 0; r < kBlock; ++r) v[r] = __fmul_rn(v[r], inv);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) w[j] = byte == 255u ? 0u : pack_e2m1x8(v + 8 * j);
-      *reinterpret_cast<uint4 *>(codes_s + (2 * lane + h) * kCodeRow + b * 16) = make_uint4(w[0], w[1], w[2], w[3]);
-      scale_s[2 * lane + h][b] = static_cast<uint8_t>(byte);
-    }
+    *dst0 = byte[0] == 255u ? make_uint4(0, 0, 0, 0) : make_uint4(q0[0], q0[1], q0[2], q0[3]);
+    *dst1 = byte[1] == 255u ? make_uint4(0, 0, 0, 0) : make_uint4(q1[0], q1[1], q1[2], q1[3]);
+    scale_s[2 * lane][b] = static_cast<uint8_t>(byte[0]);
+    scale_s[2 * lane + 1][b] = static_cast<uint8_t>(byte[1]);
   }
   __syncthreads();
   constexpr int kPieces = TR / kBlock;                   // 16-byte pieces of a column's codes
   const int64_t code_bytes = (p.rows + 1) / 2, blocks = (p.rows + kBlock - 1) / kBlock;
-  for (int i = tid; i < kTC * kPieces; i += 256) {
+  for (int i = tid; i < kTC * kPieces; i += kColThreads) {
     const int c = i / kPieces, b = i % kPieces;
     const int64_t col = c0 + c, at = r0 / 2 + b * 16;
     if (col >= p.cols || at >= code_bytes) continue;
@@ -293,53 +389,94 @@ struct DequantParams {
   uint32_t nvec;
   int q_words;
 };
-template <int DT, bool VEC>
-__global__ void __launch_bounds__(256) mxfp4_dequant_kernel(DequantParams p) {
+// eight codes and their exponent byte -> eight elements as they lie in memory.  A code's magnitude bits, put at the
+// bottom of bf16's exponent and top of its mantissa, are the value times 2^-126; two multiplications by powers of two
+// (one would need 2^253) give the scaled value on pairs, exact down to bf16's subnormals.
+template <int DT>
+__device__ __forceinline__ void dequant8(uint32_t codes, uint32_t byte, uint32_t *w) {
   constexpr int kPer = FloatTraits<DT>::kPerWord;
+  // 2^(byte - 127): byte 0 is 2^-127, under f32's normals (bits 0x00400000); 255 is NaN
+  const uint32_t sc = byte == 255u ? 0x7fc00000u : byte == 0u ? 0x00400000u : byte << 23;
+  if constexpr (DT == BSIR_BF16) {
+    const uint32_t sc2 = sc | (sc >> 16);
+    uint32_t t[4];                                  // elements i and i + 4
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t c = codes >> (4 * i);
+      t[i] = mul_bf16x2(mul_bf16x2(((c << 6) & 0x01c001c0u) | ((c << 12) & 0x80008000u), 0x7e807e80u), sc2);
+    }
+    w[0] = __byte_perm(t[0], t[1], 0x5410);
+    w[1] = __byte_perm(t[2], t[3], 0x5410);
+    w[2] = __byte_perm(t[0], t[1], 0x7632);
+    w[3] = __byte_perm(t[2], t[3], 0x7632);
+  } else {
+    float v[8];
+    unpack_e2m1x8(codes, v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = __fmul_rn(v[j], __uint_as_float(sc));
+#pragma unroll
+    for (int j = 0; j < 8 / kPer; ++j) w[j] = FloatTraits<DT>::pack(v + j * kPer);
+  }
+}
+template <int DT, bool VEC, bool FLAT>
+__global__ void __launch_bounds__(256) mxfp4_dequant_kernel(DequantParams p) {
+  constexpr int kPer = FloatTraits<DT>::kPerWord, kWords = 8 / kPer;
   pdl_launch_dependents();
   pdl_wait();
   const uint32_t v0 = blockIdx.x * (256u * kRowVecs) + threadIdx.x;
-  uint32_t codes[kRowVecs], byte[kRowVecs];
+  uint32_t codes[kRowVecs], byte[kRowVecs], row[kRowVecs], col[kRowVecs];
 #pragma unroll
   for (int u = 0; u < kRowVecs; ++u) {
     const uint32_t i = v0 + u * 256u;
-    codes[u] = byte[u] = 0;
-    if (i >= p.nvec) continue;
-    const uint32_t row = fast_div(p.div, i);
-    const int64_t col = static_cast<int64_t>(i - row * p.div.d) * 8;
-    if (col >= p.cols) continue;
-    const uint8_t *src = p.q + static_cast<int64_t>(row) * p.qs + col / 2;
-    const int nbytes = static_cast<int>(min(static_cast<int64_t>(4), (p.cols - col + 1) / 2));
-    if (p.q_words && nbytes == 4) {
-      codes[u] = *reinterpret_cast<const uint32_t *>(src);
+    codes[u] = byte[u] = row[u] = col[u] = 0;
+    if constexpr (FLAT) {
+      if (i < p.nvec) {
+        codes[u] = reinterpret_cast<const uint32_t *>(p.q)[i];
+        byte[u] = p.s[i >> 2];
+      }
     } else {
-      for (int j = 0; j < 4 && j < nbytes; ++j) codes[u] |= static_cast<uint32_t>(src[j]) << (8 * j);
+      if (i >= p.nvec) continue;
+      row[u] = fast_div(p.div, i);
+      col[u] = (i - row[u] * p.div.d) * 8u;
+      if (col[u] >= p.cols) continue;
+      const uint8_t *src = p.q + static_cast<int64_t>(row[u]) * p.qs + col[u] / 2;
+      const int nbytes = static_cast<int>(min(static_cast<int64_t>(4), (p.cols - col[u] + 1) / 2));
+      if (p.q_words && nbytes == 4) {
+        codes[u] = *reinterpret_cast<const uint32_t *>(src);
+      } else {
+        for (int j = 0; j < 4 && j < nbytes; ++j) codes[u] |= static_cast<uint32_t>(src[j]) << (8 * j);
+      }
+      byte[u] = p.s[static_cast<int64_t>(row[u]) * p.ss + col[u] / kBlock];
     }
-    byte[u] = p.s[static_cast<int64_t>(row) * p.ss + col / kBlock];
   }
 #pragma unroll
   for (int u = 0; u < kRowVecs; ++u) {
     const uint32_t i = v0 + u * 256u;
-    if (i >= p.nvec) continue;
-    const uint32_t row = fast_div(p.div, i);
-    const int64_t col = static_cast<int64_t>(i - row * p.div.d) * 8;
-    if (col >= p.cols) continue;
-    float v[8];
-    unpack_e2m1x8(codes[u], v);
-    // 2^(byte - 127): byte 0 is 2^-127, under f32's normals (bits 0x00400000); 255 is NaN
-    const float sc = byte[u] == 255u ? __uint_as_float(0x7fc00000u) : byte[u] == 0u ? __uint_as_float(0x00400000u) : __uint_as_float(byte[u] << 23);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = __fmul_rn(v[j], sc);
-    const int64_t at = static_cast<int64_t>(row) * p.ys + col;
-    uint32_t w[8 / kPer];
-#pragma unroll
-    for (int j = 0; j < 8 / kPer; ++j) w[j] = FloatTraits<DT>::pack(v + j * kPer);
-    if (VEC) {
+    if (i >= p.nvec || (!FLAT && col[u] >= p.cols)) continue;
+    uint32_t w[kWords];
+    dequant8<DT>(codes[u], byte[u], w);
+    const int64_t at = FLAT ? static_cast<int64_t>(i) * 8 : static_cast<int64_t>(row[u]) * p.ys + col[u];
+    if constexpr (VEC) {
       char *dst = static_cast<char *>(p.y) + at * (4 / kPer);
+      if constexpr (FLAT && kWords == 8) {
+        // 32 bytes a lane: neighbours swap halves, so that a store covers whole sectors (nvec is a multiple of 4: both
+        // of a pair are here)
+        const bool odd = threadIdx.x & 1;
+        uint32_t a[4];
 #pragma unroll
-      for (int j = 0; j < 8 / kPer; j += 4) st_stream(dst + 4 * j, Vec16{{w[j], w[j + 1], w[j + 2], w[j + 3]}});
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t got = __shfl_xor_sync(__activemask(), odd ? w[j] : w[4 + j], 1);
+          a[j] = got;
+        }
+        const Vec16 mine{{odd ? w[4] : w[0], odd ? w[5] : w[1], odd ? w[6] : w[2], odd ? w[7] : w[3]}}, other{{a[0], a[1], a[2], a[3]}};
+        st_stream(odd ? dst - 16 : dst, odd ? other : mine);
+        st_stream(odd ? dst + 16 : dst + 32, odd ? mine : other);
+      } else {
+#pragma unroll
+        for (int j = 0; j < kWords; j += 4) st_stream(dst + 4 * j, Vec16{{w[j], w[j + 1], w[j + 2], w[j + 3]}});
+      }
     } else {
-      for (int j = 0; j < 8 && col + j < p.cols; ++j) {
+      for (int j = 0; j < 8 && col[u] + j < p.cols; ++j) {
         if constexpr (DT == BSIR_F32) static_cast<uint32_t *>(p.y)[at + j] = w[j];
         else static_cast<uint16_t *>(p.y)[at + j] = static_cast<uint16_t>(w[j >> 1] >> (16 * (j & 1)));
       }
@@ -350,20 +487,21 @@ __global__ void __launch_bounds__(256) mxfp4_dequant_kernel(DequantParams p) {
 template <int DT, bool VEC>
 int32_t launch_quant(QuantParams p, cudaStream_t st) {
   if (p.qt) {
-    constexpr int TR = kTR<DT>;
+    constexpr int TR = kTR;
     constexpr size_t smem = TR * kTC * (DT == BSIR_F32 ? 4 : 2) + kTC * (TR / 2 + 16);
     cudaFuncSetAttribute(mxfp4_cols_kernel<DT, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-    const int64_t gx = ceil_div(p.rows, TR), gy = ceil_div(p.cols, kTC);
-    // the grid's y axis ends at 65535: wider matrices go in column strips (a strip starts at a whole block)
+    // column tiles run fastest: the CTAs at work together read whole rows.  The grid's y axis ends at 65535: longer
+    // matrices go in strips of rows (a strip starts at a whole block).
+    const int64_t gx = ceil_div(p.cols, kTC), gy = ceil_div(p.rows, TR);
     for (int64_t y0 = 0; y0 < gy; y0 += 65535) {
       QuantParams s = p;
-      const int64_t c0 = y0 * kTC, ny = gy - y0 < 65535 ? gy - y0 : 65535;
-      s.x = static_cast<const char *>(p.x) + c0 * dtype_bytes(DT);
-      s.cols = p.cols - c0 < ny * kTC ? p.cols - c0 : ny * kTC;
-      if (p.q) { s.q = p.q + c0 / 2; s.s = p.s + c0 / kBlock; }
-      s.qt = p.qt + c0 * p.qts;
-      s.st = p.st + c0 * p.sts;
-      launch_pdl(mxfp4_cols_kernel<DT, VEC>, dim3(static_cast<unsigned>(gx), static_cast<unsigned>(ny)), dim3(256), smem, st, s);
+      const int64_t r0 = y0 * TR, ny = gy - y0 < 65535 ? gy - y0 : 65535;
+      s.x = static_cast<const char *>(p.x) + r0 * p.xs * dtype_bytes(DT);
+      s.rows = p.rows - r0 < ny * TR ? p.rows - r0 : ny * TR;
+      if (p.q) { s.q = p.q + r0 * p.qs; s.s = p.s + r0 * p.ss; }
+      s.qt = p.qt + r0 / 2;
+      s.st = p.st + r0 / kBlock;
+      launch_pdl(mxfp4_cols_kernel<DT, VEC>, dim3(static_cast<unsigned>(gx), static_cast<unsigned>(ny)), dim3(kColThreads), smem, st, s);
       count_launch();
     }
     return check_launch("quant_mxfp4");
@@ -378,7 +516,14 @@ int32_t launch_quant(QuantParams p, cudaStream_t st) {
     s.s = p.s + r * p.ss;
     s.div = make_fastdiv(static_cast<uint32_t>(vpr));
     s.nvec = static_cast<uint32_t>(s.rows * vpr);
-    launch_pdl(mxfp4_rows_kernel<DT, VEC>, dim3(static_cast<unsigned>(ceil_div(s.nvec, 256 * kRowVecs))), dim3(256), 0, st, s);
+    const dim3 grid(static_cast<unsigned>(ceil_div(s.nvec, 256 * kRowVecs)));
+    if constexpr (VEC) {
+      const bool flat = p.cols % kBlock == 0 && p.q_words && (p.rows == 1 || (p.xs == p.cols && p.qs == p.cols / 2 && p.ss == p.cols / kBlock));
+      if (flat) launch_pdl(mxfp4_rows_kernel<DT, true, true>, grid, dim3(256), 0, st, s);
+      else launch_pdl(mxfp4_rows_kernel<DT, true, false>, grid, dim3(256), 0, st, s);
+    } else {
+      launch_pdl(mxfp4_rows_kernel<DT, false, false>, grid, dim3(256), 0, st, s);
+    }
     count_launch();
   }
   return check_launch("quant_mxfp4");
@@ -394,7 +539,14 @@ int32_t launch_dequant(DequantParams p, int64_t rows, cudaStream_t st) {
     s.y = static_cast<char *>(p.y) + r * p.ys * dtype_bytes(DT);
     s.div = make_fastdiv(static_cast<uint32_t>(vpr));
     s.nvec = static_cast<uint32_t>((rows - r < step ? rows - r : step) * vpr);
-    launch_pdl(mxfp4_dequant_kernel<DT, VEC>, dim3(static_cast<unsigned>(ceil_div(s.nvec, 256 * kRowVecs))), dim3(256), 0, st, s);
+    const dim3 grid(static_cast<unsigned>(ceil_div(s.nvec, 256 * kRowVecs)));
+    if constexpr (VEC) {
+      const bool flat = p.cols % kBlock == 0 && p.q_words && (rows == 1 || (p.ys == p.cols && p.qs == p.cols / 2 && p.ss == p.cols / kBlock));
+      if (flat) launch_pdl(mxfp4_dequant_kernel<DT, true, true>, grid, dim3(256), 0, st, s);
+      else launch_pdl(mxfp4_dequant_kernel<DT, true, false>, grid, dim3(256), 0, st, s);
+    } else {
+      launch_pdl(mxfp4_dequant_kernel<DT, false, false>, grid, dim3(256), 0, st, s);
+    }
     count_launch();
   }
   return check_launch("dequant_mxfp4");
