@@ -283,12 +283,25 @@ struct RowWriter {
         }
       }
     } else {
-      for (int r = 0; r < rows; ++r) {
-        char *dst = static_cast<char *>(p.out) + ((row0 + r) * p.ldo + col0) * eb;
-        for (int i = lane * eb; i < have; i += 32 * eb) {
-          const uint8_t *src = buf + r * 128 + (((i >> 4) ^ (r & 7)) * 16) + (i & 15);
-          if (eb == 4) *reinterpret_cast<uint32_t *>(dst + i) = *reinterpret_cast<const uint32_t *>(src);
-          else *reinterpret_cast<uint16_t *>(dst + i) = *reinterpret_cast<const uint16_t *>(src);
+      // four bytes a lane, eight rows in flight
+      const int at = lane * 4;
+      const bool low = at < have, high = at + 2 < have;
+      char *dst = static_cast<char *>(p.out) + (static_cast<int64_t>(row0) * p.ldo + col0) * eb + at;
+      const int64_t pitch = p.ldo * eb;
+      for (int r0 = 0; r0 < rows; r0 += 8) {
+        uint32_t v[8];
+#pragma unroll
+        for (int r = 0; r < 8; ++r) v[r] = *reinterpret_cast<const uint32_t *>(buf + (r0 + r) * 128 + (((at >> 4) ^ r) * 16) + (at & 15));
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+          if (r0 + r >= rows || !low) continue;
+          char *d = dst + (r0 + r) * pitch;
+          if (eb == 4) {
+            *reinterpret_cast<uint32_t *>(d) = v[r];
+          } else {
+            *reinterpret_cast<uint16_t *>(d) = static_cast<uint16_t>(v[r]);
+            if (high) *reinterpret_cast<uint16_t *>(d + 2) = static_cast<uint16_t>(v[r] >> 16);
+          }
         }
       }
     }
@@ -313,11 +326,25 @@ __device__ __forceinline__ void store_rows(const MxParams &p, RowWriter &out, ui
     release();
   } else if constexpr (kDrain) {
     uint32_t w[BN / 2];
+    const float4 *bias = reinterpret_cast<const float4 *>(out.stage);     // put there before the accumulator was waited for
 #pragma unroll
-    for (int c = 0; c < BN / 32; ++c) {
-      uint32_t r[32];
-      load_columns(p, acc + static_cast<uint32_t>(32 * c), t.group, t.n0 + 32 * c, lane, r);
-      round_columns(p, r, w + 16 * c);
+    for (int c = 0; c < BN / 64; ++c) {
+      uint32_t r[64];
+      tmem_ld32(acc + static_cast<uint32_t>(64 * c), r);
+      tmem_ld32(acc + static_cast<uint32_t>(64 * c + 32), r + 32);
+      tmem_ld_wait();
+      if (p.bias) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const float4 b = bias[16 * c + j];
+          r[4 * j] = __float_as_uint(__fadd_rn(__uint_as_float(r[4 * j]), b.x));
+          r[4 * j + 1] = __float_as_uint(__fadd_rn(__uint_as_float(r[4 * j + 1]), b.y));
+          r[4 * j + 2] = __float_as_uint(__fadd_rn(__uint_as_float(r[4 * j + 2]), b.z));
+          r[4 * j + 3] = __float_as_uint(__fadd_rn(__uint_as_float(r[4 * j + 3]), b.w));
+        }
+      }
+      round_columns(p, r, w + 32 * c);
+      round_columns(p, r + 32, w + 32 * c + 16);
     }
     release();
 #pragma unroll
@@ -590,6 +617,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool ok = true;
     for (int tile = first_tile; tile < total_tiles && ok; tile += tile_step) {
       find_tile<kRows, kColsC>(tile, tile_start, row_start, group, t);
+      if constexpr (!SWAP && Cfg::kAccs == 1) {       // the tile's bias into the staging buffer, which is idle until then
+        if (p.bias && p.out_dtype != BSIR_F32) {
+          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+          __syncwarp();
+          for (int c = lane; c < BN; c += 32)
+            reinterpret_cast<float *>(stage)[c] = t.n0 + c < p.n ? load_float(p.bias, p.bias_dtype, t.group * p.bias_stride + t.n0 + c) : 0.0f;
+          __syncwarp();
+        }
+      }
       if (!mbar_wait(acc_full_bar(acc), acc_phase, abort_flag, p.err)) break;
       tc_fence_after();
       const uint32_t src = tmem + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>(acc * BN);
