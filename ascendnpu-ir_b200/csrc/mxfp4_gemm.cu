@@ -13,11 +13,11 @@
 // them to tensor memory themselves were the first form: next to cta_group::2 instructions such a store took 1400
 // cycles, and a chunk of 512 elements of K is 1024 of multiplication.)
 //
-// A persistent kernel, one CTA per SM, 288 threads:
+// A persistent kernel, one CTA per SM, 256 threads:
 //   warp 0      TMA producer of codes (a ring of stages of 256 elements of K) and exponents (a ring of 1024)
 //   warp 1      issuer of tcgen05.cp and tcgen05.mma
 //   warps 2-5   epilogue: accumulator -> bias -> rounding -> C
-//   warps 6-8   exponents: rows of eight words -> lanes of four rows, 128 rows a warp
+//   warps 6-7   exponents: rows of eight words -> lanes of four rows, 128 rows at a time
 // in three forms:
 //   kPair    256 rows of A x BN columns of C on two CTAs (cta_group::2): each holds its 128 rows of A and half of the
 //            tile's rows of B, so that an SM's shared memory is read and filled for B half as often;
@@ -34,7 +34,7 @@ namespace {
 constexpr int kTileM = 128;
 constexpr int kStageK = 256;       // elements of K a stage: one 128-byte swizzle row of codes
 constexpr int kChunk = 4;           // stages that a piece of exponents lasts: 32 bytes (a sector) of each row
-constexpr int kThreads = 288;
+constexpr int kThreads = 256;      // registers are handed out for multiples of 128 threads: 288 would leave 168 each
 constexpr int kMaxGroups = 1024;
 enum MxMode { kSingle, kPair, kFew };
 
@@ -573,14 +573,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp >= 6) {
     // ---------------- exponents: this warp's block of 128 rows, turned in place: row r's words w -> lane r % 32 of word w
-    const int block = warp - 6;
-    if (block < Cfg::kSfBlocks) {
-      int sf = 0;
-      uint32_t sf_phase = 0;
-      bool ok = true;
-      for (int tile = first_tile; tile < total_tiles && ok; tile += tile_step) {
-        for (int c = chunk0; c < chunk1; ++c) {
-          if (!mbar_wait(sf_full_bar(sf), sf_phase, abort_flag, p.err)) { ok = false; break; }
+    int sf = 0;
+    uint32_t sf_phase = 0;
+    bool ok = true;
+    for (int tile = first_tile; tile < total_tiles && ok; tile += tile_step) {
+      for (int c = chunk0; c < chunk1; ++c) {
+        if (!mbar_wait(sf_full_bar(sf), sf_phase, abort_flag, p.err)) { ok = false; break; }
+        for (int block = warp - 6; block < Cfg::kSfBlocks; block += 2) {
           uint4 *rows = reinterpret_cast<uint4 *>(gen + Cfg::kSfOff + sf * Cfg::kSfStage + block * 4096);
           uint4 lo[4], hi[4];                          // rows lane, 32 + lane, ..: words 0-3 and 4-7
 #pragma unroll
@@ -603,8 +602,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             if constexpr (PAIR) mbar_arrive_leader(map_to_cta(sf_ready_bar(sf), 0));
             else mbar_arrive(sf_ready_bar(sf));
           }
-          if (++sf == Cfg::kSfStages) { sf = 0; sf_phase ^= 1u; }
         }
+        if (++sf == Cfg::kSfStages) { sf = 0; sf_phase ^= 1u; }
       }
     }
   } else {
