@@ -24,8 +24,9 @@
 //   kSingle  128 rows x BN columns on one CTA, for groups that would leave much of a 256-row tile empty;
 //   kFew     operands swapped: 128 rows of B are the instruction's M side and BN rows of A its N side, so that weights
 //            are streamed for as few as 16 rows of A.  With few tiles a cluster of up to eight CTAs shares a tile's K:
-//            every CTA hands each other one that CTA's part of its partial tile through distributed shared memory,
-//            and the parts are added in the order of the CTAs (the same bits on every run).
+//            every CTA hands each other one that CTA's rows of its partial tile (asynchronous stores into distributed
+//            shared memory), and the parts are added in the order of the CTAs (the same bits on every run).  A cluster
+//            then has one tile only.
 #include "tc_ptx.cuh"
 
 namespace bsir {
@@ -167,10 +168,12 @@ __device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap
 __device__ __forceinline__ void mbar_arrive_leader(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
-__device__ __forceinline__ void st_cluster_f32(uint32_t cluster_addr, uint32_t bits) {
-  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr), "r"(bits) : "memory");
+// eight bytes into a CTA of the cluster, counted on a barrier there: the receiver needs no other synchronisation
+__device__ __forceinline__ void st_async(uint32_t cluster_addr, uint32_t a, uint32_t b, uint32_t cluster_bar) {
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.b32 [%0], {%1, %2}, [%3];" ::"r"(cluster_addr), "r"(a), "r"(b),
+               "r"(cluster_bar)
+               : "memory");
 }
-__device__ __forceinline__ void fence_cluster() { asm volatile("fence.acq_rel.cluster;" ::: "memory"); }
 
 __device__ __forceinline__ uint32_t elect_one() {       // 1 in one lane of the (whole) warp
   uint32_t one;
@@ -394,9 +397,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   constexpr int kB3 = kB2 + Cfg::kSfStages;
   auto acc_full_bar = [&](int b) { return bars + 8u * (kB3 + b); };
   auto acc_empty_bar = [&](int b) { return bars + 8u * (kB3 + 2 + b); };
-  const uint32_t red_full = bars + 8u * (kB3 + 4), red_empty = bars + 8u * (kB3 + 5);   // partial tiles of the cluster
-  static_assert(8 * (kB3 + 6) + 16 <= 512, "barriers");
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(gen + Cfg::kBarOff + 8 * (kB3 + 6));
+  const uint32_t red_full = bars + 8u * (kB3 + 4);                          // the cluster's partial tiles
+  static_assert(8 * (kB3 + 5) + 16 <= 512, "barriers");
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(gen + Cfg::kBarOff + 8 * (kB3 + 5));
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
   int *tile_start = reinterpret_cast<int *>(gen + Cfg::kTableOff);         // [groups + 1]
   int *row_start = tile_start + kMaxGroups + 1;                            // [groups + 1]
@@ -415,8 +418,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int b = 0; b < 2; ++b) {
       mbar_init(acc_full_bar(b), 1); mbar_init(acc_empty_bar(b), PAIR ? 8 : 4);
     }
-    mbar_init(red_full, 4 * team);
-    mbar_init(red_empty, 4 * team);
+    mbar_init(red_full, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     prefetch_tmap(&tmap_m); prefetch_tmap(&tmap_n); prefetch_tmap(&tmap_sm); prefetch_tmap(&tmap_sn);
@@ -612,7 +614,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint8_t *stage = gen + Cfg::kEpiOff + (warp - 2) * 8192;
     const uint32_t stage_addr = base + Cfg::kEpiOff + (warp - 2) * 8192;
     int acc = 0;
-    uint32_t acc_phase = 0, red_phase = 0, nstores = 0;
+    uint32_t acc_phase = 0, nstores = 0;
     bool ok = true;
     for (int tile = first_tile; tile < total_tiles && ok; tile += tile_step) {
       find_tile<kRows, kColsC>(tile, tile_start, row_start, group, t);
@@ -654,36 +656,36 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         } else {
-          // this CTA's partial tile: row j goes to CTA j / own of the cluster, slot [rank][j % own][128]
+          // this CTA's partial tile: row j goes to CTA j / own of the cluster, pairs of rows side by side:
+          // [from][j % own / 2][128 columns][2].  The team has this one tile (see the launch).
           const int own = BN / team;
           const uint32_t red = base + Cfg::kEpiOff;
-          if (!mbar_wait(red_empty, red_phase ^ 1u, abort_flag, p.err)) break;
+          if (threadIdx.x == 64) mbar_expect_tx(red_full, BN * kTileM * 4);
 #pragma unroll 1
           for (int c0 = 0; c0 < BN; c0 += 16) {
             uint32_t r[16];
             tmem_ld16(src + static_cast<uint32_t>(c0), r);
             tmem_ld_wait();
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
+            for (int j = 0; j < 16; j += 2) {
               const int to = (c0 + j) / own, slot = (c0 + j) - to * own;
-              st_cluster_f32(map_to_cta(red + static_cast<uint32_t>(((rank * own + slot) * kTileM + quad * 32 + lane) * 4), to), r[j]);
+              st_async(map_to_cta(red + static_cast<uint32_t>(((rank * own + slot) * kTileM + 2 * (quad * 32 + lane)) * 4), to), r[j], r[j + 1],
+                       map_to_cta(red_full, to));
             }
           }
-          fence_cluster();
-          __syncwarp();
-          if (lane < team) mbar_arrive_cluster(map_to_cta(red_full, lane));
-          if (!mbar_wait(red_full, red_phase, abort_flag, p.err)) break;
-          fence_cluster();
-          const float *part = reinterpret_cast<const float *>(gen + Cfg::kEpiOff) + quad * 32 + lane;
-          for (int j = 0; j < own; ++j) {
-            float sum = part[j * kTileM];
-            for (int s = 1; s < team; ++s) sum += part[(s * own + j) * kTileM];
+          if (!mbar_wait(red_full, 0u, abort_flag, p.err)) break;
+          const float2 *part = reinterpret_cast<const float2 *>(gen + Cfg::kEpiOff) + quad * 32 + lane;
+          for (int j = 0; j < own; j += 2) {
+            float2 sum = part[j / 2 * kTileM];
+            for (int f = 1; f < team; ++f) {
+              const float2 v = part[(f * own + j) / 2 * kTileM];
+              sum.x += v.x;
+              sum.y += v.y;
+            }
             const int64_t row = t.row0 + rank * own + j;
-            if (col_ok && row < t.row_end) store_out(p, row * p.ldo + col, __fadd_rn(sum, bias));
+            if (col_ok && row < t.row_end) store_out(p, row * p.ldo + col, __fadd_rn(sum.x, bias));
+            if (col_ok && row + 1 < t.row_end) store_out(p, (row + 1) * p.ldo + col, __fadd_rn(sum.y, bias));
           }
-          __syncwarp();
-          if (lane < team) mbar_arrive_cluster(map_to_cta(red_empty, lane));
-          red_phase ^= 1u;
         }
         release();
       } else {
@@ -732,7 +734,7 @@ int32_t launch_mx(const MxOperand &a, const MxOperand &b, int64_t k, MxParams p,
   const int team = MODE == kPair ? 2 : MODE == kFew ? split : 1;
   p.split = team;
   int64_t teams = (device_info().sm_count > 0 ? device_info().sm_count : 148) / team;
-  if (teams > max_tiles) teams = max_tiles;
+  if (teams > max_tiles || (MODE == kFew && split > 1)) teams = max_tiles;     // a cluster that shares K has one tile
   const dim3 grid(static_cast<unsigned>(teams * team));
   if (team > 1) launch_pdl_cluster(mxfp4_gemm_kernel<BN, MODE>, grid, dim3(kThreads), Cfg::kSmem, st, team, tm, tn, tsm, tsn, tout, p);
   else launch_pdl(mxfp4_gemm_kernel<BN, MODE>, grid, dim3(kThreads), Cfg::kSmem, st, tm, tn, tsm, tsn, tout, p);
@@ -798,27 +800,33 @@ extern "C" int32_t bsir_matmul_mxfp4(const bsir_matmul_mxfp4_desc *d, void *stre
   p.err = device_error_word();
   if (!p.err) return fail(BSIR_ERR_WORKSPACE, "matmul_mxfp4: no device error word");
   cudaStream_t st = resolve_stream(stream);
-  // rows of a group that a tile should hold: all rows, or the groups' mean (their sizes are on the device)
-  const int64_t rows = ceil_div(d->m, groups);
-  auto tiles = [&](int64_t r, int64_t c) { return (d->m / r + groups) * ceil_div(d->n, c); };   // at most
   p.tma_out = aligned_to(d->out, 16) && (ldo * eb) % 16 == 0;
-  const int mode = std::getenv("MX_MODE") ? atoi(std::getenv("MX_MODE")) : -1;
-  const int sms = device_info().sm_count > 0 ? device_info().sm_count : 148;
-  auto split_of = [&](int64_t nt) {
-    if (std::getenv("MX_SPLIT")) return atoi(std::getenv("MX_SPLIT"));
-    const int chunks = static_cast<int>(ceil_div(p.k_blocks, kChunk));
-    int s = 1;
-    while (s < 8 && nt * s * 2 <= sms && ceil_div(chunks, 2 * s) * (2 * s - 1) < chunks) s *= 2;
-    return s;
+  // Which form: from the rows of a group, all of them or the groups' mean (their sizes are on the device).  Measured
+  // (N x K = 4096 x 4096 | 14336 x 4096, bf16 out): up to 16 rows kFew<16> 7.0-7.6 | 9.1-9.6 us, kSingle 7.8 | 12-14;
+  // 32 rows kFew<32> 8.6 | 10.4, kSingle 8.0 | 12.2; 48 rows kFew<32> 8.7 | 13.8, kSingle 7.8 | 12.3.
+  const int64_t rows = ceil_div(d->m, groups);
+  const int64_t sms = device_info().sm_count > 0 ? device_info().sm_count : 148;
+  auto tiles = [&](int64_t r, int64_t c) { return (groups > 1 ? d->m / r + groups : ceil_div(d->m, r)) * ceil_div(d->n, c); };   // at most
+  if (rows <= 32) {
+    const int64_t nt = rows <= 16 ? tiles(16, kTileM) : tiles(32, kTileM);
+    // K shared out over a cluster while that does not make more CTAs than SMs and every CTA gets a part
+    // (1 row, 4096 x 4096: 7.6 us whole, 7.0 by four; 4096 x 14336: 17.6 and 11.1)
+    const int64_t chunks = ceil_div(p.k_blocks, kChunk);
+    int split = 1;
+    while (split < 8 && nt * split * 2 <= sms && ceil_div(chunks, 2 * split) * (2 * split - 1) < chunks) split *= 2;
+    return rows <= 16 ? launch_mx<16, kFew>(a, b, d->k, p, split, nt, st) : launch_mx<32, kFew>(a, b, d->k, p, split, nt, st);
+  }
+  // Rounds of tiles over the SMs x time of a tile, in units of 5 ns: a stage takes 305 ns on one CTA with 128 x 128
+  // and 345 on a pair, with 256 x 256 (plus 1.4 us to drain the one accumulator) or 256 x 192 (two accumulators; f32
+  // results, which a drain could not hold, take this one).  Groups leave half of a last tile empty on average.
+  auto rounds = [&](int64_t r, int64_t c, int64_t at_once) {
+    const int64_t nt = groups > 1 ? (d->m / r + groups / 2 + 1) * ceil_div(d->n, c) : tiles(r, c);
+    return ceil_div(nt, at_once);
   };
-  if (mode == 0) return launch_mx<128, kSingle>(a, b, d->k, p, 1, tiles(kTileM, 128), st);
-  if (mode == 1) return launch_mx<192, kPair>(a, b, d->k, p, 1, tiles(256, 192), st);
-  if (mode == 2) return launch_mx<256, kPair>(a, b, d->k, p, 1, tiles(256, 256), st);
-  if (mode == 3) return launch_mx<192, kSingle>(a, b, d->k, p, 1, tiles(128, 192), st);
-  if (mode == 4) return launch_mx<32, kFew>(a, b, d->k, p, split_of(tiles(32, kTileM)), tiles(32, kTileM), st);
-  if (mode == 5) return launch_mx<128, kPair>(a, b, d->k, p, 1, tiles(256, 128), st);
-  if (rows <= 16) return launch_mx<16, kFew>(a, b, d->k, p, split_of(tiles(16, kTileM)), tiles(16, kTileM), st);
-  if (rows <= 64) return launch_mx<64, kFew>(a, b, d->k, p, split_of(tiles(64, kTileM)), tiles(64, kTileM), st);
-  if (rows >= 512) return launch_mx<192, kPair>(a, b, d->k, p, 1, tiles(256, 192), st);
-  return launch_mx<128, kSingle>(a, b, d->k, p, 1, tiles(kTileM, 128), st);
+  const bool wide = d->out_dtype == BSIR_F32;
+  const int64_t single = rounds(128, 128, sms) * 61 * p.k_blocks;
+  const int64_t pair = wide ? rounds(256, 192, sms / 2) * 69 * p.k_blocks : rounds(256, 256, sms / 2) * (69 * p.k_blocks + 280);
+  if (single <= pair) return launch_mx<128, kSingle>(a, b, d->k, p, 1, tiles(128, 128), st);
+  if (wide) return launch_mx<192, kPair>(a, b, d->k, p, 1, tiles(256, 192), st);
+  return launch_mx<256, kPair>(a, b, d->k, p, 1, tiles(256, 256), st);
 }

@@ -264,17 +264,17 @@ __global__ void __launch_bounds__(kColThreads) mxfp4_cols_kernel(QuantParams p) 
   const int64_t r0 = static_cast<int64_t>(blockIdx.y) * TR;
   const int64_t c0 = static_cast<int64_t>(blockIdx.x) * kTC;
   const int tid = threadIdx.x;
-  constexpr int kPasses = TR * (kTC / 8) / kColThreads;
+  constexpr int kPasses = TR * (kTC / 8) / kColThreads, kAhead = DT == BSIR_F32 ? 4 : kPasses;     // 16-bit: all of a thread's loads ahead of the first use
 #pragma unroll
-  for (int u0 = 0; u0 < kPasses; u0 += 4) {
-    uint32_t w[4][kWords];
+  for (int u0 = 0; u0 < kPasses; u0 += kAhead) {
+    uint32_t w[kAhead][kWords];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < kAhead; ++u) {
       const int i = (u0 + u) * kColThreads + tid, r = i >> 3, c = (i & 7) * 8;
       load8<DT, VEC>(p.x, (r0 + r) * p.xs, c0 + c, r0 + r < p.rows ? p.cols : 0, w[u]);
     }
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < kAhead; ++u) {
       const int i = (u0 + u) * kColThreads + tid, r = i >> 3, c = (i & 7) * 8;
 #pragma unroll
       for (int j = 0; j < kWords; j += 4)
