@@ -13,11 +13,11 @@
 // them to tensor memory themselves were the first form: next to cta_group::2 instructions such a store took 1400
 // cycles, and a chunk of 512 elements of K is 1024 of multiplication.)
 //
-// A persistent kernel, one CTA per SM, 256 threads:
-//   warp 0      TMA producer of codes (a ring of stages of 256 elements of K) and exponents (a ring of 1024)
-//   warp 1      issuer of tcgen05.cp and tcgen05.mma
-//   warps 2-5   epilogue: accumulator -> bias -> rounding -> C
-//   warps 6-7   exponents: rows of eight words -> lanes of four rows, 128 rows at a time
+// A persistent kernel, one CTA per SM, 256 threads (384 with one accumulator):
+//   warp 0            TMA producer of codes (a ring of stages of 256 elements of K) and exponents (a ring of 1024)
+//   warp 1            issuer of tcgen05.cp and tcgen05.mma
+//   warps 2-5 (2-9)   epilogue: accumulator -> bias -> rounding -> C
+//   the last two      exponents: rows of eight words -> lanes of four rows, 128 rows at a time
 // in three forms:
 //   kPair    256 rows of A x BN columns of C on two CTAs (cta_group::2): each holds its 128 rows of A and half of the
 //            tile's rows of B, so that an SM's shared memory is read and filled for B half as often;
@@ -35,7 +35,6 @@ namespace {
 constexpr int kTileM = 128;
 constexpr int kStageK = 256;       // elements of K a stage: one 128-byte swizzle row of codes
 constexpr int kChunk = 4;           // stages that a piece of exponents lasts: 32 bytes (a sector) of each row
-constexpr int kThreads = 256;      // registers are handed out for multiples of 128 threads: 288 would leave 168 each
 constexpr int kMaxGroups = 1024;
 enum MxMode { kSingle, kPair, kFew };
 
@@ -68,8 +67,11 @@ struct MxCfg {
   static constexpr int kSfCols = 2 * (kSfN + 4);
   static constexpr int kSfBase = kAccs * BN;
   static constexpr int kSfBufs = (512 - kSfBase) / kSfCols;
-  // staging: two buffers of 32 rows x 128 bytes of C a warp, or the partial tiles of a cluster
-  static constexpr int kEpi = MODE == kFew ? BN * kTileM * 4 : 4 * 2 * 4096;
+  // staging: one or two buffers of 32 rows x 128 bytes of C a warp, or the partial tiles of a cluster
+  static constexpr int kEpiWarps = kAccs == 1 ? 8 : 4;               // two a lane quadrant share the columns of a lone accumulator
+  static constexpr int kEpiBufs = kAccs == 1 ? 1 : 2;
+  static constexpr int kThreads = 128 + 32 * kEpiWarps;
+  static constexpr int kEpi = MODE == kFew ? BN * kTileM * 4 : kEpiWarps * kEpiBufs * 4096;
   static constexpr int kTable = 2 * (kMaxGroups + 1) * 4;
   static constexpr int kFixed = kSfStages * kSfStage + kEpi + 512 /*barriers*/ + kTable + 1024 /*alignment*/;
   static constexpr int kFit = (227 * 1024 - kFixed) / kStage;
@@ -239,7 +241,7 @@ __device__ __forceinline__ void stage_half(uint8_t *row, int lane, int half, con
 // An epilogue warp's 32 rows of C, 128 bytes a row at a time: staged in shared memory and sent by a TMA store; where
 // that cannot be (rows behind the group's end in the box, C's rows not 16-byte aligned) the warp stores them itself,
 // row by row.
-struct RowWriter {
+template <int BUFS> struct RowWriter {
   const MxParams &p;
   const CUtensorMap *tmap_out;
   const MxTile &t;
@@ -256,16 +258,17 @@ struct RowWriter {
   }
   // the buffer for the next piece: this lane's row of it
   __device__ __forceinline__ uint8_t *begin() {
-    if (by_tma && lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");   // the store of two pieces ago has read it
+    // the store that last used it has read it (it may have been an earlier tile's)
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(BUFS - 1) : "memory");
     __syncwarp();
-    return stage + (nstores & 1u) * 4096 + lane * 128;
+    return stage + nstores % BUFS * 4096 + lane * 128;
   }
   __device__ __forceinline__ void send(int64_t col0, int cols) {     // `cols` of C from col0 on, at most 128 bytes
-    uint8_t *buf = stage + (nstores & 1u) * 4096;
+    uint8_t *buf = stage + nstores % BUFS * 4096;
     if (by_tma) {
       fence_proxy_async();
       __syncwarp();
-      if (lane == 0) tma_store_2d(tmap_out, static_cast<int>(col0) * eb, row0, stage_addr + (nstores & 1u) * 4096);
+      if (lane == 0) tma_store_2d(tmap_out, static_cast<int>(col0) * eb, row0, stage_addr + nstores % BUFS * 4096);
       ++nstores;
       return;
     }
@@ -315,16 +318,17 @@ struct RowWriter {
 // One accumulator -> C.  `release()` hands the accumulator back to the issuer.  With a second accumulator the issuer is
 // busy meanwhile and the columns go out as they come; with one (BN = 256) it is waiting: 16-bit results are first taken
 // into registers whole.
-template <int BN, bool kDrain, class Release>
-__device__ __forceinline__ void store_rows(const MxParams &p, RowWriter &out, uint32_t acc, const MxTile &t, int lane, Release release) {
+// (BN columns from n0 on are this warp's; acc is their first.)
+template <int BN, bool kDrain, class Writer, class Release>
+__device__ __forceinline__ void store_rows(const MxParams &p, Writer &out, uint32_t acc, int group, int n0, int lane, Release release) {
   if (p.out_dtype == BSIR_F32) {
-    for (int c0 = 0; c0 < BN && t.n0 + c0 < p.n; c0 += 32) {
+    for (int c0 = 0; c0 < BN && n0 + c0 < p.n; c0 += 32) {
       uint32_t r[32];
-      load_columns(p, acc + static_cast<uint32_t>(c0), t.group, t.n0 + c0, lane, r);
+      load_columns(p, acc + static_cast<uint32_t>(c0), group, n0 + c0, lane, r);
       uint8_t *row = out.begin();
       stage_half(row, lane, 0, r);
       stage_half(row, lane, 1, r + 16);
-      out.send(t.n0 + c0, 32);
+      out.send(n0 + c0, 32);
     }
     release();
   } else if constexpr (kDrain) {
@@ -352,30 +356,30 @@ __device__ __forceinline__ void store_rows(const MxParams &p, RowWriter &out, ui
     release();
 #pragma unroll
     for (int c = 0; c < BN / 64; ++c) {
-      if (t.n0 + 64 * c >= p.n) break;
+      if (n0 + 64 * c >= p.n) break;
       uint8_t *row = out.begin();
       stage_half(row, lane, 0, w + 32 * c);
       stage_half(row, lane, 1, w + 32 * c + 16);
-      out.send(t.n0 + 64 * c, 64);
+      out.send(n0 + 64 * c, 64);
     }
   } else {
-    for (int c0 = 0; c0 < BN && t.n0 + c0 < p.n; c0 += 64) {
+    for (int c0 = 0; c0 < BN && n0 + c0 < p.n; c0 += 64) {
       uint32_t r[32], w[16];
-      load_columns(p, acc + static_cast<uint32_t>(c0), t.group, t.n0 + c0, lane, r);
+      load_columns(p, acc + static_cast<uint32_t>(c0), group, n0 + c0, lane, r);
       round_columns(p, r, w);
       uint8_t *row = out.begin();
       stage_half(row, lane, 0, w);
-      load_columns(p, acc + static_cast<uint32_t>(c0 + 32), t.group, t.n0 + c0 + 32, lane, r);
+      load_columns(p, acc + static_cast<uint32_t>(c0 + 32), group, n0 + c0 + 32, lane, r);
       round_columns(p, r, w);
       stage_half(row, lane, 1, w);
-      out.send(t.n0 + c0, 64);
+      out.send(n0 + c0, 64);
     }
     release();
   }
 }
 
 template <int BN, int MODE>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(MxCfg<BN, MODE>::kThreads, 1)
     mxfp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_m, const __grid_constant__ CUtensorMap tmap_n,
                       const __grid_constant__ CUtensorMap tmap_sm, const __grid_constant__ CUtensorMap tmap_sn,
                       const __grid_constant__ CUtensorMap tmap_out, MxParams p) {
@@ -416,7 +420,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(sf_full_bar(s), 1); mbar_init(sf_empty_bar(s), 1); mbar_init(sf_ready_bar(s), Cfg::kSfBlocks * (PAIR ? 2 : 1));
     }
     for (int b = 0; b < 2; ++b) {
-      mbar_init(acc_full_bar(b), 1); mbar_init(acc_empty_bar(b), PAIR ? 8 : 4);
+      mbar_init(acc_full_bar(b), 1); mbar_init(acc_empty_bar(b), Cfg::kEpiWarps * (PAIR ? 2 : 1));
     }
     mbar_init(red_full, 1);
     *abort_flag = 0;
@@ -573,15 +577,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (++acc == Cfg::kAccs) { acc = 0; acc_phase ^= 1u; }
       }
     }
-  } else if (warp >= 6) {
-    // ---------------- exponents: this warp's block of 128 rows, turned in place: row r's words w -> lane r % 32 of word w
+  } else if (warp >= 2 + Cfg::kEpiWarps) {
+    // ---------------- exponents: blocks of 128 rows, turned in place: row r's words w -> lane r % 32 of word w
     int sf = 0;
     uint32_t sf_phase = 0;
     bool ok = true;
     for (int tile = first_tile; tile < total_tiles && ok; tile += tile_step) {
       for (int c = chunk0; c < chunk1; ++c) {
         if (!mbar_wait(sf_full_bar(sf), sf_phase, abort_flag, p.err)) { ok = false; break; }
-        for (int block = warp - 6; block < Cfg::kSfBlocks; block += 2) {
+        for (int block = warp - 2 - Cfg::kEpiWarps; block < Cfg::kSfBlocks; block += 2) {
           uint4 *rows = reinterpret_cast<uint4 *>(gen + Cfg::kSfOff + sf * Cfg::kSfStage + block * 4096);
           uint4 lo[4], hi[4];                          // rows lane, 32 + lane, ..: words 0-3 and 4-7
 #pragma unroll
@@ -611,8 +615,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else {
     // ---------------- epilogue
     const int quad = warp & 3;
-    uint8_t *stage = gen + Cfg::kEpiOff + (warp - 2) * 8192;
-    const uint32_t stage_addr = base + Cfg::kEpiOff + (warp - 2) * 8192;
+    uint8_t *stage = gen + Cfg::kEpiOff + (warp - 2) * (Cfg::kEpiBufs * 4096);
+    const uint32_t stage_addr = base + Cfg::kEpiOff + (warp - 2) * (Cfg::kEpiBufs * 4096);
+    constexpr int kCols = BN / (Cfg::kEpiWarps / 4);         // this warp's columns of a tile, from c_first on
+    const int c_first = (warp - 2) / 4 * kCols;
     int acc = 0;
     uint32_t acc_phase = 0, nstores = 0;
     bool ok = true;
@@ -622,8 +628,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (p.bias && p.out_dtype != BSIR_F32) {
           if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
           __syncwarp();
-          for (int c = lane; c < BN; c += 32)
-            reinterpret_cast<float *>(stage)[c] = t.n0 + c < p.n ? load_float(p.bias, p.bias_dtype, t.group * p.bias_stride + t.n0 + c) : 0.0f;
+          const int64_t n0 = t.n0 + c_first;
+          for (int c = lane; c < kCols; c += 32)
+            reinterpret_cast<float *>(stage)[c] = n0 + c < p.n ? load_float(p.bias, p.bias_dtype, t.group * p.bias_stride + n0 + c) : 0.0f;
           __syncwarp();
         }
       }
@@ -691,8 +698,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       } else {
         const int row0 = t.row0 + (PAIR ? rank * kTileM : 0) + quad * 32;
         if (row0 < t.row_end) {
-          RowWriter out(p, &tmap_out, t, row0, lane, stage, stage_addr, nstores);
-          store_rows<BN, Cfg::kAccs == 1>(p, out, src, t, lane, release);
+          RowWriter<Cfg::kEpiBufs> out(p, &tmap_out, t, row0, lane, stage, stage_addr, nstores);
+          store_rows<kCols, Cfg::kAccs == 1>(p, out, src + static_cast<uint32_t>(c_first), t.group, t.n0 + c_first, lane, release);
         } else {
           release();
         }
@@ -736,8 +743,8 @@ int32_t launch_mx(const MxOperand &a, const MxOperand &b, int64_t k, MxParams p,
   int64_t teams = (device_info().sm_count > 0 ? device_info().sm_count : 148) / team;
   if (teams > max_tiles || (MODE == kFew && split > 1)) teams = max_tiles;     // a cluster that shares K has one tile
   const dim3 grid(static_cast<unsigned>(teams * team));
-  if (team > 1) launch_pdl_cluster(mxfp4_gemm_kernel<BN, MODE>, grid, dim3(kThreads), Cfg::kSmem, st, team, tm, tn, tsm, tsn, tout, p);
-  else launch_pdl(mxfp4_gemm_kernel<BN, MODE>, grid, dim3(kThreads), Cfg::kSmem, st, tm, tn, tsm, tsn, tout, p);
+  if (team > 1) launch_pdl_cluster(mxfp4_gemm_kernel<BN, MODE>, grid, dim3(Cfg::kThreads), Cfg::kSmem, st, team, tm, tn, tsm, tsn, tout, p);
+  else launch_pdl(mxfp4_gemm_kernel<BN, MODE>, grid, dim3(Cfg::kThreads), Cfg::kSmem, st, tm, tn, tsm, tsn, tout, p);
   count_launch();
   return check_launch("matmul_mxfp4");
 }
