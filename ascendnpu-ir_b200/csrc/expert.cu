@@ -18,28 +18,30 @@ namespace bsir {
 namespace {
 
 // ------------------------------------------------------------------------------------------------ sort
-// A stable counting sort.  A CTA counts the experts of its 4096 choices per warp (each warp owns 128 consecutive
-// choices, 32 at a time: the lanes with one expert find each other with match.any, and a choice's rank among them is a
-// popcount), and the counts of the warps before it, of the CTAs before it and of the experts before its own add up to a
-// choice's row.  Up to 4096 choices are one CTA and one launch; more take a counting launch first, whose table of
-// [experts] counts per CTA the placing launch adds up.
+// A stable counting sort in one launch: one CTA for up to 4096 choices, a cluster of eight for more.  Each of the
+// cluster's warps owns a run of consecutive choices and goes over it 32 at a time: the lanes with one expert find each
+// other by ballots over the bits of its number (match.any takes about 70 cycles of the SM, for whatever warp), and a
+// choice's rank among them is a popcount.  That leaves every warp's count of every expert; the counts of the warps
+// before it, of the CTAs before it (read through distributed shared memory) and of the experts before its own add up to
+// a choice's row.  Runs of up to 32 * kSortGroups choices stay in registers with their ranks, longer ones are gone over
+// twice.  No scratch in global memory, and no atomics.
 constexpr int kSortThreads = 1024;
 constexpr int kSortWarps = kSortThreads / 32;
-constexpr int kSortPerWarp = 128;
-constexpr int kSortChunk = kSortWarps * kSortPerWarp;
+constexpr int kSortOneCta = 4096;
+constexpr int kSortCluster = 8;
 constexpr int kMaxExperts = 1024;
 
 struct SortParams {
   const void *ids;
   int64_t n;                  // choices
+  int64_t run;                // choices of a warp, a multiple of 32
   int experts;
   int wide;                   // ids are int64
+  int ctas;                   // of the cluster
   int32_t *offsets, *slots;
-  int32_t *table;             // [chunks][experts] counts, null with one chunk
-  int chunks;
 };
-__device__ __forceinline__ int load_id(const SortParams &p, int64_t i) {
-  if (i >= p.n) return -1;
+__device__ __forceinline__ int load_id(const SortParams &p, int64_t i, int64_t end) {
+  if (i >= end) return -1;
   if (p.wide) {
     const long long v = static_cast<const long long *>(p.ids)[i];
     return v >= 0 && v < p.experts ? static_cast<int>(v) : -1;
@@ -48,8 +50,18 @@ __device__ __forceinline__ int load_id(const SortParams &p, int64_t i) {
   return v >= 0 && v < p.experts ? v : -1;
 }
 
-// exclusive prefix sum over `count[0 .. experts)` by the whole CTA (experts <= kSortThreads); returns this thread's
-// prefix, *total the sum
+// the lanes of the warp whose expert is this lane's (masked choices are one more expert)
+__device__ __forceinline__ unsigned same_expert(int id, int experts, int bits) {
+  const unsigned key = static_cast<unsigned>(id < 0 ? experts : id);
+  unsigned peers = 0xffffffffu;
+  for (int b = 0; b < bits; ++b) {
+    const unsigned set = __ballot_sync(0xffffffffu, key >> b & 1u);
+    peers &= key >> b & 1u ? set : ~set;
+  }
+  return peers;
+}
+
+// exclusive prefix sum of one value a thread over the whole CTA; *total the sum
 __device__ __forceinline__ int cta_prefix(int v, int *warp_sum_s, int *total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int inc = v;
@@ -74,78 +86,115 @@ __device__ __forceinline__ int cta_prefix(int v, int *warp_sum_s, int *total) {
   return inc - v + (warp ? warp_sum_s[warp - 1] : 0);
 }
 
-__global__ void __launch_bounds__(kSortThreads) expert_count_kernel(SortParams p) {
-  __shared__ int count[kMaxExperts];
-  for (int e = threadIdx.x; e < p.experts; e += kSortThreads) count[e] = 0;
-  pdl_launch_dependents();
-  pdl_wait();
-  __syncthreads();
-  const int64_t c0 = static_cast<int64_t>(blockIdx.x) * kSortChunk;
-#pragma unroll
-  for (int u = 0; u < kSortChunk / kSortThreads; ++u) {
-    const int id = load_id(p, c0 + u * kSortThreads + threadIdx.x);
-    if (id >= 0) atomicAdd(&count[id], 1);       // integers: the order does not show
-  }
-  __syncthreads();
-  for (int e = threadIdx.x; e < p.experts; e += kSortThreads) p.table[static_cast<int64_t>(blockIdx.x) * p.experts + e] = count[e];
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ int load_peer(const int *own, int cta) {       // the same shared-memory word in another CTA
+  uint32_t addr = static_cast<uint32_t>(__cvta_generic_to_shared(own)), peer;
+  int v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer) : "r"(addr), "r"(cta));
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(peer) : "memory");
+  return v;
 }
 
-__global__ void __launch_bounds__(kSortThreads) expert_place_kernel(SortParams p) {
-  extern __shared__ uint16_t warp_count[];       // [experts][kSortWarps]: choices of an expert per warp, then before a warp
-  __shared__ int base_s[kMaxExperts];
+constexpr int kSortGroups = 8;                   // of 32 choices that a warp keeps in registers
+template <bool KEEP>
+__global__ void __launch_bounds__(kSortThreads) expert_sort_kernel(SortParams p) {
+  extern __shared__ int warp_count[];            // [kSortWarps][experts]: a warp's choices of an expert, then its next row
+  __shared__ int mine_s[kMaxExperts];            // this CTA's choices of an expert
   __shared__ int warp_sum_s[32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  for (int i = tid; i < p.experts * kSortWarps / 2; i += kSortThreads) reinterpret_cast<uint32_t *>(warp_count)[i] = 0;
+  const int rank = blockIdx.x;                   // the grid is one cluster
+  for (int i = tid; i < p.experts * kSortWarps; i += kSortThreads) warp_count[i] = 0;
   pdl_launch_dependents();
   pdl_wait();
   __syncthreads();
-  const int64_t c0 = static_cast<int64_t>(blockIdx.x) * kSortChunk + warp * kSortPerWarp;
-  int id[kSortPerWarp / 32], rank[kSortPerWarp / 32];
+  const int64_t first = (static_cast<int64_t>(rank) * kSortWarps + warp) * p.run;
+  const int64_t end = first + p.run < p.n ? first + p.run : p.n;
+  const unsigned below = (1u << lane) - 1u;
+  const int bits = 32 - __clz(p.experts);
+  int *own = warp_count + warp * p.experts;
+  int id[kSortGroups], ahead[kSortGroups];       // KEEP: the warp's choices, and how many of their expert come before them
+  if constexpr (KEEP) {
 #pragma unroll
-  for (int u = 0; u < kSortPerWarp / 32; ++u) id[u] = load_id(p, c0 + u * 32 + lane);
+    for (int u = 0; u < kSortGroups; ++u) id[u] = load_id(p, first + u * 32 + lane, end);
 #pragma unroll
-  for (int u = 0; u < kSortPerWarp / 32; ++u) {
-    const unsigned peers = __match_any_sync(0xffffffffu, id[u]);
-    const int before = __popc(peers & ((1u << lane) - 1u));
-    rank[u] = 0;
-    if (id[u] >= 0) rank[u] = warp_count[id[u] * kSortWarps + warp] + before;   // 0 at first, then what the groups before left
-    __syncwarp();
-    if (id[u] >= 0 && before == 0) warp_count[id[u] * kSortWarps + warp] += static_cast<uint16_t>(__popc(peers));
-    __syncwarp();
+    for (int u = 0; u < kSortGroups; ++u) {
+      if (first + u * 32 >= end) break;
+      const unsigned peers = same_expert(id[u], p.experts, bits);
+      ahead[u] = id[u] < 0 ? 0 : own[id[u]] + __popc(peers & below);
+      __syncwarp();
+      if (id[u] >= 0 && (peers & below) == 0) own[id[u]] += __popc(peers);
+      __syncwarp();
+    }
+  } else {
+    for (int64_t i0 = first; i0 < end; i0 += 128) {          // four groups of 32 in flight
+#pragma unroll
+      for (int u = 0; u < 4; ++u) id[u] = load_id(p, i0 + u * 32 + lane, end);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const unsigned peers = same_expert(id[u], p.experts, bits);
+        if (id[u] >= 0 && (peers & below) == 0) own[id[u]] += __popc(peers);
+        __syncwarp();
+      }
+    }
   }
   __syncthreads();
-  // per expert: counts of the warps -> counts of the warps before, this chunk's total; of the other chunks: those before
-  // this one and all
-  int mine = 0, earlier = 0, all = 0;
+  int mine = 0;
   if (tid < p.experts) {
-    for (int w = 0; w < kSortWarps; ++w) {
-      const int c = warp_count[tid * kSortWarps + w];
-      warp_count[tid * kSortWarps + w] = static_cast<uint16_t>(mine);
-      mine += c;
-    }
-    if (p.table) {
-      for (int b = 0; b < p.chunks; ++b) {
-        const int c = p.table[static_cast<int64_t>(b) * p.experts + tid];
-        if (b < static_cast<int>(blockIdx.x)) earlier += c;
-        all += c;
-      }
-    } else {
-      all = mine;
+#pragma unroll 8
+    for (int w = 0; w < kSortWarps; ++w) mine += warp_count[w * p.experts + tid];
+    mine_s[tid] = mine;
+  }
+  if (p.ctas > 1) cluster_barrier();
+  int earlier = 0, all = mine;
+  if (p.ctas > 1 && tid < p.experts) {
+    all = 0;
+    for (int c = 0; c < p.ctas; ++c) {
+      const int v = load_peer(&mine_s[tid], c);
+      if (c < rank) earlier += v;
+      all += v;
     }
   }
   int total;
   const int start = cta_prefix(all, warp_sum_s, &total);
   if (tid < p.experts) {
-    base_s[tid] = start + earlier;
-    if (blockIdx.x == 0) p.offsets[tid] = start;
+    int next = start + earlier;
+#pragma unroll 8
+    for (int w = 0; w < kSortWarps; ++w) {
+      const int c = warp_count[w * p.experts + tid];
+      warp_count[w * p.experts + tid] = next;
+      next += c;
+    }
+    if (rank == 0) p.offsets[tid] = start;
   }
-  if (blockIdx.x == 0 && tid == 0) p.offsets[p.experts] = total;
+  if (rank == 0 && tid == 0) p.offsets[p.experts] = total;
   __syncthreads();
+  if constexpr (KEEP) {
 #pragma unroll
-  for (int u = 0; u < kSortPerWarp / 32; ++u) {
-    const int64_t i = c0 + u * 32 + lane;
-    if (i < p.n) p.slots[i] = id[u] < 0 ? -1 : base_s[id[u]] + warp_count[id[u] * kSortWarps + warp] + rank[u];
+    for (int u = 0; u < kSortGroups; ++u) {
+      const int64_t i = first + u * 32 + lane;
+      if (i < end) p.slots[i] = id[u] < 0 ? -1 : own[id[u]] + ahead[u];
+    }
+  } else {
+    for (int64_t i0 = first; i0 < end; i0 += 128) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) id[u] = load_id(p, i0 + u * 32 + lane, end);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const unsigned peers = same_expert(id[u], p.experts, bits);
+        const int at = id[u] < 0 ? 0 : id[u];
+        const int row = own[at] + __popc(peers & below);
+        __syncwarp();
+        if (id[u] >= 0 && (peers & below) == 0) own[at] += __popc(peers);
+        __syncwarp();
+        const int64_t i = i0 + u * 32 + lane;
+        if (i < end) p.slots[i] = id[u] < 0 ? -1 : row;
+      }
+    }
   }
+  if (p.ctas > 1) cluster_barrier();             // a peer may still be reading this CTA's counts
 }
 
 // ------------------------------------------------------------------------------------------------ movement
@@ -447,17 +496,13 @@ int32_t bsir_expert_sort(int32_t id_dtype, int64_t tokens, int64_t top_k, int64_
   SortParams p{};
   p.ids = ids; p.n = n; p.experts = static_cast<int>(experts); p.wide = id_dtype == BSIR_I64;
   p.offsets = offsets; p.slots = slots;
-  p.chunks = static_cast<int>(n > 0 ? ceil_div(n, kSortChunk) : 1);
-  const size_t smem = static_cast<size_t>(experts) * kSortWarps * 2;
-  cudaFuncSetAttribute(expert_place_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxExperts * kSortWarps * 2);
-  if (p.chunks > 1) {
-    char *ws = static_cast<char *>(device_workspace(kScratchCounterBytes + static_cast<size_t>(p.chunks) * experts * 4, st));
-    if (!ws) return BSIR_ERR_WORKSPACE;
-    p.table = reinterpret_cast<int32_t *>(ws + kScratchCounterBytes);
-    launch_pdl(expert_count_kernel, dim3(p.chunks), dim3(kSortThreads), 0, st, p);
-    count_launch();
-  }
-  launch_pdl(expert_place_kernel, dim3(p.chunks), dim3(kSortThreads), smem, st, p);
+  p.ctas = n > kSortOneCta ? kSortCluster : 1;
+  p.run = ceil_div(ceil_div(n, static_cast<int64_t>(p.ctas) * kSortWarps), 32) * 32;
+  const size_t smem = static_cast<size_t>(experts) * kSortWarps * 4;
+  auto kernel = p.run <= 32 * kSortGroups ? expert_sort_kernel<true> : expert_sort_kernel<false>;
+  cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxExperts * kSortWarps * 4);
+  if (p.ctas > 1) launch_pdl_cluster(kernel, dim3(p.ctas), dim3(kSortThreads), smem, st, p.ctas, p);
+  else launch_pdl(kernel, dim3(1), dim3(kSortThreads), smem, st, p);
   count_launch();
   return check_launch("expert_sort");
 }

@@ -316,21 +316,48 @@ template <int BUFS> struct RowWriter {
 };
 
 // One accumulator -> C.  `release()` hands the accumulator back to the issuer.  With a second accumulator the issuer is
-// busy meanwhile and the columns go out as they come; with one (BN = 256) it is waiting: 16-bit results are first taken
-// into registers whole.
+// busy meanwhile and the columns go out as they come; with one (BN = 256) it is waiting: the warp's columns are first
+// taken into registers whole.
 // (BN columns from n0 on are this warp's; acc is their first.)
 template <int BN, bool kDrain, class Writer, class Release>
 __device__ __forceinline__ void store_rows(const MxParams &p, Writer &out, uint32_t acc, int group, int n0, int lane, Release release) {
   if (p.out_dtype == BSIR_F32) {
-    for (int c0 = 0; c0 < BN && n0 + c0 < p.n; c0 += 32) {
-      uint32_t r[32];
-      load_columns(p, acc + static_cast<uint32_t>(c0), group, n0 + c0, lane, r);
-      uint8_t *row = out.begin();
-      stage_half(row, lane, 0, r);
-      stage_half(row, lane, 1, r + 16);
-      out.send(n0 + c0, 32);
+    if constexpr (kDrain) {
+      uint32_t r[BN];
+#pragma unroll
+      for (int c = 0; c < BN; c += 32) tmem_ld32(acc + static_cast<uint32_t>(c), r + c);
+      tmem_ld_wait();
+      release();
+      if (p.bias) {
+        const float4 *bias = reinterpret_cast<const float4 *>(out.stage);
+#pragma unroll
+        for (int j = 0; j < BN / 4; ++j) {
+          const float4 b = bias[j];
+          r[4 * j] = __float_as_uint(__fadd_rn(__uint_as_float(r[4 * j]), b.x));
+          r[4 * j + 1] = __float_as_uint(__fadd_rn(__uint_as_float(r[4 * j + 1]), b.y));
+          r[4 * j + 2] = __float_as_uint(__fadd_rn(__uint_as_float(r[4 * j + 2]), b.z));
+          r[4 * j + 3] = __float_as_uint(__fadd_rn(__uint_as_float(r[4 * j + 3]), b.w));
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < BN; c += 32) {
+        if (n0 + c >= p.n) break;
+        uint8_t *row = out.begin();
+        stage_half(row, lane, 0, r + c);
+        stage_half(row, lane, 1, r + c + 16);
+        out.send(n0 + c, 32);
+      }
+    } else {
+      for (int c0 = 0; c0 < BN && n0 + c0 < p.n; c0 += 32) {
+        uint32_t r[32];
+        load_columns(p, acc + static_cast<uint32_t>(c0), group, n0 + c0, lane, r);
+        uint8_t *row = out.begin();
+        stage_half(row, lane, 0, r);
+        stage_half(row, lane, 1, r + 16);
+        out.send(n0 + c0, 32);
+      }
+      release();
     }
-    release();
   } else if constexpr (kDrain) {
     uint32_t w[BN / 2];
     const float4 *bias = reinterpret_cast<const float4 *>(out.stage);     // put there before the accumulator was waited for
@@ -625,7 +652,7 @@ __global__ void __launch_bounds__(MxCfg<BN, MODE>::kThreads, 1)
     for (int tile = first_tile; tile < total_tiles && ok; tile += tile_step) {
       find_tile<kRows, kColsC>(tile, tile_start, row_start, group, t);
       if constexpr (!SWAP && Cfg::kAccs == 1) {       // the tile's bias into the staging buffer, which is idle until then
-        if (p.bias && p.out_dtype != BSIR_F32) {
+        if (p.bias) {
           if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
           __syncwarp();
           const int64_t n0 = t.n0 + c_first;
@@ -807,7 +834,7 @@ extern "C" int32_t bsir_matmul_mxfp4(const bsir_matmul_mxfp4_desc *d, void *stre
   p.err = device_error_word();
   if (!p.err) return fail(BSIR_ERR_WORKSPACE, "matmul_mxfp4: no device error word");
   cudaStream_t st = resolve_stream(stream);
-  p.tma_out = aligned_to(d->out, 16) && (ldo * eb) % 16 == 0;
+  p.tma_out = aligned_to(d->out, 16) && (ldo * eb) % 16 == 0 && d->n * eb <= 0x7fffffff;     // its coordinates are 32-bit bytes
   // Which form: from the rows of a group, all of them or the groups' mean (their sizes are on the device).  Measured
   // (N x K = 4096 x 4096 | 14336 x 4096, bf16 out): up to 16 rows kFew<16> 7.0-7.6 | 9.1-9.6 us, kSingle 7.8 | 12-14;
   // 32 rows kFew<32> 8.6 | 10.4, kSingle 8.0 | 12.2; 48 rows kFew<32> 8.7 | 13.8, kSingle 7.8 | 12.3.
@@ -823,17 +850,15 @@ extern "C" int32_t bsir_matmul_mxfp4(const bsir_matmul_mxfp4_desc *d, void *stre
     while (split < 8 && nt * split * 2 <= sms && ceil_div(chunks, 2 * split) * (2 * split - 1) < chunks) split *= 2;
     return rows <= 16 ? launch_mx<16, kFew>(a, b, d->k, p, split, nt, st) : launch_mx<32, kFew>(a, b, d->k, p, split, nt, st);
   }
-  // Rounds of tiles over the SMs x time of a tile, in units of 5 ns: a stage takes 305 ns on one CTA with 128 x 128
-  // and 345 on a pair, with 256 x 256 (plus 1.4 us to drain the one accumulator) or 256 x 192 (two accumulators; f32
-  // results, which a drain could not hold, take this one).  Groups leave half of a last tile empty on average.
+  // Rounds of tiles over the SMs x time of a tile, in units of 5 ns: a stage takes 305 ns on one CTA with 128 x 128 and
+  // 345 on a pair with 256 x 256, plus 1.3 us to drain the one accumulator (measured over 96 .. 4096 rows).  Groups leave
+  // half of a last tile empty on average.
   auto rounds = [&](int64_t r, int64_t c, int64_t at_once) {
     const int64_t nt = groups > 1 ? (d->m / r + groups / 2 + 1) * ceil_div(d->n, c) : tiles(r, c);
     return ceil_div(nt, at_once);
   };
-  const bool wide = d->out_dtype == BSIR_F32;
   const int64_t single = rounds(128, 128, sms) * 61 * p.k_blocks;
-  const int64_t pair = wide ? rounds(256, 192, sms / 2) * 69 * p.k_blocks : rounds(256, 256, sms / 2) * (69 * p.k_blocks + 280);
+  const int64_t pair = rounds(256, 256, sms / 2) * (69 * p.k_blocks + 260);
   if (single <= pair) return launch_mx<128, kSingle>(a, b, d->k, p, 1, tiles(128, 128), st);
-  if (wide) return launch_mx<192, kPair>(a, b, d->k, p, 1, tiles(256, 192), st);
   return launch_mx<256, kPair>(a, b, d->k, p, 1, tiles(256, 256), st);
 }

@@ -452,7 +452,7 @@ __global__ void __launch_bounds__(256) mxfp4_dequant_kernel(DequantParams p) {
 #pragma unroll
   for (int u = 0; u < kRowVecs; ++u) {
     const uint32_t i = v0 + u * 256u;
-    if (i >= p.nvec || (!FLAT && col[u] >= p.cols)) continue;
+    const bool live = i < p.nvec && (FLAT || col[u] < p.cols);
     uint32_t w[kWords];
     dequant8<DT>(codes[u], byte[u], w);
     const int64_t at = FLAT ? static_cast<int64_t>(i) * 8 : static_cast<int64_t>(row[u]) * p.ys + col[u];
@@ -465,17 +465,18 @@ __global__ void __launch_bounds__(256) mxfp4_dequant_kernel(DequantParams p) {
         uint32_t a[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const uint32_t got = __shfl_xor_sync(__activemask(), odd ? w[j] : w[4 + j], 1);
-          a[j] = got;
+          a[j] = __shfl_xor_sync(0xffffffffu, odd ? w[j] : w[4 + j], 1);
         }
         const Vec16 mine{{odd ? w[4] : w[0], odd ? w[5] : w[1], odd ? w[6] : w[2], odd ? w[7] : w[3]}}, other{{a[0], a[1], a[2], a[3]}};
-        st_stream(odd ? dst - 16 : dst, odd ? other : mine);
-        st_stream(odd ? dst + 16 : dst + 32, odd ? mine : other);
-      } else {
+        if (live) {
+          st_stream(odd ? dst - 16 : dst, odd ? other : mine);
+          st_stream(odd ? dst + 16 : dst + 32, odd ? mine : other);
+        }
+      } else if (live) {
 #pragma unroll
         for (int j = 0; j < kWords; j += 4) st_stream(dst + 4 * j, Vec16{{w[j], w[j + 1], w[j + 2], w[j + 3]}});
       }
-    } else {
+    } else if (live) {
       for (int j = 0; j < 8 && col[u] + j < p.cols; ++j) {
         if constexpr (DT == BSIR_F32) static_cast<uint32_t *>(p.y)[at + j] = w[j];
         else static_cast<uint16_t *>(p.y)[at + j] = static_cast<uint16_t>(w[j >> 1] >> (16 * (j & 1)));

@@ -562,8 +562,7 @@ BSIR_API int32_t bsir_matmul_mxfp4(const bsir_matmul_mxfp4_desc *desc, void *str
 /* Tokens sorted by expert.  ids [tokens, top_k] (int32 or int64): the expert of each choice; a number outside
  * 0 .. experts - 1 names none (a padding token, an expert of another rank): such a choice is masked.
  * offsets [experts + 1]: rows offsets[e] .. offsets[e + 1] belong to expert e.  slots [tokens, top_k]: the row of each
- * choice, -1 for a masked one; rows of one expert keep the order of their choices.  experts <= 1024; more than 4096
- * choices take the library's scratch (4 bytes x experts for each 4096 choices). */
+ * choice, -1 for a masked one; rows of one expert keep the order of their choices.  experts <= 1024. */
 BSIR_API int32_t bsir_expert_sort(int32_t id_dtype, int64_t tokens, int64_t top_k, int64_t experts, const void *ids,
                                   int32_t *offsets, int32_t *slots, void *stream);
 /* out[slots[t, j]] = x[t] for every choice that is not masked; other rows of out are left as they were.  Any element
