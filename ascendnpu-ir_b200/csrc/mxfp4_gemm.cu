@@ -8,10 +8,14 @@
 // (a 128-byte row is 256 elements of K); the exponents have to lie in tensor memory: row r of an operand tile at lane
 // r % 32, column r / 32, four bytes (128 elements of K) a cell, the same in all four lane quadrants.  The exponent
 // matrices keep the plain [rows, K / 32] layout, so groups may start at any row: TMA brings [rows x 32 bytes] (1024
-// elements of K), a warp per 128 rows turns them in shared memory from a row's eight words into a lane's four rows, and
-// the MMA issuer copies them to tensor memory with tcgen05.cp ahead of the instructions that use them.  (Warps storing
-// them to tensor memory themselves were the first form: next to cta_group::2 instructions such a store took 1400
-// cycles, and a chunk of 512 elements of K is 1024 of multiplication.)
+// elements of K; 16 bytes a row moved half-empty sectors and cost 4 to 9 %), warps turn them in shared memory from a row's
+// eight words into a lane's four rows, and the MMA issuer copies them to tensor memory with tcgen05.cp ahead of the
+// instructions that use them, in order and without a barrier between.
+//
+// What bounds it (B200, 4096 x 14336 x 4096): a stage of 256 x 256 tiles is 512 cycles of multiplication and takes about
+// 550, with the pair's 35 KB a CTA coming from L2 at 60 of the 64 bytes a cycle that reach an SM; the accumulator's way
+// out costs 1400 cycles a tile; sustained, the board's power limit lowers the clock to 1.5 GHz.  92 us when cool, 110
+// sustained (4.4 PFLOP/s).  Up to 32 rows the weights' way from HBM bounds it.
 //
 // A persistent kernel, one CTA per SM, 256 threads (384 with one accumulator):
 //   warp 0            TMA producer of codes (a ring of stages of 256 elements of K) and exponents (a ring of 1024)
@@ -405,6 +409,11 @@ __device__ __forceinline__ void store_rows(const MxParams &p, Writer &out, uint3
   }
 }
 
+// The bounded wait for a whole warp: all lanes go on or all give up, so that none is left at a warp barrier.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int *abort_flag, int *err) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, err)) != 0;
+}
+
 template <int BN, int MODE>
 __global__ void __launch_bounds__(MxCfg<BN, MODE>::kThreads, 1)
     mxfp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_m, const __grid_constant__ CUtensorMap tmap_n,
@@ -570,13 +579,13 @@ __global__ void __launch_bounds__(MxCfg<BN, MODE>::kThreads, 1)
       uint32_t phase = 0, sf_phase = 0, acc_phase = 0;
       bool ok = true, here = false, sf_here = false;
       for (int tile = first_tile; tile < total_tiles && ok; tile += tile_step) {
-        if (!mbar_wait(acc_empty_bar(acc), acc_phase ^ 1u, abort_flag, p.err)) break;
+        if (!warp_wait(acc_empty_bar(acc), acc_phase ^ 1u, abort_flag, p.err)) break;
         const uint32_t d = tmem + static_cast<uint32_t>(acc * BN);
         for (int kb = kb0; kb < kb1; ++kb) {
           const uint32_t part = static_cast<uint32_t>(kb) % kChunk;          // of the chunk
           // the next barriers were looked at while the last stage's instructions went out
-          if (part == 0 && !sf_here && !mbar_wait(sf_ready_bar(sf), sf_phase, abort_flag, p.err)) { ok = false; break; }
-          if (!here && !mbar_wait(full_bar(stage), phase, abort_flag, p.err)) { ok = false; break; }
+          if (part == 0 && !sf_here && !warp_wait(sf_ready_bar(sf), sf_phase, abort_flag, p.err)) { ok = false; break; }
+          if (!here && !warp_wait(full_bar(stage), phase, abort_flag, p.err)) { ok = false; break; }
           tc_fence_after();
           // the stage's codes have landed, so the instructions that used its columns of exponents before are done
           const uint32_t sfb = tmem + static_cast<uint32_t>(Cfg::kSfBase + stage * Cfg::kSfCols), sfa = sfb + 2 * Cfg::kSfN;
@@ -598,8 +607,8 @@ __global__ void __launch_bounds__(MxCfg<BN, MODE>::kThreads, 1)
           if (kb + 1 == kb1) commit_to<MODE>(elected, acc_full_bar(acc));
           if (++stage == Cfg::kStages) { stage = 0; phase ^= 1u; }
           if (sf_done && ++sf == Cfg::kSfStages) { sf = 0; sf_phase ^= 1u; }
-          here = mbar_test(full_bar(stage), phase);
-          sf_here = sf_done && mbar_test(sf_ready_bar(sf), sf_phase);
+          here = __all_sync(0xffffffffu, mbar_test(full_bar(stage), phase));
+          sf_here = sf_done && __all_sync(0xffffffffu, mbar_test(sf_ready_bar(sf), sf_phase));
         }
         if (++acc == Cfg::kAccs) { acc = 0; acc_phase ^= 1u; }
       }
@@ -611,7 +620,7 @@ __global__ void __launch_bounds__(MxCfg<BN, MODE>::kThreads, 1)
     bool ok = true;
     for (int tile = first_tile; tile < total_tiles && ok; tile += tile_step) {
       for (int c = chunk0; c < chunk1; ++c) {
-        if (!mbar_wait(sf_full_bar(sf), sf_phase, abort_flag, p.err)) { ok = false; break; }
+        if (!warp_wait(sf_full_bar(sf), sf_phase, abort_flag, p.err)) { ok = false; break; }
         for (int block = warp - 2 - Cfg::kEpiWarps; block < Cfg::kSfBlocks; block += 2) {
           uint4 *rows = reinterpret_cast<uint4 *>(gen + Cfg::kSfOff + sf * Cfg::kSfStage + block * 4096);
           uint4 lo[4], hi[4];                          // rows lane, 32 + lane, ..: words 0-3 and 4-7
@@ -661,7 +670,7 @@ __global__ void __launch_bounds__(MxCfg<BN, MODE>::kThreads, 1)
           __syncwarp();
         }
       }
-      if (!mbar_wait(acc_full_bar(acc), acc_phase, abort_flag, p.err)) break;
+      if (!warp_wait(acc_full_bar(acc), acc_phase, abort_flag, p.err)) break;
       tc_fence_after();
       const uint32_t src = tmem + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>(acc * BN);
       auto release = [&]() {
@@ -707,7 +716,7 @@ __global__ void __launch_bounds__(MxCfg<BN, MODE>::kThreads, 1)
                        map_to_cta(red_full, to));
             }
           }
-          if (!mbar_wait(red_full, 0u, abort_flag, p.err)) break;
+          if (!warp_wait(red_full, 0u, abort_flag, p.err)) break;
           const float2 *part = reinterpret_cast<const float2 *>(gen + Cfg::kEpiOff) + quad * 32 + lane;
           for (int j = 0; j < own; j += 2) {
             float2 sum = part[j / 2 * kTileM];
@@ -809,6 +818,7 @@ extern "C" int32_t bsir_matmul_mxfp4(const bsir_matmul_mxfp4_desc *d, void *stre
                   (long long)o->code_bs, (long long)o->scale_bs);
     if (!aligned_to(o->codes, 16) || !aligned_to(o->scales, 16)) return fail(BSIR_ERR_ALIGN, "matmul_mxfp4: %s and its exponents want 16-byte aligned bases", name);
   }
+  if (d->bias && d->bias_stride < 0) return fail(BSIR_ERR_STRIDE, "matmul_mxfp4: %lld elements between the groups' biases", (long long)d->bias_stride);
   const int eb = dtype_bytes(d->out_dtype);
   const int64_t ldo = d->m == 1 ? d->n : d->ldo;
   if (ldo < d->n) return fail(BSIR_ERR_STRIDE, "matmul_mxfp4: row stride %lld of out for %lld columns", (long long)ldo, (long long)d->n);

@@ -28,7 +28,7 @@ def _ids(tokens, top_k, experts, seed, masked=0.2, skew=False):
     return ids
 
 
-SORTS = [(1, 1, 1), (1, 8, 256), (7, 3, 5), (32, 4, 64), (512, 8, 8), (513, 8, 60), (1000, 5, 1024), (4096, 1, 2), (9001, 6, 128), (70000, 8, 33)]
+SORTS = [(1, 1, 1), (1, 8, 256), (7, 3, 5), (32, 4, 64), (512, 8, 8), (513, 8, 60), (1000, 5, 1024), (4096, 1, 2), (9001, 6, 128), (9000, 7, 127), (70000, 8, 33)]
 
 
 @pytest.mark.parametrize("wide", [False, True])
@@ -51,7 +51,7 @@ def test_sort_extremes(B):
     assert B.expert_sort(big, 2)[1].tolist() == [[-1, -1, 0]]
 
 
-CASES = [(1, 1, 1, 1), (1, 2, 4, 8), (3, 2, 4, 33), (40, 4, 8, 4096), (17, 8, 16, 1000), (65, 6, 7, 514), (300, 9, 40, 72), (5, 16, 64, 12288)]
+CASES = [(1, 1, 1, 1), (1, 2, 4, 8), (3, 2, 4, 33), (40, 4, 8, 4096), (17, 8, 16, 1000), (65, 6, 7, 514), (300, 9, 40, 72), (5, 16, 64, 12288), (4, 70, 100, 200)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16, torch.uint8, torch.int64])
@@ -154,6 +154,23 @@ def test_strided_and_unaligned_rows(B):
     dy2, dw2 = B.expert_combine_grad(x.contiguous(), want, slots, w)
     assert torch.equal(dy, dy2)
     assert (dw - dw2).abs().max() <= 2 * cols * 2.0 ** -24 * (x.float().abs().amax() * want.float().abs().amax() * cols)
+
+
+def test_rows_far_apart(B):
+    """Rows 2^27 elements apart: offsets pass 2^31."""
+    tokens, top_k, cols, pitch = 12, 2, 64, 1 << 27
+    _, slots = B.expert_sort(_ids(tokens, top_k, 4, 9).cuda(), 4)
+    x = torch.randn(tokens, cols, device="cuda").to(torch.bfloat16)
+    w = torch.rand(tokens, top_k, device="cuda")
+    far = torch.empty(24 * pitch, dtype=torch.bfloat16, device="cuda").as_strided((24, cols), (pitch, 1))
+    far.zero_()
+    B.expert_dispatch(x, slots, out=far)
+    near = B.expert_dispatch(x, slots)
+    assert torch.equal(far.contiguous(), near)
+    assert torch.equal(B.expert_combine(far, slots, w), B.expert_combine(near, slots, w))
+    dy, dw = B.expert_combine_grad(x, near, slots, w)
+    far_dy, far_dw = B.expert_combine_grad(x, far, slots, w)
+    assert torch.equal(dy, far_dy) and torch.equal(dw, far_dw)
 
 
 def test_bad_slots_are_masked_and_reported(B):

@@ -82,6 +82,39 @@ def test_quant_columns_and_both(B, rows, cols, dtype):
     _same(torch.from_numpy(R.decode(q2, s2, cols)), wv)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_quant_ends_of_the_range(B, dtype):
+    """Blocks at every exponent of the type, subnormals and the largest values among them, both ways."""
+    g = torch.Generator().manual_seed(0)
+    lo, hi = (-24, 15) if dtype == torch.float16 else (-140, 127)
+    e = torch.arange(lo, hi + 1).double()
+    x = torch.ldexp(torch.rand(len(e), 32, generator=g).double() * 1.98 - 0.99, e[:, None]).to(dtype)
+    _, ws, wv = R.quant(x)
+    q, s = B.quant_mxfp4(x.cuda())
+    assert np.array_equal(s.cpu().numpy(), ws)
+    _same(torch.from_numpy(R.decode(q, s, 32)), wv)
+    _same(B.dequant_mxfp4(q, s, dtype), wv)
+    qt, st = B.quant_mxfp4(x.t().contiguous().cuda(), axis=0)
+    assert torch.equal(qt, q) and torch.equal(st, s)
+
+
+def test_quant_beyond_32_bits(B):
+    """9.7e9 elements: element numbers, byte offsets and the launch's own indices pass 2^31 and 2^32."""
+    rows, cols = 9, 1 << 30
+    x = torch.zeros(rows, cols, dtype=torch.bfloat16, device="cuda")
+    spots = [(0, 5), (3, cols - 1), (8, 7), (8, cols - 33), (8, cols - 1)]
+    for i, (r, c) in enumerate(spots):
+        x[r, c] = i + 1.0
+    q, s = B.quant_mxfp4(x)
+    for i, (r, c) in enumerate(spots):
+        _, byte, v = R.quant(x[r:r + 1, c // 32 * 32:c // 32 * 32 + 32])
+        assert s[r, c // 32].item() == byte[0, 0]
+        assert R.decode(q[r:r + 1, c // 32 * 16:c // 32 * 16 + 16], s[r:r + 1, c // 32:c // 32 + 1], 32)[0, c % 32] == v[0, c % 32]
+    assert sum(int((q[r] != 0).sum()) for r in range(rows)) == len(spots)
+    y = B.dequant_mxfp4(q, s, torch.bfloat16)
+    assert all(y[r, c].item() == {1: 1, 2: 2, 3: 3, 4: 4, 5: 4}[i + 1] for i, (r, c) in enumerate(spots))
+
+
 @pytest.mark.parametrize("offset,pitch", [(0, 0), (1, 3), (8, 8), (2, 0)])
 def test_quant_strides_and_alignment(B, offset, pitch):
     rows, cols = 9, 96
@@ -240,6 +273,19 @@ def test_linear_backward_and_gradient_by_differences(B):
             vals.append(f())
         a[r, c // 2] = keep
         assert (vals[0] - vals[1]) / 2 == grad[r, c]
+
+
+@pytest.mark.parametrize("m", [20, 60, 300])
+def test_product_into_rows_far_apart(B, m):
+    """Rows of C 2^26 elements apart: their offsets pass 2^31."""
+    n, k, pitch = 128, 512, 1 << 26
+    a, sa = R.random_codes(m, k, 1, 127, 127)
+    b, sb = R.random_codes(n, k, 2, 127, 127)
+    out = torch.empty(m * pitch, dtype=torch.bfloat16, device="cuda").as_strided((m, n), (pitch, 1))
+    B.matmul_mxfp4(a, sa, b, sb, out=out)
+    assert torch.equal(out.contiguous(), B.matmul_mxfp4(a, sa, b, sb))
+    want = torch.from_numpy(R.decode(a, sa, k) @ R.decode(b, sb, k).T).float().to(torch.bfloat16)
+    assert torch.equal(out.cpu(), want)
 
 
 def test_capture_streams_and_repeats(B):

@@ -93,6 +93,7 @@ def test_product_refusals(L):
     assert _product(L, batch_stride_b=64 * 256 - 16, **off) == -3 and _product(L, batch_stride_sb=1000, **off) == -3
     assert _product(L, a=A0 + 8) == -6 and _product(L, scale_b=A3 + 4) == -6 and _product(L, out=A4 + 1) == -6
     assert _product(L, ldo=63) == -3
+    assert _product(L, bias=A4 + 0x1000000, bias_stride=-64, **off) == -3
     assert _product(L, out=A0 + 16) == -11 and _product(L, offsets=A4 + 64, groups=1) == -11
 
 
