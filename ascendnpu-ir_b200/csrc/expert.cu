@@ -363,7 +363,8 @@ __global__ void __launch_bounds__(kMoveThreads) expert_combine_kernel(RowParams 
   }
 }
 
-// One CTA per token, four choices at a time (eight took 120 registers and 267 us where four take 190): y's rows are
+// One CTA per token, four choices at a time (eight at a time, or dout kept for eight: 120 registers and 267 us, 194 us,
+// where this takes 180 on 64k rows of 4096 bf16): y's rows are
 // read once, dy's written once, dout's once for the four; the dot products meet across the warps in a fixed order.
 constexpr int kGradThreads = 128;
 constexpr int kGradChoices = 4;
