@@ -12,7 +12,7 @@
 //
 // Both directions of a matrix can come out of one read: blocks along the rows (what C = A * B^T contracts) and blocks
 // down the columns with the result transposed (what the products of a backward pass contract).
-#include "common.cuh"
+#include "tc_ptx.cuh"
 
 namespace bsir {
 namespace {
@@ -242,127 +242,88 @@ __global__ void __launch_bounds__(256) mxfp4_rows_kernel(QuantParams p) {
   }
 }
 
-// Blocks down the columns, and along the rows as well when `q` is wanted: a CTA brings a tile of kTR rows x 64 columns
-// into shared memory (16-byte loads, 128 bytes of a row of a 16-bit type; the row-wise form is made from the registers
-// on the way), then a thread takes two neighbouring columns of a 32-row block -- a warp reads one row of the tile at a
-// time -- and its two blocks' codes (16 bytes each) go through shared memory so that a column's codes leave as kTR / 2
-// consecutive bytes.
+// Blocks down the columns, and along the rows as well when `q` is wanted, on tiles of kTR rows x 64 columns in shared
+// memory (128 bytes of a row of a 16-bit type).  Along the rows a thread takes 16 bytes, as above; down the columns it
+// takes two neighbouring columns of a 32-row block -- a warp reads one row of the tile at a time -- and its two blocks'
+// codes (16 bytes each) go through shared memory so that a column's codes leave as kTR / 2 consecutive bytes.
 constexpr int kTC = 64;
 constexpr int kTR = 128;
 constexpr int kColThreads = 128;
-template <int DT, bool VEC>
-__global__ void __launch_bounds__(kColThreads) mxfp4_cols_kernel(QuantParams p) {
-  constexpr int TR = kTR;
+constexpr int kCodeRow = kTR / 2 + 16;                   // bytes of a column's codes, padded against bank conflicts
+constexpr int kColPieces = kTR / kBlock;                 // 16-byte pieces (blocks) of a column of a tile
+
+// this warp's 32-row block b of the tile, lane = a pair of columns -> codes and exponents down the columns
+template <int DT>
+__device__ __forceinline__ void quant_down(const uint8_t *tile, uint8_t *codes_s, uint8_t (*scale_s)[kColPieces], int b) {
   constexpr int EB = 4 / FloatTraits<DT>::kPerWord;
-  constexpr int kWords = 8 / FloatTraits<DT>::kPerWord;
-  constexpr int kCodeRow = TR / 2 + 16;                  // bytes of a column's codes, padded against bank conflicts
-  extern __shared__ __align__(16) uint8_t tile[];        // [TR][kTC] elements, then [kTC][kCodeRow] codes
-  uint8_t *codes_s = tile + TR * kTC * EB;
-  __shared__ uint8_t scale_s[kTC][TR / kBlock];
-  pdl_launch_dependents();
-  pdl_wait();
-  const int64_t r0 = static_cast<int64_t>(blockIdx.y) * TR;
-  const int64_t c0 = static_cast<int64_t>(blockIdx.x) * kTC;
-  const int tid = threadIdx.x;
-  constexpr int kPasses = TR * (kTC / 8) / kColThreads, kAhead = DT == BSIR_F32 ? 4 : kPasses;     // 16-bit: all of a thread's loads ahead of the first use
+  const int lane = threadIdx.x & 31;
+  uint32_t byte[2];
+  uint32_t q0[4], q1[4];
+  const uint8_t *src = tile + (b * kBlock * kTC + 2 * lane) * EB;
+  if constexpr (DT == BSIR_F32) {
+    uint32_t m0 = 0, m1 = 0;
+    float2 x[kBlock];
 #pragma unroll
-  for (int u0 = 0; u0 < kPasses; u0 += kAhead) {
-    uint32_t w[kAhead][kWords];
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      const int i = (u0 + u) * kColThreads + tid, r = i >> 3, c = (i & 7) * 8;
-      load8<DT, VEC>(p.x, (r0 + r) * p.xs, c0 + c, r0 + r < p.rows ? p.cols : 0, w[u]);
+    for (int r = 0; r < kBlock; ++r) {
+      x[r] = *reinterpret_cast<const float2 *>(src + r * kTC * EB);
+      m0 = max(m0, __float_as_uint(x[r].x) & 0x7fffffffu);
+      m1 = max(m1, __float_as_uint(x[r].y) & 0x7fffffffu);
     }
+    byte[0] = scale_byte(m0);
+    byte[1] = scale_byte(m1);
+    const float i0 = inv_scale(byte[0]), i1 = inv_scale(byte[1]);
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      const int i = (u0 + u) * kColThreads + tid, r = i >> 3, c = (i & 7) * 8;
+    for (int j = 0; j < 4; ++j) {
+      float v[8], y[8];
 #pragma unroll
-      for (int j = 0; j < kWords; j += 4)
-        *reinterpret_cast<uint4 *>(tile + (r * kTC + c) * EB + 4 * j) = make_uint4(w[u][j], w[u][j + 1], w[u][j + 2], w[u][j + 3]);
-      if (p.q) {
-        uint32_t byte;
-        const uint32_t codes = quant8<DT>(w[u], &byte);
-        const int64_t row = r0 + r, col = c0 + c;
-        if (row < p.rows && col < p.cols) {
-          const int nbytes = static_cast<int>(min(static_cast<int64_t>(4), (p.cols - col + 1) / 2));
-          store_codes(p.q + row * p.qs + col / 2, codes, nbytes, p.q_words);
-          if ((tid & 3) == 0) p.s[row * p.ss + col / kBlock] = static_cast<uint8_t>(byte);
-        }
+      for (int r = 0; r < 8; ++r) {
+        v[r] = __fmul_rn(x[8 * j + r].x, i0);
+        y[r] = __fmul_rn(x[8 * j + r].y, i1);
       }
+      q0[j] = pack_e2m1x8(v);
+      q1[j] = pack_e2m1x8(y);
+    }
+  } else {
+    uint32_t x[kBlock], m = 0;
+#pragma unroll
+    for (int r = 0; r < kBlock; ++r) {
+      x[r] = *reinterpret_cast<const uint32_t *>(src + r * kTC * EB);
+      m = max_u16x2(m, x[r] & 0x7fff7fffu);
+    }
+    byte[0] = scale_byte(widen_abs<DT>(m & 0xffffu));
+    byte[1] = scale_byte(widen_abs<DT>(m >> 16));
+    const float i0 = inv_scale(byte[0]), i1 = inv_scale(byte[1]);
+    const uint32_t inv2 = (__float_as_uint(i0) >> 16) | __float_as_uint(i1);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float v[8], y[8];
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        float f[2];
+        if constexpr (DT == BSIR_BF16) {
+          FloatTraits<DT>::unpack(mul_bf16x2(x[8 * j + r], inv2), f);
+        } else {
+          FloatTraits<DT>::unpack(x[8 * j + r], f);
+          f[0] = __fmul_rn(f[0], i0);
+          f[1] = __fmul_rn(f[1], i1);
+        }
+        v[r] = f[0];
+        y[r] = f[1];
+      }
+      q0[j] = pack_e2m1x8(v);
+      q1[j] = pack_e2m1x8(y);
     }
   }
-  __syncthreads();
-  const int lane = tid & 31;
-  for (int b = tid >> 5; b < TR / kBlock; b += kColThreads / 32) {      // this warp's 32-row block; lane = a pair of columns
-    uint32_t byte[2];
-    uint4 *dst0 = reinterpret_cast<uint4 *>(codes_s + 2 * lane * kCodeRow + b * 16);
-    uint4 *dst1 = reinterpret_cast<uint4 *>(codes_s + (2 * lane + 1) * kCodeRow + b * 16);
-    uint32_t q0[4], q1[4];
-    const uint8_t *src = tile + (b * kBlock * kTC + 2 * lane) * EB;
-    if constexpr (DT == BSIR_F32) {
-      uint32_t m0 = 0, m1 = 0;
-      float2 x[kBlock];
-#pragma unroll
-      for (int r = 0; r < kBlock; ++r) {
-        x[r] = *reinterpret_cast<const float2 *>(src + r * kTC * EB);
-        m0 = max(m0, __float_as_uint(x[r].x) & 0x7fffffffu);
-        m1 = max(m1, __float_as_uint(x[r].y) & 0x7fffffffu);
-      }
-      byte[0] = scale_byte(m0);
-      byte[1] = scale_byte(m1);
-      const float i0 = inv_scale(byte[0]), i1 = inv_scale(byte[1]);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        float v[8], y[8];
-#pragma unroll
-        for (int r = 0; r < 8; ++r) {
-          v[r] = __fmul_rn(x[8 * j + r].x, i0);
-          y[r] = __fmul_rn(x[8 * j + r].y, i1);
-        }
-        q0[j] = pack_e2m1x8(v);
-        q1[j] = pack_e2m1x8(y);
-      }
-    } else {
-      uint32_t x[kBlock], m = 0;
-#pragma unroll
-      for (int r = 0; r < kBlock; ++r) {
-        x[r] = *reinterpret_cast<const uint32_t *>(src + r * kTC * EB);
-        m = max_u16x2(m, x[r] & 0x7fff7fffu);
-      }
-      byte[0] = scale_byte(widen_abs<DT>(m & 0xffffu));
-      byte[1] = scale_byte(widen_abs<DT>(m >> 16));
-      const float i0 = inv_scale(byte[0]), i1 = inv_scale(byte[1]);
-      const uint32_t inv2 = (__float_as_uint(i0) >> 16) | __float_as_uint(i1);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        float v[8], y[8];
-#pragma unroll
-        for (int r = 0; r < 8; ++r) {
-          float f[2];
-          if constexpr (DT == BSIR_BF16) {
-            FloatTraits<DT>::unpack(mul_bf16x2(x[8 * j + r], inv2), f);
-          } else {
-            FloatTraits<DT>::unpack(x[8 * j + r], f);
-            f[0] = __fmul_rn(f[0], i0);
-            f[1] = __fmul_rn(f[1], i1);
-          }
-          v[r] = f[0];
-          y[r] = f[1];
-        }
-        q0[j] = pack_e2m1x8(v);
-        q1[j] = pack_e2m1x8(y);
-      }
-    }
-    *dst0 = byte[0] == 255u ? make_uint4(0, 0, 0, 0) : make_uint4(q0[0], q0[1], q0[2], q0[3]);
-    *dst1 = byte[1] == 255u ? make_uint4(0, 0, 0, 0) : make_uint4(q1[0], q1[1], q1[2], q1[3]);
-    scale_s[2 * lane][b] = static_cast<uint8_t>(byte[0]);
-    scale_s[2 * lane + 1][b] = static_cast<uint8_t>(byte[1]);
-  }
-  __syncthreads();
-  constexpr int kPieces = TR / kBlock;                   // 16-byte pieces of a column's codes
+  *reinterpret_cast<uint4 *>(codes_s + 2 * lane * kCodeRow + b * 16) = byte[0] == 255u ? make_uint4(0, 0, 0, 0) : make_uint4(q0[0], q0[1], q0[2], q0[3]);
+  *reinterpret_cast<uint4 *>(codes_s + (2 * lane + 1) * kCodeRow + b * 16) = byte[1] == 255u ? make_uint4(0, 0, 0, 0) : make_uint4(q1[0], q1[1], q1[2], q1[3]);
+  scale_s[2 * lane][b] = static_cast<uint8_t>(byte[0]);
+  scale_s[2 * lane + 1][b] = static_cast<uint8_t>(byte[1]);
+}
+// the tile's codes and exponents down the columns, from shared memory to their rows
+__device__ __forceinline__ void store_down(const QuantParams &p, const uint8_t *codes_s, const uint8_t (*scale_s)[kColPieces], int64_t r0, int64_t c0) {
   const int64_t code_bytes = (p.rows + 1) / 2, blocks = (p.rows + kBlock - 1) / kBlock;
-  for (int i = tid; i < kTC * kPieces; i += kColThreads) {
-    const int c = i / kPieces, b = i % kPieces;
+  for (int i = threadIdx.x; i < kTC * kColPieces; i += kColThreads) {
+    const int c = i / kColPieces, b = i % kColPieces;
     const int64_t col = c0 + c, at = r0 / 2 + b * 16;
     if (col >= p.cols || at >= code_bytes) continue;
     uint8_t *dst = p.qt + col * p.qts + at;
@@ -374,6 +335,111 @@ __global__ void __launch_bounds__(kColThreads) mxfp4_cols_kernel(QuantParams p) 
     }
     if (r0 / kBlock + b < blocks) p.st[col * p.sts + r0 / kBlock + b] = scale_s[c][b];
   }
+}
+
+// Down the columns only: tiles by the copy engine, two a CTA, the next one on its way while this one is worked on (a CTA
+// that loads its tile itself, works and stores, and is then replaced, reached 0.76 of the copy rate on bf16 and 0.70 on
+// f32; this 0.83 and 0.92).  Rows and columns behind the ends arrive as zeros.  One barrier a tile: the codes' staging is
+// used in turns as well.
+template <int DT>
+__global__ void __launch_bounds__(kColThreads)
+    mxfp4_cols_tma_kernel(const __grid_constant__ CUtensorMap tmap, QuantParams p, int64_t tiles, int64_t col_tiles, int *err) {
+  constexpr int EB = 4 / FloatTraits<DT>::kPerWord, kTile = kTR * kTC * EB;
+  extern __shared__ uint8_t raw[];
+  const uint32_t base = (smem_u32(raw) + 127u) & ~127u;
+  uint8_t *tile_s = raw + (base - smem_u32(raw));
+  uint8_t *codes_s = tile_s + 2 * kTile;
+  __shared__ uint8_t scale_s[2][kTC][kColPieces];
+  __shared__ uint64_t full_s[2];
+  __shared__ int abort_s;
+  const int tid = threadIdx.x;
+  auto load = [&](int64_t t, int b) {          // by thread 0
+    const int64_t row_tile = t / col_tiles;
+    mbar_expect_tx(smem_u32(&full_s[b]), kTile);
+    tma_load_2d(base + b * kTile, &tmap, static_cast<int>((t - row_tile * col_tiles) * kTC * EB), static_cast<int>(row_tile * kTR), smem_u32(&full_s[b]));
+  };
+  if (tid == 0) {
+    mbar_init(smem_u32(&full_s[0]), 1);
+    mbar_init(smem_u32(&full_s[1]), 1);
+    abort_s = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    prefetch_tmap(&tmap);
+  }
+  pdl_launch_dependents();
+  pdl_wait();
+  __syncthreads();
+  if (tid == 0) {
+    load(blockIdx.x, 0);
+    if (blockIdx.x + gridDim.x < tiles) load(blockIdx.x + gridDim.x, 1);
+  }
+  int n = 0;
+  for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x, ++n) {
+    const int b = n & 1;
+    const bool ok = mbar_wait(smem_u32(&full_s[b]), (n >> 1) & 1, &abort_s, err);
+    const int64_t row_tile = t / col_tiles, r0 = row_tile * kTR, c0 = (t - row_tile * col_tiles) * kTC;
+    const uint8_t *tile = tile_s + b * kTile;
+    uint8_t *codes = codes_s + b * (kTC * kCodeRow);
+    quant_down<DT>(tile, codes, scale_s[b], tid >> 5);
+    if (!__syncthreads_and(ok)) {        // gave up: let the copies in flight land before the CTA leaves
+      if (tid == 0)
+        for (int s = 0; s < 2; ++s)
+          for (int i = 0; i < 200000 && !mbar_try_wait(smem_u32(&full_s[s]), ((n + ((n ^ s) & 1)) >> 1) & 1); ++i) { }
+      break;
+    }
+    if (tid == 0 && t + 2 * static_cast<int64_t>(gridDim.x) < tiles) load(t + 2 * static_cast<int64_t>(gridDim.x), b);
+    store_down(p, codes, scale_s[b], r0, c0);
+  }
+}
+
+// Both forms, or any alignment: a CTA brings its tile into shared memory itself, and makes the codes along the rows from
+// the registers on the way.  (Both forms from the copy engine's tiles were slower, 59 us to 52 on bf16 [16384, 4096]: what
+// counts there is the warps that an SM holds.)
+template <int DT, bool VEC>
+__global__ void __launch_bounds__(kColThreads) mxfp4_cols_kernel(QuantParams p) {
+  constexpr int EB = 4 / FloatTraits<DT>::kPerWord, kWords = 8 / FloatTraits<DT>::kPerWord;
+  constexpr int kPasses = kTR * (kTC / 8) / kColThreads, kAhead = DT == BSIR_F32 ? 4 : kPasses;   // loads ahead of the first use
+  constexpr int kStep = kColThreads / 8;                 // rows between a thread's vectors
+  extern __shared__ __align__(16) uint8_t tile[];        // [kTR][kTC] elements, then [kTC][kCodeRow] codes
+  uint8_t *codes_s = tile + kTR * kTC * EB;
+  __shared__ uint8_t scale_s[kTC][kColPieces];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int64_t r0 = static_cast<int64_t>(blockIdx.y) * kTR;
+  const int64_t c0 = static_cast<int64_t>(blockIdx.x) * kTC;
+  const int tid = threadIdx.x, r = tid >> 3, c = (tid & 7) * 8;
+  const int rows = static_cast<int>(min(static_cast<int64_t>(kTR), p.rows - r0));       // of the tile
+  const int nbytes = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(4), (p.cols - c0 - c + 1) / 2)));
+  uint8_t *q = p.q + (r0 + r) * p.qs + (c0 + c) / 2, *s = p.s + (r0 + r) * p.ss + (c0 + c) / kBlock;
+#pragma unroll
+  for (int u0 = 0; u0 < kPasses; u0 += kAhead) {
+    uint32_t w[kAhead][kWords];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int row = r + (u0 + u) * kStep;
+      load8<DT, VEC>(p.x, (r0 + row) * p.xs, c0 + c, row < rows ? p.cols : 0, w[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int row = r + (u0 + u) * kStep;
+#pragma unroll
+      for (int j = 0; j < kWords; j += 4)
+        *reinterpret_cast<uint4 *>(tile + (row * kTC + c) * EB + 4 * j) = make_uint4(w[u][j], w[u][j + 1], w[u][j + 2], w[u][j + 3]);
+      if (p.q) {
+        uint32_t byte;
+        const uint32_t codes = quant8<DT>(w[u], &byte);
+        if (row < rows && nbytes > 0) {
+          store_codes(q, codes, nbytes, p.q_words);
+          if ((tid & 3) == 0) *s = static_cast<uint8_t>(byte);
+        }
+        q += kStep * p.qs;
+        s += kStep * p.ss;
+      }
+    }
+  }
+  __syncthreads();
+  quant_down<DT>(tile, codes_s, scale_s, tid >> 5);
+  __syncthreads();
+  store_down(p, codes_s, scale_s, r0, c0);
 }
 
 // codes and exponents -> values: a lane takes eight codes (4 bytes in, 16 or 32 bytes out)
@@ -488,17 +554,31 @@ __global__ void __launch_bounds__(256) mxfp4_dequant_kernel(DequantParams p) {
 template <int DT, bool VEC>
 int32_t launch_quant(QuantParams p, cudaStream_t st) {
   if (p.qt) {
-    constexpr int TR = kTR;
-    constexpr size_t smem = TR * kTC * (DT == BSIR_F32 ? 4 : 2) + kTC * (TR / 2 + 16);
+    constexpr int EB = DT == BSIR_F32 ? 4 : 2;
+    const int64_t gx = ceil_div(p.cols, kTC), gy = ceil_div(p.rows, kTR);
+    // the copy engine wants 16-byte aligned rows, byte coordinates and rows in 32 bits
+    if (!p.q && aligned_to(p.x, 16) && (p.xs * EB) % 16 == 0 && p.cols * EB <= 0x7fffffff && p.rows <= 0x7fffffff) {
+      CUtensorMap map;
+      int *err = device_error_word();
+      if (!err) return fail(BSIR_ERR_WORKSPACE, "quant_mxfp4: no device error word");
+      if (make_byte_tmap2(&map, p.x, p.cols * EB, p.rows, p.xs * EB, kTC * EB, kTR)) {
+        constexpr size_t smem = 2 * (kTR * kTC * EB + kTC * kCodeRow) + 128;
+        cudaFuncSetAttribute(mxfp4_cols_tma_kernel<DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+        const int64_t sms = device_info().sm_count > 0 ? device_info().sm_count : 148, tiles = gx * gy;
+        const int64_t ctas = sms * (DT == BSIR_F32 ? 2 : 5);           // what shared memory holds
+        launch_pdl(mxfp4_cols_tma_kernel<DT>, dim3(static_cast<unsigned>(tiles < ctas ? tiles : ctas)), dim3(kColThreads), smem, st, map, p, tiles, gx, err);
+        count_launch();
+        return check_launch("quant_mxfp4");
+      }
+    }
+    constexpr size_t smem = kTR * kTC * EB + kTC * kCodeRow;
     cudaFuncSetAttribute(mxfp4_cols_kernel<DT, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-    // column tiles run fastest: the CTAs at work together read whole rows.  The grid's y axis ends at 65535: longer
-    // matrices go in strips of rows (a strip starts at a whole block).
-    const int64_t gx = ceil_div(p.cols, kTC), gy = ceil_div(p.rows, TR);
+    // The grid's y axis ends at 65535: longer matrices go in strips of rows (a strip starts at a whole block).
     for (int64_t y0 = 0; y0 < gy; y0 += 65535) {
       QuantParams s = p;
-      const int64_t r0 = y0 * TR, ny = gy - y0 < 65535 ? gy - y0 : 65535;
-      s.x = static_cast<const char *>(p.x) + r0 * p.xs * dtype_bytes(DT);
-      s.rows = p.rows - r0 < ny * TR ? p.rows - r0 : ny * TR;
+      const int64_t r0 = y0 * kTR, ny = gy - y0 < 65535 ? gy - y0 : 65535;
+      s.x = static_cast<const char *>(p.x) + r0 * p.xs * EB;
+      s.rows = p.rows - r0 < ny * kTR ? p.rows - r0 : ny * kTR;
       if (p.q) { s.q = p.q + r0 * p.qs; s.s = p.s + r0 * p.ss; }
       s.qt = p.qt + r0 / 2;
       s.st = p.st + r0 / kBlock;
