@@ -27,11 +27,14 @@
 //            tile's rows of B, so that an SM's shared memory is read and filled for B half as often;
 //   kSingle  128 rows x BN columns on one CTA, for groups that would leave much of a 256-row tile empty;
 //   kFew     operands swapped: 128 rows of B are the instruction's M side and BN rows of A its N side, so that weights
-//            are streamed for as few as 16 rows of A.  With few tiles a cluster of up to eight CTAs shares a tile's K:
-//            every CTA hands each other one that CTA's rows of its partial tile (asynchronous stores into distributed
-//            shared memory), and the parts are added in the order of the CTAs (the same bits on every run).  A cluster
-//            then has one tile only.
+//            are streamed for as few as 16 rows of A.
+// With few tiles a cluster of up to eight CTAs shares the K of a tile of kSingle or kFew, and has that tile only: each CTA
+// leaves its part in shared memory and adds its share of the rows from all of them, in their order (the same bits on every
+// run).  64 x 4096 x 14336: 11.4 us, 18.8 whole; 1 x 2048 x 8192: 6.3, 11 whole.  (Parts handed over by asynchronous
+// stores straight from tensor memory cost 0.6 to 2 us more: eight bytes each, and more instructions to fetch.)
 #include "tc_ptx.cuh"
+
+#include <atomic>
 
 namespace bsir {
 namespace {
@@ -71,7 +74,7 @@ struct MxCfg {
   static constexpr int kSfCols = 2 * (kSfN + 4);
   static constexpr int kSfBase = kAccs * BN;
   static constexpr int kSfBufs = (512 - kSfBase) / kSfCols;
-  // staging: one or two buffers of 32 rows x 128 bytes of C a warp, or the partial tiles of a cluster
+  // staging: one or two buffers of 32 rows x 128 bytes of C a warp, or a tile
   static constexpr int kEpiWarps = kAccs == 1 ? 8 : 4;               // two a lane quadrant share the columns of a lone accumulator
   static constexpr int kEpiBufs = kAccs == 1 ? 1 : 2;
   static constexpr int kThreads = 128 + 32 * kEpiWarps;
@@ -90,6 +93,7 @@ struct MxCfg {
   static constexpr int kSmem = kTableOff + kTable + 1024;
   static_assert(kCols <= 512, "tensor memory");
   static_assert(kStages >= 4 && kSmem <= 227 * 1024, "shared memory");
+  static_assert(kStages * kStage >= (MODE == kFew ? BN : kTileM) * 128 * 4, "the ring holds a partial tile");
 };
 
 // The issuing warp's instructions.  All 32 lanes execute them and the predicate of one elected lane lets them through:
@@ -174,13 +178,6 @@ __device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap
 __device__ __forceinline__ void mbar_arrive_leader(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
-// eight bytes into a CTA of the cluster, counted on a barrier there: the receiver needs no other synchronisation
-__device__ __forceinline__ void st_async(uint32_t cluster_addr, uint32_t a, uint32_t b, uint32_t cluster_bar) {
-  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.b32 [%0], {%1, %2}, [%3];" ::"r"(cluster_addr), "r"(a), "r"(b),
-               "r"(cluster_bar)
-               : "memory");
-}
-
 __device__ __forceinline__ uint32_t elect_one() {       // 1 in one lane of the (whole) warp
   uint32_t one;
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
@@ -409,6 +406,96 @@ __device__ __forceinline__ void store_rows(const MxParams &p, Writer &out, uint3
   }
 }
 
+// A tile whose K is shared by a cluster: each CTA leaves its part [rows][128] of f32 in its ring of stages (16-byte
+// pieces permuted within a row, so that neither a column of pieces nor a row meets in one bank), and after a cluster
+// barrier each reads its share of the rows that C has from all of them and adds in the order of the CTAs.
+template <int BN> __device__ __forceinline__ void store_partial(uint8_t *ring, uint32_t acc, int row) {
+#pragma unroll
+  for (int c0 = 0; c0 < BN; c0 += 32) {
+    uint32_t r[32];
+    tmem_ld32(acc + static_cast<uint32_t>(c0), r);
+    tmem_ld_wait();
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      *reinterpret_cast<uint4 *>(ring + row * (BN * 4) + (((c0 / 4 + j) ^ (row & 7)) * 16)) = make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
+  }
+}
+// the same of a tile whose operands were swapped: lane = column of C
+template <int BN> __device__ __forceinline__ void store_partial_swapped(uint8_t *ring, uint32_t acc, int col) {
+#pragma unroll
+  for (int c0 = 0; c0 < BN; c0 += 16) {
+    uint32_t r[16];
+    tmem_ld16(acc + static_cast<uint32_t>(c0), r);
+    tmem_ld_wait();
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const int row = c0 + j;
+      *reinterpret_cast<uint32_t *>(ring + row * (kTileM * 4) + (((col >> 2) ^ (row & 7)) * 16) + (col & 3) * 4) = r[j];
+    }
+  }
+}
+__device__ __forceinline__ float4 load_peer4(uint32_t cluster_addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(cluster_addr) : "memory");
+  return v;
+}
+// four neighbouring columns of C
+__device__ __forceinline__ void load_bias4(const MxParams &p, int group, int64_t col, float *bias) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) bias[i] = p.bias && col + i < p.n ? load_float(p.bias, p.bias_dtype, group * p.bias_stride + col + i) : 0.0f;
+}
+__device__ __forceinline__ void store_piece(const MxParams &p, int64_t row, int64_t col, float4 sum, const float *bias) {
+  const int64_t at = row * p.ldo + col;
+  const float f[4] = {__fadd_rn(sum.x, bias[0]), __fadd_rn(sum.y, bias[1]), __fadd_rn(sum.z, bias[2]), __fadd_rn(sum.w, bias[3])};
+  if (p.tma_out && col + 4 <= p.n) {
+    if (p.out_dtype == BSIR_F32) {
+      *reinterpret_cast<float4 *>(static_cast<float *>(p.out) + at) = make_float4(f[0], f[1], f[2], f[3]);
+    } else {
+      const uint2 w = p.out_dtype == BSIR_F16 ? make_uint2(pack_f16x2(f[0], f[1]), pack_f16x2(f[2], f[3]))
+                                              : make_uint2(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]));
+      *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.out) + at) = w;
+    }
+  } else {
+#pragma unroll 1
+    for (int i = 0; i < 4 && col + i < p.n; ++i) store_out(p, at + i, f[i]);
+  }
+}
+template <int ROWS, int THREADS, int TEAM>
+__device__ __forceinline__ void join_partials(const MxParams &p, const MxTile &t, uint32_t ring, int rank) {
+  constexpr int kPieces = 32, kShare = ROWS / TEAM, kStep = THREADS / kPieces, kRows = (kShare + kStep - 1) / kStep;   // a thread's rows
+  const int piece = threadIdx.x % kPieces, first = rank + threadIdx.x / kPieces * TEAM;      // every TEAM-th row is this CTA's
+  if (first >= ROWS) return;
+  float4 v[TEAM][kRows];
+#pragma unroll
+  for (int c = 0; c < TEAM; ++c) {                      // all of a thread's parts are on their way before the first is added
+    const uint32_t peer = map_to_cta(ring, c);
+#pragma unroll
+    for (int u = 0; u < kRows; ++u) {
+      const int row = first + u * (kStep * TEAM);
+      if (t.row0 + row < t.row_end) v[c][u] = load_peer4(peer + static_cast<uint32_t>(row * (kTileM * 4) + ((piece ^ (row & 7)) * 16)));
+    }
+  }
+  const int64_t col = t.n0 + 4 * piece;
+  float bias[4];
+  load_bias4(p, t.group, col, bias);
+#pragma unroll
+  for (int u = 0; u < kRows; ++u) {
+    const int row = first + u * (kStep * TEAM);
+    float4 sum = v[0][u];
+#pragma unroll
+    for (int c = 1; c < TEAM; ++c) {
+      sum.x += v[c][u].x;
+      sum.y += v[c][u].y;
+      sum.z += v[c][u].z;
+      sum.w += v[c][u].w;
+    }
+    if (t.row0 + row >= t.row_end) break;               // rows go up
+    store_piece(p, t.row0 + row, col, sum, bias);
+  }
+}
+
+__device__ __forceinline__ void epilogue_barrier() { asm volatile("bar.sync 1, 128;" ::: "memory"); }      // its four warps
+
 // The bounded wait for a whole warp: all lanes go on or all give up, so that none is left at a warp barrier.
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int *abort_flag, int *err) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, err)) != 0;
@@ -437,16 +524,15 @@ __global__ void __launch_bounds__(MxCfg<BN, MODE>::kThreads, 1)
   constexpr int kB3 = kB2 + Cfg::kSfStages;
   auto acc_full_bar = [&](int b) { return bars + 8u * (kB3 + b); };
   auto acc_empty_bar = [&](int b) { return bars + 8u * (kB3 + 2 + b); };
-  const uint32_t red_full = bars + 8u * (kB3 + 4);                          // the cluster's partial tiles
-  static_assert(8 * (kB3 + 5) + 16 <= 512, "barriers");
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(gen + Cfg::kBarOff + 8 * (kB3 + 5));
+  static_assert(8 * (kB3 + 4) + 16 <= 512, "barriers");
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(gen + Cfg::kBarOff + 8 * (kB3 + 4));
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
   int *tile_start = reinterpret_cast<int *>(gen + Cfg::kTableOff);         // [groups + 1]
   int *row_start = tile_start + kMaxGroups + 1;                            // [groups + 1]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  // CTAs that work on one tile: a pair (rows cut in two), a cluster that shares K, or one
-  const int team = PAIR ? 2 : SWAP ? p.split : 1;
+  // CTAs that work on one tile: a pair (rows cut in two), or those that share its K (a cluster with one tile, or one CTA)
+  const int team = PAIR ? 2 : p.split;
   const int rank = team > 1 ? static_cast<int>(cluster_rank()) : 0;
   const int first_tile = blockIdx.x / team, tile_step = gridDim.x / team;
   pdl_launch_dependents();
@@ -458,7 +544,6 @@ __global__ void __launch_bounds__(MxCfg<BN, MODE>::kThreads, 1)
     for (int b = 0; b < 2; ++b) {
       mbar_init(acc_full_bar(b), 1); mbar_init(acc_empty_bar(b), Cfg::kEpiWarps * (PAIR ? 2 : 1));
     }
-    mbar_init(red_full, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     prefetch_tmap(&tmap_m); prefetch_tmap(&tmap_n); prefetch_tmap(&tmap_sm); prefetch_tmap(&tmap_sn);
@@ -519,8 +604,8 @@ __global__ void __launch_bounds__(MxCfg<BN, MODE>::kThreads, 1)
   const int total_tiles = tile_start[p.groups];
   // this CTA's chunks of kChunk stages
   const int all_chunks = (p.k_blocks + kChunk - 1) / kChunk;
-  const int per = SWAP ? (all_chunks + team - 1) / team : all_chunks;
-  const int chunk0 = SWAP ? rank * per : 0;
+  const int per = PAIR ? all_chunks : (all_chunks + team - 1) / team;
+  const int chunk0 = PAIR ? 0 : rank * per;
   const int chunk1 = min(all_chunks, chunk0 + per);
   const int kb0 = kChunk * chunk0, kb1 = min(p.k_blocks, kChunk * chunk1);       // its stages
   int group = 0;
@@ -682,58 +767,35 @@ __global__ void __launch_bounds__(MxCfg<BN, MODE>::kThreads, 1)
         }
       };
       if constexpr (SWAP) {                           // lane = column of C, register = row
-        const int64_t col = t.n0 + quad * 32 + lane;
-        const bool col_ok = col < p.n;
-        const float bias = p.bias && col_ok ? load_float(p.bias, p.bias_dtype, t.group * p.bias_stride + col) : 0.0f;
-        if (team == 1) {
-#pragma unroll 1
-          for (int c0 = 0; c0 < BN; c0 += 16) {
-            uint32_t r[16];
-            tmem_ld16(src + static_cast<uint32_t>(c0), r);
-            tmem_ld_wait();
-            if (!col_ok) continue;
+        if (team == 1) {                              // through shared memory: rows of C leave in 8- or 16-byte pieces
+          uint8_t *tile_s = gen + Cfg::kEpiOff;
+          epilogue_barrier();                         // the tile before has left
+          store_partial_swapped<BN>(tile_s, src, quad * 32 + lane);
+          release();
+          epilogue_barrier();
+          const int64_t col = t.n0 + 4 * lane;
+          float bias[4];
+          load_bias4(p, t.group, col, bias);
+          const int rows = t.row_end - t.row0 < BN ? t.row_end - t.row0 : BN;
+          for (int r0 = warp - 2; r0 < rows; r0 += 16) {
+            float4 v[4];
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              const int64_t row = t.row0 + c0 + j;
-              if (row < t.row_end) store_out(p, row * p.ldo + col, __fadd_rn(__uint_as_float(r[j]), bias));
+            for (int u = 0; u < 4; ++u) {
+              const int row = r0 + 4 * u;             // inside the staging buffer: BN is a multiple of 16
+              v[u] = *reinterpret_cast<const float4 *>(tile_s + row * (kTileM * 4) + ((lane ^ (row & 7)) * 16));
             }
-          }
-        } else {
-          // this CTA's partial tile: row j goes to CTA j / own of the cluster, pairs of rows side by side:
-          // [from][j % own / 2][128 columns][2].  The team has this one tile (see the launch).
-          const int own = BN / team;
-          const uint32_t red = base + Cfg::kEpiOff;
-          if (threadIdx.x == 64) mbar_expect_tx(red_full, BN * kTileM * 4);
-#pragma unroll 1
-          for (int c0 = 0; c0 < BN; c0 += 16) {
-            uint32_t r[16];
-            tmem_ld16(src + static_cast<uint32_t>(c0), r);
-            tmem_ld_wait();
 #pragma unroll
-            for (int j = 0; j < 16; j += 2) {
-              const int to = (c0 + j) / own, slot = (c0 + j) - to * own;
-              st_async(map_to_cta(red + static_cast<uint32_t>(((rank * own + slot) * kTileM + 2 * (quad * 32 + lane)) * 4), to), r[j], r[j + 1],
-                       map_to_cta(red_full, to));
-            }
+            for (int u = 0; u < 4; ++u)
+              if (r0 + 4 * u < rows) store_piece(p, t.row0 + r0 + 4 * u, col, v[u], bias);
           }
-          if (!warp_wait(red_full, 0u, abort_flag, p.err)) break;
-          const float2 *part = reinterpret_cast<const float2 *>(gen + Cfg::kEpiOff) + quad * 32 + lane;
-          for (int j = 0; j < own; j += 2) {
-            float2 sum = part[j / 2 * kTileM];
-            for (int f = 1; f < team; ++f) {
-              const float2 v = part[(f * own + j) / 2 * kTileM];
-              sum.x += v.x;
-              sum.y += v.y;
-            }
-            const int64_t row = t.row0 + rank * own + j;
-            if (col_ok && row < t.row_end) store_out(p, row * p.ldo + col, __fadd_rn(sum.x, bias));
-            if (col_ok && row + 1 < t.row_end) store_out(p, (row + 1) * p.ldo + col, __fadd_rn(sum.y, bias));
-          }
+        } else {                                      // joined below
+          store_partial_swapped<BN>(gen, src, quad * 32 + lane);
         }
-        release();
       } else {
         const int row0 = t.row0 + (PAIR ? rank * kTileM : 0) + quad * 32;
-        if (row0 < t.row_end) {
+        if (MODE == kSingle && team > 1) {            // the partial tile into the ring, which is done with; joined below
+          if (row0 < t.row_end) store_partial<BN>(gen, src, quad * 32 + lane);
+        } else if (row0 < t.row_end) {
           RowWriter<Cfg::kEpiBufs> out(p, &tmap_out, t, row0, lane, stage, stage_addr, nstores);
           store_rows<kCols, Cfg::kAccs == 1>(p, out, src + static_cast<uint32_t>(c_first), t.group, t.n0 + c_first, lane, release);
         } else {
@@ -743,6 +805,19 @@ __global__ void __launch_bounds__(MxCfg<BN, MODE>::kThreads, 1)
       if (++acc == Cfg::kAccs) { acc = 0; acc_phase ^= 1u; }
     }
     if (!SWAP && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+  }
+  if constexpr (!PAIR) {
+    if (team > 1) {                       // every CTA joins its share of the tile's rows
+      __syncthreads();
+      cluster_sync_all();
+      group = 0;
+      if (first_tile < total_tiles) {
+        find_tile<kRows, kColsC>(first_tile, tile_start, row_start, group, t);
+        if (team == 2) join_partials<kRows, Cfg::kThreads, 2>(p, t, base, rank);
+        else if (team == 4) join_partials<kRows, Cfg::kThreads, 4>(p, t, base, rank);
+        else join_partials<kRows, Cfg::kThreads, 8>(p, t, base, rank);
+      }
+    }
   }
   tc_fence_before();
   __syncthreads();
@@ -760,6 +835,37 @@ struct MxOperand {
   int64_t rows, batch;
 };
 
+// How many clusters of `split` CTAs run at once on the current device (a GPC's SMs are shared out in whole clusters, and
+// which SMs it has differs from GPU to GPU).  Asked once per device.
+template <int BN, int MODE> int64_t clusters_at_once(int split) {
+  constexpr int kDevices = 64;
+  static std::atomic<int> known[kDevices][4];                     // the number + 1
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess || device >= kDevices) return 0;
+  std::atomic<int> &slot = known[device][split == 2 ? 1 : split == 4 ? 2 : 3];
+  int n = slot.load(std::memory_order_relaxed) - 1;
+  if (n < 0) {
+    using Cfg = MxCfg<BN, MODE>;
+    cudaFuncSetAttribute(mxfp4_gemm_kernel<BN, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmem);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(split));
+    cfg.blockDim = dim3(Cfg::kThreads);
+    cfg.dynamicSmemBytes = Cfg::kSmem;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = static_cast<unsigned>(split);
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&n, mxfp4_gemm_kernel<BN, MODE>, &cfg) != cudaSuccess) {
+      cudaGetLastError();
+      n = 0;
+    }
+    slot.store(n + 1, std::memory_order_relaxed);
+  }
+  return n;
+}
+
 template <int BN, int MODE>
 int32_t launch_mx(const MxOperand &a, const MxOperand &b, int64_t k, MxParams p, int split, int64_t max_tiles, cudaStream_t st) {
   using Cfg = MxCfg<BN, MODE>;
@@ -774,10 +880,10 @@ int32_t launch_mx(const MxOperand &a, const MxOperand &b, int64_t k, MxParams p,
       (MODE != kFew && p.tma_out && !make_byte_tmap(&tout, p.out, p.n * eb, p.m, p.ldo * eb, 32)))
     return fail(BSIR_ERR_STRIDE, "matmul_mxfp4: the driver refuses a tensor map of these sizes and strides");
   cudaFuncSetAttribute(mxfp4_gemm_kernel<BN, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmem);
-  const int team = MODE == kPair ? 2 : MODE == kFew ? split : 1;
+  const int team = MODE == kPair ? 2 : split;
   p.split = team;
   int64_t teams = (device_info().sm_count > 0 ? device_info().sm_count : 148) / team;
-  if (teams > max_tiles || (MODE == kFew && split > 1)) teams = max_tiles;     // a cluster that shares K has one tile
+  if (teams > max_tiles || (MODE != kPair && split > 1)) teams = max_tiles;     // a cluster that shares K has one tile
   const dim3 grid(static_cast<unsigned>(teams * team));
   if (team > 1) launch_pdl_cluster(mxfp4_gemm_kernel<BN, MODE>, grid, dim3(Cfg::kThreads), Cfg::kSmem, st, team, tm, tn, tsm, tsn, tout, p);
   else launch_pdl(mxfp4_gemm_kernel<BN, MODE>, grid, dim3(Cfg::kThreads), Cfg::kSmem, st, tm, tn, tsm, tsn, tout, p);
@@ -845,30 +951,49 @@ extern "C" int32_t bsir_matmul_mxfp4(const bsir_matmul_mxfp4_desc *d, void *stre
   if (!p.err) return fail(BSIR_ERR_WORKSPACE, "matmul_mxfp4: no device error word");
   cudaStream_t st = resolve_stream(stream);
   p.tma_out = aligned_to(d->out, 16) && (ldo * eb) % 16 == 0 && d->n * eb <= 0x7fffffff;     // its coordinates are 32-bit bytes
-  // Which form: from the rows of a group, all of them or the groups' mean (their sizes are on the device).  Measured
-  // (N x K = 4096 x 4096 | 14336 x 4096, bf16 out): up to 16 rows kFew<16> 7.0-7.6 | 9.1-9.6 us, kSingle 7.8 | 12-14;
-  // 32 rows kFew<32> 8.6 | 10.4, kSingle 8.0 | 12.2; 48 rows kFew<32> 8.7 | 13.8, kSingle 7.8 | 12.3.
-  const int64_t rows = ceil_div(d->m, groups);
+  // Which form: from the rows of a group, all of them or the groups' mean (their sizes are on the device).
+  const int64_t rows = ceil_div(d->m, groups), stages = p.k_blocks, chunks = ceil_div(stages, kChunk);
   const int64_t sms = device_info().sm_count > 0 ? device_info().sm_count : 148;
   auto tiles = [&](int64_t r, int64_t c) { return (groups > 1 ? d->m / r + groups : ceil_div(d->m, r)) * ceil_div(d->n, c); };   // at most
+  // K may be shared out over a cluster if every CTA gets a part and all clusters are at work at once (37 of four CTAs in
+  // two rounds: 13 us where one CTA a tile takes 8).
+  auto can_split = [&](auto at_once, int64_t nt, int s) { return nt * s <= sms && ceil_div(chunks, s) * (s - 1) < chunks && nt <= at_once(s); };
   if (rows <= 32) {
-    const int64_t nt = rows <= 16 ? tiles(16, kTileM) : tiles(32, kTileM);
-    // K shared out over a cluster while that does not make more CTAs than SMs and every CTA gets a part
-    // (1 row, 4096 x 4096: 7.6 us whole, 7.0 by four; 4096 x 14336: 17.6 and 11.1)
-    const int64_t chunks = ceil_div(p.k_blocks, kChunk);
+    // the more CTAs the better (1 row, N x K = 4096 x 4096: 6.7 us whole, 6.4 by two, 6.2 by four; 4096 x 14336: 15.4,
+    // 11.2, 9.6); kSingle takes 8.2 and 18 to 21 us there, and 10 to 13 us on 14336 x 4096, where this takes 8.7 to 9.9
     int split = 1;
-    while (split < 8 && nt * split * 2 <= sms && ceil_div(chunks, 2 * split) * (2 * split - 1) < chunks) split *= 2;
-    return rows <= 16 ? launch_mx<16, kFew>(a, b, d->k, p, split, nt, st) : launch_mx<32, kFew>(a, b, d->k, p, split, nt, st);
+    auto widest = [&](auto at_once, int64_t nt) {
+      for (int s = 8; s > 1 && split == 1; s /= 2)
+        if (can_split(at_once, nt, s)) split = s;
+      return nt;
+    };
+    if (rows <= 16) {
+      const int64_t nt = widest(clusters_at_once<16, kFew>, tiles(16, kTileM));
+      return launch_mx<16, kFew>(a, b, d->k, p, split, nt, st);
+    }
+    const int64_t nt = widest(clusters_at_once<32, kFew>, tiles(32, kTileM));
+    return launch_mx<32, kFew>(a, b, d->k, p, split, nt, st);
   }
-  // Rounds of tiles over the SMs x time of a tile, in units of 5 ns: a stage takes 305 ns on one CTA with 128 x 128 and
-  // 345 on a pair with 256 x 256, plus 1.3 us to drain the one accumulator (measured over 96 .. 4096 rows).  Groups leave
-  // half of a last tile empty on average.
+  // Otherwise the least of these estimates, in units of 5 ns beside what every launch takes: rounds of tiles over the SMs x
+  // (stages x a stage's time + a tile's own), plus the join of a shared K, which grows with the rows of a tile.  Measured
+  // over 33 .. 4096 rows, N x K from 1000 x 8192 to 40000 x 1024.  Groups leave half of a last tile empty on average.
   auto rounds = [&](int64_t r, int64_t c, int64_t at_once) {
-    const int64_t nt = groups > 1 ? (d->m / r + groups / 2 + 1) * ceil_div(d->n, c) : tiles(r, c);
+    const int64_t most = d->m < groups ? d->m : groups, mean = d->m / r + groups / 2 + 1;
+    const int64_t nt = groups > 1 ? (mean < most ? most : mean) * ceil_div(d->n, c) : tiles(r, c);
     return ceil_div(nt, at_once);
   };
-  const int64_t single = rounds(128, 128, sms) * 61 * p.k_blocks;
-  const int64_t pair = rounds(256, 256, sms / 2) * (69 * p.k_blocks + 260);
-  if (single <= pair) return launch_mx<128, kSingle>(a, b, d->k, p, 1, tiles(128, 128), st);
+  auto part = [&](int s) { return kChunk * ceil_div(chunks, s); };            // stages of a CTA
+  const int64_t r64 = rows < 64 ? rows : 64, r128 = rows < 128 ? rows : 128;
+  int64_t few = rounds(64, kTileM, sms) * (50 * stages + 5 * (r64 - 24)), single = rounds(kTileM, 128, sms) * 61 * stages;
+  int few_split = 1, single_split = 1;
+  for (int s = 2; s <= 8; s *= 2) {
+    const int64_t f = s == 2 ? 51 * part(s) + 180 + 23 * r64 / 10 : 58 * part(s) + (s == 4 ? 370 : 470) + 24 * r64 / 10;
+    if (f < few && can_split(clusters_at_once<64, kFew>, tiles(64, kTileM), s)) { few = f; few_split = s; }
+    const int64_t g = s == 2 ? 57 * part(s) + 240 + 26 * r128 / 10 : 63 * part(s) + (s == 4 ? 350 : 450) + 41 * r128 / 10;
+    if (g < single && can_split(clusters_at_once<128, kSingle>, tiles(kTileM, 128), s)) { single = g; single_split = s; }
+  }
+  const int64_t pair = rounds(256, 256, sms / 2) * (69 * stages + 260);
+  if (few < single && few < pair) return launch_mx<64, kFew>(a, b, d->k, p, few_split, tiles(64, kTileM), st);
+  if (single <= pair) return launch_mx<128, kSingle>(a, b, d->k, p, single_split, tiles(128, 128), st);
   return launch_mx<256, kPair>(a, b, d->k, p, 1, tiles(256, 256), st);
 }

@@ -275,6 +275,47 @@ def test_linear_backward_and_gradient_by_differences(B):
         assert (vals[0] - vals[1]) / 2 == grad[r, c]
 
 
+# few tiles and a long K: a cluster shares a tile's K, in tiles of 16, 32, 64 and 128 rows
+SHARED_K = [(1, 1920, 8192), (9, 130, 9000), (16, 2048, 8192), (31, 2100, 2500), (33, 300, 8192), (64, 1000, 4100), (100, 1000, 8192),
+            (120, 4096, 5000), (200, 3900, 14000), (256, 700, 8100)]
+
+
+@pytest.mark.parametrize("m,n,k", SHARED_K)
+def test_product_with_shared_k(B, m, n, k):
+    """Sums of multiples of 1/4 under 2^20: f32 holds them in any order, so results are exact."""
+    a, sa = R.random_codes(m, k, seed=m + n, lo=127, hi=127)
+    b, sb = R.random_codes(n, k, seed=k, lo=127, hi=127)
+    bias = torch.randint(-8, 9, (n,), generator=torch.Generator().manual_seed(2)).float().cuda()
+    ref = R.decode(a, sa, k) @ R.decode(b, sb, k).T
+    wide = torch.full((m + 1, n + 3), -7.0, device="cuda")       # rows that vector stores cannot take
+    B.matmul_mxfp4(a, sa, b, sb, bias=bias, out=wide[:m, 1:n + 1])
+    assert np.array_equal(wide[:m, 1:n + 1].cpu().double().numpy(), ref + bias.cpu().double().numpy())
+    assert (wide[m] == -7).all() and (wide[:, 0] == -7).all() and (wide[:, n + 1:] == -7).all()
+    for dtype in (torch.float32, torch.bfloat16, torch.float16):
+        got = B.matmul_mxfp4(a, sa, b, sb, out_dtype=dtype)
+        assert torch.equal(got.cpu(), torch.from_numpy(ref).float().to(dtype)), dtype
+    assert B.device_error() == 0
+
+
+@pytest.mark.parametrize("sizes,n,k", [([3, 0, 20], 260, 8192), ([40, 0, 33, 64], 200, 8192), ([130, 0, 100], 390, 6000), ([0, 90], 100, 4096),
+                                       ([20, 1, 70], 250, 5000)])
+def test_grouped_product_with_shared_k(B, sizes, n, k):
+    m, e = sum(sizes) + 2, len(sizes)
+    a, sa = R.random_codes(m, k, seed=m, lo=127, hi=127)
+    b, sb = R.random_codes(e * n, k, seed=n, lo=127, hi=127)
+    b3 = b.as_strided((e, n, b.shape[1]), (n * b.stride(0), b.stride(0), 1))
+    sb3 = sb.as_strided((e, n, sb.shape[1]), (n * sb.stride(0), sb.stride(0), 1))
+    offs = np.concatenate(([1], 1 + np.cumsum(sizes))).astype(np.int32)
+    bias = torch.randint(-8, 9, (e, n), generator=torch.Generator().manual_seed(2)).float().cuda()
+    out = torch.full((m, n), 123.0, device="cuda")
+    B.matmul_mxfp4(a, sa, b3, sb3, offsets=torch.from_numpy(offs).cuda(), bias=bias, out=out)
+    av, bv = R.decode(a, sa, k), R.decode(b, sb, k).reshape(e, n, k)
+    ref = np.full((m, n), 123.0)
+    for g in range(e):
+        ref[offs[g]:offs[g + 1]] = av[offs[g]:offs[g + 1]] @ bv[g].T + bias[g].cpu().double().numpy()
+    assert np.array_equal(out.cpu().double().numpy(), ref)
+
+
 @pytest.mark.parametrize("m", [20, 60, 300])
 def test_product_into_rows_far_apart(B, m):
     """Rows of C 2^26 elements apart: their offsets pass 2^31."""
