@@ -86,9 +86,9 @@ __device__ __forceinline__ int cta_prefix(int v, int *warp_sum_s, int *total) {
   return inc - v + (warp ? warp_sum_s[warp - 1] : 0);
 }
 
-__device__ __forceinline__ void cluster_barrier() {
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+__device__ __forceinline__ void cluster_barrier() {            // warps may come to it in parts
+  asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
 }
 __device__ __forceinline__ int load_peer(const int *own, int cta) {       // the same shared-memory word in another CTA
   uint32_t addr = static_cast<uint32_t>(__cvta_generic_to_shared(own)), peer;
@@ -363,9 +363,9 @@ __global__ void __launch_bounds__(kMoveThreads) expert_combine_kernel(RowParams 
   }
 }
 
-// One CTA per token, four choices at a time (eight at a time, or dout kept for eight: 120 registers and 267 us, 194 us,
-// where this takes 180 on 64k rows of 4096 bf16): y's rows are
-// read once, dy's written once, dout's once for the four; the dot products meet across the warps in a fixed order.
+// One CTA per token, four choices at a time: y's rows are read once, dy's written once, dout's once for the four; the dot
+// products meet across the warps in a fixed order.  (64k rows of 4096 bf16: 180 us; eight choices at a time 267, dout kept
+// in registers for eight 194.)
 constexpr int kGradThreads = 128;
 constexpr int kGradChoices = 4;
 template <int DT, bool VEC>

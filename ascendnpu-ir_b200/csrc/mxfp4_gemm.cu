@@ -951,8 +951,10 @@ extern "C" int32_t bsir_matmul_mxfp4(const bsir_matmul_mxfp4_desc *d, void *stre
   if (!p.err) return fail(BSIR_ERR_WORKSPACE, "matmul_mxfp4: no device error word");
   cudaStream_t st = resolve_stream(stream);
   p.tma_out = aligned_to(d->out, 16) && (ldo * eb) % 16 == 0 && d->n * eb <= 0x7fffffff;     // its coordinates are 32-bit bytes
-  // Which form: from the rows of a group, all of them or the groups' mean (their sizes are on the device).
-  const int64_t rows = ceil_div(d->m, groups), stages = p.k_blocks, chunks = ceil_div(stages, kChunk);
+  // Which form: from the rows of a group, all of them or one and a half times the groups' mean, which most groups stay
+  // under (their sizes are on the device; a group that needs a second tile reads its weights twice.  128 groups of 16 rows
+  // on average, 4096 x 1536: 90 us in tiles of 16, 74 in tiles of 32; of 32 rows: 93 in tiles of 32, 78 in tiles of 64).
+  const int64_t rows = groups > 1 ? ceil_div(3 * d->m, 2 * groups) : d->m, stages = p.k_blocks, chunks = ceil_div(stages, kChunk);
   const int64_t sms = device_info().sm_count > 0 ? device_info().sm_count : 148;
   auto tiles = [&](int64_t r, int64_t c) { return (groups > 1 ? d->m / r + groups : ceil_div(d->m, r)) * ceil_div(d->n, c); };   // at most
   // K may be shared out over a cluster if every CTA gets a part and all clusters are at work at once (37 of four CTAs in
@@ -976,15 +978,17 @@ extern "C" int32_t bsir_matmul_mxfp4(const bsir_matmul_mxfp4_desc *d, void *stre
   }
   // Otherwise the least of these estimates, in units of 5 ns beside what every launch takes: rounds of tiles over the SMs x
   // (stages x a stage's time + a tile's own), plus the join of a shared K, which grows with the rows of a tile.  Measured
-  // over 33 .. 4096 rows, N x K from 1000 x 8192 to 40000 x 1024.  Groups leave half of a last tile empty on average.
-  auto rounds = [&](int64_t r, int64_t c, int64_t at_once) {
-    const int64_t most = d->m < groups ? d->m : groups, mean = d->m / r + groups / 2 + 1;
-    const int64_t nt = groups > 1 ? (mean < most ? most : mean) * ceil_div(d->n, c) : tiles(r, c);
-    return ceil_div(nt, at_once);
+  // over 33 .. 4096 rows, N x K from 1000 x 8192 to 40000 x 1024.  Groups leave half of a last tile empty on average, and
+  // their last round is half full.
+  auto cost = [&](int64_t r, int64_t c, int64_t at_once, int64_t tile) {
+    if (groups == 1) return ceil_div(tiles(r, c), at_once) * tile;
+    const int64_t most = d->m < groups ? d->m : groups, mean = d->m / r + groups / 2 + 1;     // every group has a tile
+    return (mean < most ? most : mean) * ceil_div(d->n, c) * tile / at_once + tile / 2;
   };
   auto part = [&](int s) { return kChunk * ceil_div(chunks, s); };            // stages of a CTA
   const int64_t r64 = rows < 64 ? rows : 64, r128 = rows < 128 ? rows : 128;
-  int64_t few = rounds(64, kTileM, sms) * (50 * stages + 5 * (r64 - 24)), single = rounds(kTileM, 128, sms) * 61 * stages;
+  const int64_t tail = groups > 1 ? 128 : 0;              // rows next to another group's are stored by the warps
+  int64_t few = cost(64, kTileM, sms, 50 * stages + 5 * (r64 - 24)), single = cost(kTileM, 128, sms, 61 * stages + tail);
   int few_split = 1, single_split = 1;
   for (int s = 2; s <= 8; s *= 2) {
     const int64_t f = s == 2 ? 51 * part(s) + 180 + 23 * r64 / 10 : 58 * part(s) + (s == 4 ? 370 : 470) + 24 * r64 / 10;
@@ -992,7 +996,7 @@ extern "C" int32_t bsir_matmul_mxfp4(const bsir_matmul_mxfp4_desc *d, void *stre
     const int64_t g = s == 2 ? 57 * part(s) + 240 + 26 * r128 / 10 : 63 * part(s) + (s == 4 ? 350 : 450) + 41 * r128 / 10;
     if (g < single && can_split(clusters_at_once<128, kSingle>, tiles(kTileM, 128), s)) { single = g; single_split = s; }
   }
-  const int64_t pair = rounds(256, 256, sms / 2) * (69 * stages + 260);
+  const int64_t pair = cost(256, 256, sms / 2, 69 * stages + 260 + tail);
   if (few < single && few < pair) return launch_mx<64, kFew>(a, b, d->k, p, few_split, tiles(64, kTileM), st);
   if (single <= pair) return launch_mx<128, kSingle>(a, b, d->k, p, single_split, tiles(128, 128), st);
   return launch_mx<256, kPair>(a, b, d->k, p, 1, tiles(256, 256), st);
