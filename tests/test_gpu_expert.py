@@ -293,3 +293,26 @@ def test_two_streams_at_once(B):
         torch.cuda.synchronize()
         for (o, s), (wo, ws) in zip(got, want):
             assert np.array_equal(o.cpu().numpy(), wo) and np.array_equal(s.cpu().numpy(), ws)
+
+
+@pytest.mark.parametrize("k", [96, 2900])
+def test_dispatched_codes_go_into_a_product(B, k):
+    """Rows of codes and exponents whose length is no multiple of 16 bytes, through dispatch's own result."""
+    g = torch.Generator(device="cuda").manual_seed(k)
+    x = torch.randn(40, k, device="cuda", generator=g)
+    w = torch.randn(4 * 70, k, device="cuda", generator=g)
+    ids = torch.randint(0, 4, (40, 2), device="cuda", generator=g)
+    off, slots = B.expert_sort(ids, 4)
+    q, s = B.quant_mxfp4(x)
+    qw, sw = B.quant_mxfp4(w)
+    qr, sr = B.expert_dispatch(q, slots), B.expert_dispatch(s, slots)
+    cut = lambda t: t.as_strided((4, 70, t.shape[1]), (70 * t.stride(0), t.stride(0), 1))
+    y = B.matmul_mxfp4(qr, sr, cut(qw), cut(sw), offsets=off, out_dtype=torch.float32)
+    full = B.matmul_mxfp4(q, s, qw, sw, out_dtype=torch.float32)          # every token with every expert: the same sums up to order
+    for t in range(40):
+        for j in range(2):
+            e = int(ids[t, j])
+            ref = full[t, 70 * e:70 * e + 70].double()
+            # sums of k products in f32, each order off by at most k / 2 ulps of the sum of magnitudes
+            mags = B.dequant_mxfp4(q[t:t + 1], s[t:t + 1]).abs().double() @ B.dequant_mxfp4(qw, sw).abs().double()[70 * e:70 * e + 70].T
+            assert ((y[int(slots[t, j])].double() - ref).abs() <= 2 * k * 2.0 ** -24 * mags[0]).all()
