@@ -158,7 +158,8 @@ bool make_byte_tmap(CUtensorMap *map, const void *ptr, uint64_t inner, uint64_t 
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-bool make_byte_tmap2(CUtensorMap *map, const void *ptr, uint64_t inner, uint64_t outer, uint64_t pitch, uint32_t box_inner, uint32_t box_rows) {
+bool make_byte_tmap2(CUtensorMap *map, const void *ptr, uint64_t inner, uint64_t outer, uint64_t pitch, uint32_t box_inner, uint32_t box_rows,
+                     bool swizzle) {
   EncodeFn enc = tmap_encoder();
   if (!enc) return false;
   cuuint64_t dims[2] = {inner, outer};
@@ -166,7 +167,7 @@ bool make_byte_tmap2(CUtensorMap *map, const void *ptr, uint64_t inner, uint64_t
   cuuint32_t box[2] = {box_inner, box_rows};
   cuuint32_t estr[2] = {1u, 1u};
   return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-             CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+             swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 bool make_byte_tmap3(CUtensorMap *map, const void *ptr, uint64_t inner, uint64_t outer, uint64_t batch, uint64_t pitch, uint64_t batch_stride,

@@ -74,12 +74,13 @@ __device__ __forceinline__ void unpack_e2m1x8(uint32_t q, float *v) {
   }
 }
 
-// Two 16-bit floats at once.  Magnitudes compare like unsigned numbers, so the largest one of a block is found on packed
-// bits; a bf16 times a power of two is exact, so pairs are scaled before they are widened (the power and its product
+// Two 16-bit floats at once: the larger magnitude with some sign (a NaN stays one), one instruction where clearing the
+// signs and comparing bits is two.  A bf16 times a power of two is exact, so pairs are scaled before they are widened (the power and its product
 // with anything that does not round to zero are bf16 numbers; f16's exponent range is too short for that).
-__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+template <int DT> __device__ __forceinline__ uint32_t max_abs2(uint32_t a, uint32_t b) {
   uint32_t r;
-  asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  if constexpr (DT == BSIR_BF16) asm("max.NaN.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  else asm("max.NaN.xorsign.abs.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
 __device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
@@ -104,10 +105,10 @@ __device__ __forceinline__ uint32_t quant8(const uint32_t *w, uint32_t *byte_out
     m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
     m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
   } else {
-    uint32_t h = max_u16x2(max_u16x2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu), max_u16x2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
-    h = max_u16x2(h, __shfl_xor_sync(0xffffffffu, h, 1));
-    h = max_u16x2(h, __shfl_xor_sync(0xffffffffu, h, 2));
-    m = widen_abs<DT>(max(h & 0xffffu, h >> 16));
+    uint32_t h = max_abs2<DT>(max_abs2<DT>(w[0], w[1]), max_abs2<DT>(w[2], w[3]));
+    h = max_abs2<DT>(h, __shfl_xor_sync(0xffffffffu, h, 1));
+    h = max_abs2<DT>(h, __shfl_xor_sync(0xffffffffu, h, 2));
+    m = widen_abs<DT>(max(h & 0x7fffu, h >> 16 & 0x7fffu));
   }
   const uint32_t byte = scale_byte(m);
   const float inv = inv_scale(byte);
@@ -243,8 +244,7 @@ __global__ void __launch_bounds__(256) mxfp4_rows_kernel(QuantParams p) {
 }
 
 // Blocks down the columns, and along the rows as well when `q` is wanted, on tiles of kTR rows x 64 columns in shared
-// memory (128 bytes of a row of a 16-bit type).  Along the rows a thread takes 16 bytes, as above; down the columns it
-// takes two neighbouring columns of a 32-row block -- a warp reads one row of the tile at a time -- and its two blocks'
+// memory (128 bytes of a row of a 16-bit type).  Down the columns a thread takes two neighbouring columns of a 32-row block -- a warp reads one row of the tile at a time -- and its two blocks'
 // codes (16 bytes each) go through shared memory so that a column's codes leave as kTR / 2 consecutive bytes.
 constexpr int kTC = 64;
 constexpr int kTR = 128;
@@ -252,8 +252,44 @@ constexpr int kColThreads = 128;
 constexpr int kCodeRow = kTR / 2 + 16;                   // bytes of a column's codes, padded against bank conflicts
 constexpr int kColPieces = kTR / kBlock;                 // 16-byte pieces (blocks) of a column of a tile
 
-// this warp's 32-row block b of the tile, lane = a pair of columns -> codes and exponents down the columns
+// half of a swizzled row of a tile of 16-bit floats (`row8`: the row modulo 8): one block along the row
 template <int DT>
+__device__ __forceinline__ uint4 quant_block(const uint8_t *row, int half, int row8, uint32_t *byte_out) {
+  uint32_t w[16];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint4 v = *reinterpret_cast<const uint4 *>(row + (((4 * half + j) ^ row8) * 16));
+    w[4 * j] = v.x; w[4 * j + 1] = v.y; w[4 * j + 2] = v.z; w[4 * j + 3] = v.w;
+  }
+  uint32_t h = w[0];
+#pragma unroll
+  for (int i = 1; i < 16; ++i) h = max_abs2<DT>(h, w[i]);
+  const uint32_t byte = scale_byte(widen_abs<DT>(max(h & 0x7fffu, h >> 16 & 0x7fffu)));
+  const float inv = inv_scale(byte);
+  const uint32_t inv2 = __float_as_uint(inv) | (__float_as_uint(inv) >> 16);
+  uint32_t q[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (DT == BSIR_BF16) {
+        FloatTraits<DT>::unpack(mul_bf16x2(w[4 * j + i], inv2), v + 2 * i);
+      } else {
+        FloatTraits<DT>::unpack(w[4 * j + i], v + 2 * i);
+        v[2 * i] = __fmul_rn(v[2 * i], inv);
+        v[2 * i + 1] = __fmul_rn(v[2 * i + 1], inv);
+      }
+    }
+    q[j] = pack_e2m1x8(v);
+  }
+  *byte_out = byte;
+  return byte == 255u ? make_uint4(0, 0, 0, 0) : make_uint4(q[0], q[1], q[2], q[3]);
+}
+
+// this warp's 32-row block b of the tile, lane = a pair of columns -> codes and exponents down the columns
+// (SWZ: 16-byte pieces of a row of the tile permuted by the row, as the copy engine's 128-byte swizzle leaves them)
+template <int DT, bool SWZ = false>
 __device__ __forceinline__ void quant_down(const uint8_t *tile, uint8_t *codes_s, uint8_t (*scale_s)[kColPieces], int b) {
   constexpr int EB = 4 / FloatTraits<DT>::kPerWord;
   const int lane = threadIdx.x & 31;
@@ -287,11 +323,11 @@ __device__ __forceinline__ void quant_down(const uint8_t *tile, uint8_t *codes_s
     uint32_t x[kBlock], m = 0;
 #pragma unroll
     for (int r = 0; r < kBlock; ++r) {
-      x[r] = *reinterpret_cast<const uint32_t *>(src + r * kTC * EB);
-      m = max_u16x2(m, x[r] & 0x7fff7fffu);
+      x[r] = *reinterpret_cast<const uint32_t *>(SWZ ? tile + (b * kBlock + r) * kTC * EB + ((4 * lane) ^ ((r & 7) * 16)) : src + r * kTC * EB);
+      m = max_abs2<DT>(m, x[r]);
     }
-    byte[0] = scale_byte(widen_abs<DT>(m & 0xffffu));
-    byte[1] = scale_byte(widen_abs<DT>(m >> 16));
+    byte[0] = scale_byte(widen_abs<DT>(m & 0x7fffu));
+    byte[1] = scale_byte(widen_abs<DT>(m >> 16 & 0x7fffu));
     const float i0 = inv_scale(byte[0]), i1 = inv_scale(byte[1]);
     const uint32_t inv2 = (__float_as_uint(i0) >> 16) | __float_as_uint(i1);
 #pragma unroll
@@ -337,21 +373,27 @@ __device__ __forceinline__ void store_down(const QuantParams &p, const uint8_t *
   }
 }
 
-// Down the columns only: tiles by the copy engine, two a CTA, the next one on its way while this one is worked on (a CTA
-// that loads its tile itself, works and stores, and is then replaced, reached 0.76 of the copy rate on bf16 and 0.70 on
-// f32; this 0.83 and 0.92).  Rows and columns behind the ends arrive as zeros.  One barrier a tile: the codes' staging is
-// used in turns as well.
-template <int DT>
-__global__ void __launch_bounds__(kColThreads)
+// Tiles by the copy engine, two a CTA, the next one on its way while this one is worked on (a CTA that loads its tile
+// itself, works and stores, and is then replaced, reached 0.76 of the copy rate on bf16 and 0.70 on f32 down the columns;
+// this 0.85 and 0.93).  Rows and columns behind the ends arrive as zeros.  One barrier a tile: the codes' staging is used
+// in turns as well.  BOTH: four more warps make the blocks along the rows of the same tile.  Instructions bound that
+// (eight elements a lane and two shuffles a block, as in the kernel above: 55 us on bf16 [16384, 4096]), so on 16-bit types
+// a thread takes a whole block, 64 bytes of a row, which the 128-byte swizzle spreads over the banks: 40.5 us, 0.78 of the
+// copy rate; f32, with eight elements a lane, 64.5, 0.80.
+template <int DT, bool BOTH>
+__global__ void __launch_bounds__(BOTH ? 2 * kColThreads : kColThreads, BOTH ? (DT == BSIR_F32 ? 3 : 4) : 1)
     mxfp4_cols_tma_kernel(const __grid_constant__ CUtensorMap tmap, QuantParams p, int64_t tiles, int64_t col_tiles, int *err) {
-  constexpr int EB = 4 / FloatTraits<DT>::kPerWord, kTile = kTR * kTC * EB;
+  constexpr int EB = 4 / FloatTraits<DT>::kPerWord, kWords = 8 / FloatTraits<DT>::kPerWord, kTile = kTR * kTC * EB;
   extern __shared__ uint8_t raw[];
-  const uint32_t base = (smem_u32(raw) + 127u) & ~127u;
-  uint8_t *tile_s = raw + (base - smem_u32(raw));
-  uint8_t *codes_s = tile_s + 2 * kTile;
   __shared__ uint8_t scale_s[2][kTC][kColPieces];
   __shared__ uint64_t full_s[2];
   __shared__ int abort_s;
+  constexpr bool kSwz = BOTH && DT != BSIR_F32;
+  constexpr uint32_t kAlign = kSwz ? 1024 : 128;
+  const uint32_t base = (smem_u32(raw) + kAlign - 1) & ~(kAlign - 1);
+  uint8_t *tile_s = raw + (base - smem_u32(raw));
+  uint8_t *codes_s = tile_s + 2 * kTile;
+  const bool q_vec = BOTH && ((reinterpret_cast<uintptr_t>(p.q) | static_cast<uintptr_t>(p.qs)) & 15) == 0;
   const int tid = threadIdx.x;
   auto load = [&](int64_t t, int b) {          // by thread 0
     const int64_t row_tile = t / col_tiles;
@@ -379,7 +421,56 @@ __global__ void __launch_bounds__(kColThreads)
     const int64_t row_tile = t / col_tiles, r0 = row_tile * kTR, c0 = (t - row_tile * col_tiles) * kTC;
     const uint8_t *tile = tile_s + b * kTile;
     uint8_t *codes = codes_s + b * (kTC * kCodeRow);
-    quant_down<DT>(tile, codes, scale_s[b], tid >> 5);
+    if (!BOTH || tid < kColThreads) {
+      quant_down<DT, kSwz>(tile, codes, scale_s[b], tid >> 5);
+    } else if constexpr (kSwz) {
+      // a block a thread, two of them: nothing to pass between lanes, and one exponent's arithmetic for 32 elements
+      const int rows = static_cast<int>(min(static_cast<int64_t>(kTR), p.rows - r0));       // of the tile
+      const int half = tid & 1;
+      const int64_t col = c0 + half * kBlock, left = (p.cols - col + 1) / 2;
+      const int nbytes = left < 0 ? 0 : left < 16 ? static_cast<int>(left) : 16;
+#pragma unroll 1
+      for (int row = (tid - kColThreads) >> 1; row < kTR; row += kColThreads / 2) {
+        uint32_t byte;
+        const uint4 q16 = quant_block<DT>(tile + row * kTC * EB, half, row & 7, &byte);
+        if (row >= rows || nbytes <= 0) continue;
+        uint8_t *q = p.q + (r0 + row) * p.qs + col / 2;
+        if (q_vec && nbytes == 16) {
+          *reinterpret_cast<uint4 *>(q) = q16;
+        } else {
+          const uint32_t w[4] = {q16.x, q16.y, q16.z, q16.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) store_codes(q + 4 * j, w[j], nbytes - 4 * j, p.q_words);
+        }
+        p.s[(r0 + row) * p.ss + col / kBlock] = static_cast<uint8_t>(byte);
+      }
+    } else {
+      const int r = (tid - kColThreads) >> 3, c = (tid & 7) * 8;
+      const int rows = static_cast<int>(min(static_cast<int64_t>(kTR), p.rows - r0));       // of the tile
+      const int nbytes = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(4), (p.cols - c0 - c + 1) / 2)));
+      uint8_t *q = p.q + (r0 + r) * p.qs + (c0 + c) / 2, *s = p.s + (r0 + r) * p.ss + (c0 + c) / kBlock;
+      const bool whole = rows == kTR && c0 + kTC <= p.cols && p.q_words;
+#pragma unroll
+      for (int u = 0; u < kTR * 8 / kColThreads; ++u) {
+        const int row = r + u * (kColThreads / 8);
+        uint32_t w[kWords], byte;
+#pragma unroll
+        for (int j = 0; j < kWords; j += 4) {
+          const uint4 v = *reinterpret_cast<const uint4 *>(tile + (row * kTC + c) * EB + 4 * j);
+          w[j] = v.x; w[j + 1] = v.y; w[j + 2] = v.z; w[j + 3] = v.w;
+        }
+        const uint32_t q8 = quant8<DT>(w, &byte);
+        if (whole) {
+          *reinterpret_cast<uint32_t *>(q) = q8;
+          if ((tid & 3) == 0) *s = static_cast<uint8_t>(byte);
+        } else if (row < rows && nbytes > 0) {
+          store_codes(q, q8, nbytes, p.q_words);
+          if ((tid & 3) == 0) *s = static_cast<uint8_t>(byte);
+        }
+        q += (kColThreads / 8) * p.qs;
+        s += (kColThreads / 8) * p.ss;
+      }
+    }
     if (!__syncthreads_and(ok)) {        // gave up: let the copies in flight land before the CTA leaves
       if (tid == 0)
         for (int s = 0; s < 2; ++s)
@@ -387,14 +478,13 @@ __global__ void __launch_bounds__(kColThreads)
       break;
     }
     if (tid == 0 && t + 2 * static_cast<int64_t>(gridDim.x) < tiles) load(t + 2 * static_cast<int64_t>(gridDim.x), b);
-    store_down(p, codes, scale_s[b], r0, c0);
+    if (!BOTH || tid < kColThreads) store_down(p, codes, scale_s[b], r0, c0);
   }
 }
 
-// Both forms, or any alignment: a CTA brings its tile into shared memory itself, and makes the codes along the rows from
-// the registers on the way.  (Both forms from the copy engine's tiles were slower, 59 us to 52 on bf16 [16384, 4096]: what
-// counts there is the warps that an SM holds.)
-template <int DT, bool VEC>
+// Rows of any alignment: a CTA brings its tile into shared memory itself, and makes the codes along the rows from the
+// registers on the way.
+template <int DT>
 __global__ void __launch_bounds__(kColThreads) mxfp4_cols_kernel(QuantParams p) {
   constexpr int EB = 4 / FloatTraits<DT>::kPerWord, kWords = 8 / FloatTraits<DT>::kPerWord;
   constexpr int kPasses = kTR * (kTC / 8) / kColThreads, kAhead = DT == BSIR_F32 ? 4 : kPasses;   // loads ahead of the first use
@@ -416,7 +506,7 @@ __global__ void __launch_bounds__(kColThreads) mxfp4_cols_kernel(QuantParams p) 
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       const int row = r + (u0 + u) * kStep;
-      load8<DT, VEC>(p.x, (r0 + row) * p.xs, c0 + c, row < rows ? p.cols : 0, w[u]);
+      load8<DT, false>(p.x, (r0 + row) * p.xs, c0 + c, row < rows ? p.cols : 0, w[u]);
     }
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
@@ -557,22 +647,23 @@ int32_t launch_quant(QuantParams p, cudaStream_t st) {
     constexpr int EB = DT == BSIR_F32 ? 4 : 2;
     const int64_t gx = ceil_div(p.cols, kTC), gy = ceil_div(p.rows, kTR);
     // the copy engine wants 16-byte aligned rows, byte coordinates and rows in 32 bits
-    if (!p.q && aligned_to(p.x, 16) && (p.xs * EB) % 16 == 0 && p.cols * EB <= 0x7fffffff && p.rows <= 0x7fffffff) {
+    if (aligned_to(p.x, 16) && (p.xs * EB) % 16 == 0 && p.cols * EB <= 0x7fffffff && p.rows <= 0x7fffffff) {
       CUtensorMap map;
       int *err = device_error_word();
       if (!err) return fail(BSIR_ERR_WORKSPACE, "quant_mxfp4: no device error word");
-      if (make_byte_tmap2(&map, p.x, p.cols * EB, p.rows, p.xs * EB, kTC * EB, kTR)) {
-        constexpr size_t smem = 2 * (kTR * kTC * EB + kTC * kCodeRow) + 128;
-        cudaFuncSetAttribute(mxfp4_cols_tma_kernel<DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+      if (make_byte_tmap2(&map, p.x, p.cols * EB, p.rows, p.xs * EB, kTC * EB, kTR, p.q && DT != BSIR_F32)) {
+        constexpr size_t smem = 2 * (kTR * kTC * EB + kTC * kCodeRow) + (EB == 2 ? 1024 : 128);
+        const auto kernel = p.q ? mxfp4_cols_tma_kernel<DT, true> : mxfp4_cols_tma_kernel<DT, false>;
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
         const int64_t sms = device_info().sm_count > 0 ? device_info().sm_count : 148, tiles = gx * gy;
-        const int64_t ctas = sms * (DT == BSIR_F32 ? 2 : 5);           // what shared memory holds
-        launch_pdl(mxfp4_cols_tma_kernel<DT>, dim3(static_cast<unsigned>(tiles < ctas ? tiles : ctas)), dim3(kColThreads), smem, st, map, p, tiles, gx, err);
+        const int64_t ctas = sms * (DT == BSIR_F32 ? (p.q ? 3 : 2) : p.q ? 4 : 5);           // what shared memory holds
+        launch_pdl(kernel, dim3(static_cast<unsigned>(tiles < ctas ? tiles : ctas)), dim3(p.q ? 2 * kColThreads : kColThreads), smem, st, map, p, tiles, gx, err);
         count_launch();
         return check_launch("quant_mxfp4");
       }
     }
     constexpr size_t smem = kTR * kTC * EB + kTC * kCodeRow;
-    cudaFuncSetAttribute(mxfp4_cols_kernel<DT, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    cudaFuncSetAttribute(mxfp4_cols_kernel<DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     // The grid's y axis ends at 65535: longer matrices go in strips of rows (a strip starts at a whole block).
     for (int64_t y0 = 0; y0 < gy; y0 += 65535) {
       QuantParams s = p;
@@ -582,7 +673,7 @@ int32_t launch_quant(QuantParams p, cudaStream_t st) {
       if (p.q) { s.q = p.q + r0 * p.qs; s.s = p.s + r0 * p.ss; }
       s.qt = p.qt + r0 / 2;
       s.st = p.st + r0 / kBlock;
-      launch_pdl(mxfp4_cols_kernel<DT, VEC>, dim3(static_cast<unsigned>(gx), static_cast<unsigned>(ny)), dim3(kColThreads), smem, st, s);
+      launch_pdl(mxfp4_cols_kernel<DT>, dim3(static_cast<unsigned>(gx), static_cast<unsigned>(ny)), dim3(kColThreads), smem, st, s);
       count_launch();
     }
     return check_launch("quant_mxfp4");

@@ -136,6 +136,25 @@ def test_quant_strides_and_alignment(B, offset, pitch):
     assert np.array_equal(R.decode(qt, st, rows), R.quant(x.t())[2], equal_nan=True)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rows,cols,odd", [(130, 69, 1), (128, 64, 0), (128, 64, 4), (97, 129, 0), (300, 200, 2), (1, 8, 0), (257, 33, 16)])
+def test_quant_both_from_aligned_rows(B, rows, cols, odd, dtype):
+    """Source rows start 16-byte aligned, results wherever the caller has them."""
+    x = torch.full((rows, (cols + 15) // 16 * 16), 1e4, device="cuda", dtype=dtype)[:, :cols]
+    x.copy_(_values(rows, cols, dtype, rows))
+    outs = []
+    for r, c in ((rows, cols), (cols, rows)):
+        for n in ((c + 1) // 2, (c + 31) // 32):
+            outs.append(torch.full((r, n + 2 * odd), 7, dtype=torch.uint8, device="cuda")[:, odd:odd + n])
+    B.quant_mxfp4_both(x, *outs)
+    want = (*B.quant_mxfp4(x.contiguous()), *B.quant_mxfp4(x.T.contiguous()))
+    for got, ref in zip(outs, want):
+        assert torch.equal(got, ref)
+        if odd:
+            whole = got.as_strided((got.shape[0], got.shape[1] + 2 * odd), (got.stride(0), 1), got.storage_offset() - odd)
+            assert (whole[:, :odd] == 7).all() and (whole[:, odd + got.shape[1]:] == 7).all()
+
+
 def test_dequant_every_code_and_exponent(B):
     q = torch.arange(256, dtype=torch.uint8).repeat(256, 1)[:, :256].contiguous()
     s = torch.arange(256, dtype=torch.uint8)[:, None].repeat(1, 16)
