@@ -14,12 +14,14 @@
 // them: one that is neither -1 nor a row is treated as masked and raises BSIR_DEVERR_GATHER_INDEX.
 #include "common.cuh"
 
+#include <atomic>
+
 namespace bsir {
 namespace {
 
 // ------------------------------------------------------------------------------------------------ sort
-// A stable counting sort in one launch: one CTA for up to 4096 choices, a cluster of eight for more.  Each of the
-// cluster's warps owns a run of consecutive choices and goes over it 32 at a time: the lanes with one expert find each
+// A stable counting sort in one launch: one CTA for up to 4096 choices, a cluster of eight for up to 16384, of sixteen for
+// more (65536 choices of 128 experts: 8.2 us, 10.7 by eight; 524288: 48 and 89).  Each of the cluster's warps owns a run of consecutive choices and goes over it 32 at a time: the lanes with one expert find each
 // other by ballots over the bits of its number (match.any takes about 70 cycles of the SM, for whatever warp), and a
 // choice's rank among them is a popcount.  That leaves every warp's count of every expert; the counts of the warps
 // before it, of the CTAs before it (read through distributed shared memory) and of the experts before its own add up to
@@ -28,7 +30,7 @@ namespace {
 constexpr int kSortThreads = 1024;
 constexpr int kSortWarps = kSortThreads / 32;
 constexpr int kSortOneCta = 4096;
-constexpr int kSortCluster = 8;
+constexpr int kSortEight = 16384;
 constexpr int kMaxExperts = 1024;
 
 struct SortParams {
@@ -426,6 +428,42 @@ __global__ void __launch_bounds__(kGradThreads) expert_combine_grad_kernel(RowPa
   }
 }
 
+// Whether the current device runs a cluster of sixteen of the sort's CTAs (more than the eight that every one does; a GPC
+// has to have as many SMs).  Asked once per device.
+bool sixteen_at_once() {
+  constexpr int kDevices = 64;
+  static std::atomic<int> known[kDevices];                        // 1: no, 2: yes
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess || device >= kDevices) return false;
+  int answer = known[device].load(std::memory_order_relaxed);
+  if (answer == 0) {
+    int n = 1;
+    for (auto kernel : {expert_sort_kernel<true>, expert_sort_kernel<false>}) {
+      constexpr int kSmem = kMaxExperts * kSortWarps * 4;
+      cudaLaunchConfig_t cfg{};
+      cfg.gridDim = dim3(16);
+      cfg.blockDim = dim3(kSortThreads);
+      cfg.dynamicSmemBytes = kSmem;
+      cudaLaunchAttribute attr;
+      attr.id = cudaLaunchAttributeClusterDimension;
+      attr.val.clusterDim.x = 16;
+      attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+      cfg.attrs = &attr;
+      cfg.numAttrs = 1;
+      int fits = 0;
+      if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess ||
+          cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess ||
+          cudaOccupancyMaxActiveClusters(&fits, kernel, &cfg) != cudaSuccess) {
+        cudaGetLastError();
+        fits = 0;
+      }
+      n = fits < n ? fits : n;
+    }
+    answer = n > 0 ? 2 : 1;
+    known[device].store(answer, std::memory_order_relaxed);
+  }
+  return answer == 2;
+}
 int32_t check_choice(const char *what, int64_t tokens, int64_t top_k, int64_t cols, int64_t rows) {
   if (tokens < 0 || top_k < 0 || cols < 0 || rows < 0 || top_k > 0x7fffffff)
     return fail(BSIR_ERR_SHAPE, "%s: %lld tokens x %lld choices, %lld columns, %lld rows", what, (long long)tokens, (long long)top_k, (long long)cols,
@@ -497,7 +535,7 @@ int32_t bsir_expert_sort(int32_t id_dtype, int64_t tokens, int64_t top_k, int64_
   SortParams p{};
   p.ids = ids; p.n = n; p.experts = static_cast<int>(experts); p.wide = id_dtype == BSIR_I64;
   p.offsets = offsets; p.slots = slots;
-  p.ctas = n > kSortOneCta ? kSortCluster : 1;
+  p.ctas = n <= kSortOneCta ? 1 : n <= kSortEight || !sixteen_at_once() ? 8 : 16;
   p.run = ceil_div(ceil_div(n, static_cast<int64_t>(p.ctas) * kSortWarps), 32) * 32;
   const size_t smem = static_cast<size_t>(experts) * kSortWarps * 4;
   auto kernel = p.run <= 32 * kSortGroups ? expert_sort_kernel<true> : expert_sort_kernel<false>;

@@ -40,6 +40,16 @@ def test_sort(B, tokens, top_k, experts, wide):
     assert np.array_equal(off.cpu().numpy(), wo) and np.array_equal(slots.cpu().numpy(), wsl)
 
 
+@pytest.mark.parametrize("tokens,top_k,experts", [(2048, 8, 60), (2049, 8, 61), (16000, 8, 1024), (16385, 8, 128), (30001, 9, 500)])
+def test_sort_of_many_choices(B, tokens, top_k, experts):
+    """At the borders between the sizes of the cluster, and of what its warps keep in registers."""
+    ids = _ids(tokens, top_k, experts, tokens, skew=True)
+    wo, wsl = R.sort(ids.tolist(), experts)
+    for _ in range(2):
+        off, slots = B.expert_sort(ids.int().cuda(), experts)
+        assert np.array_equal(off.cpu().numpy(), wo) and np.array_equal(slots.cpu().numpy(), wsl)
+
+
 def test_sort_extremes(B):
     off, slots = B.expert_sort(torch.full((5000, 2), -1, dtype=torch.int64, device="cuda"), 4)
     assert (off == 0).all() and (slots == -1).all()
