@@ -275,8 +275,22 @@ template <int BUFS> struct RowWriter {
     }
     __syncwarp();
     const int have = static_cast<int>(p.n - col0 < cols ? p.n - col0 : cols) * eb;    // bytes of a row
-    if (p.tma_out) {                                       // eight lanes a row, four rows at a time
+    if (p.tma_out) {                                       // eight lanes a row, four rows at a time, sixteen in flight
       const int piece = lane & 7;
+      if (have == 128) {
+        char *dst = static_cast<char *>(p.out) + ((row0 + (lane >> 3)) * p.ldo + col0) * eb + piece * 16;
+        const int64_t pitch = 4 * p.ldo * eb;
+        for (int r0 = lane >> 3; r0 < rows; r0 += 16) {
+          uint4 v[4];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) v[u] = *reinterpret_cast<const uint4 *>(buf + (r0 + 4 * u) * 128 + ((piece ^ ((r0 + 4 * u) & 7)) * 16));
+#pragma unroll
+          for (int u = 0; u < 4; ++u, dst += pitch)
+            if (r0 + 4 * u < rows) *reinterpret_cast<uint4 *>(dst) = v[u];
+        }
+        __syncwarp();
+        return;
+      }
       for (int r = lane >> 3; r < rows; r += 4) {
         const uint4 v = *reinterpret_cast<const uint4 *>(buf + r * 128 + ((piece ^ (r & 7)) * 16));
         char *dst = static_cast<char *>(p.out) + ((row0 + r) * p.ldo + col0) * eb + piece * 16;
@@ -290,7 +304,8 @@ template <int BUFS> struct RowWriter {
         }
       }
     } else {
-      // four bytes a lane, eight rows in flight
+      // four bytes a lane, eight rows in flight (16-bit rows that are here whole ask nothing on the way: 333 x 5001 x 2900
+      // 11.6 -> 10.6 us; words of two lanes' halves, stored whole, 14.7)
       const int at = lane * 4;
       const bool low = at < have, high = at + 2 < have;
       char *dst = static_cast<char *>(p.out) + (static_cast<int64_t>(row0) * p.ldo + col0) * eb + at;
@@ -299,6 +314,15 @@ template <int BUFS> struct RowWriter {
         uint32_t v[8];
 #pragma unroll
         for (int r = 0; r < 8; ++r) v[r] = *reinterpret_cast<const uint32_t *>(buf + (r0 + r) * 128 + (((at >> 4) ^ r) * 16) + (at & 15));
+        if (have == 128 && r0 + 8 <= rows && eb == 2) {              // all of it: nothing to ask a row
+          char *d = dst + r0 * pitch;
+#pragma unroll
+          for (int r = 0; r < 8; ++r, d += pitch) {
+            reinterpret_cast<uint16_t *>(d)[0] = static_cast<uint16_t>(v[r]);
+            reinterpret_cast<uint16_t *>(d)[1] = static_cast<uint16_t>(v[r] >> 16);
+          }
+          continue;
+        }
 #pragma unroll
         for (int r = 0; r < 8; ++r) {
           if (r0 + r >= rows || !low) continue;
