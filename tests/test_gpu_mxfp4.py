@@ -1,5 +1,7 @@
 """GPU: microscaled 4-bit quantisation and products against the 64-bit statements of mxfp4_reference.py.  Quantisation
 and its inverse are bit-exact; products of one exponent are exact in f32, others within the bound of an f32 sum."""
+import threading
+
 import numpy as np
 import pytest
 import torch
@@ -382,6 +384,30 @@ def test_capture_streams_and_repeats(B):
     out.zero_()
     step()
     assert torch.equal(out, replay) and (out[22:] == 0).all() and out[:22].abs().sum() > 0
+
+
+def test_two_threads_on_two_streams(B):
+    """Clusters that share K, from two threads at once: the same bits as alone."""
+    a, sa = R.random_codes(64, 8192, 1)
+    b, sb = R.random_codes(1000, 8192, 2)
+    alone = B.matmul_mxfp4(a, sa, b, sb, out_dtype=torch.float32)
+    torch.cuda.synchronize()
+    got = [[], []]
+
+    def work(i):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(20):
+                got[i].append(B.matmul_mxfp4(a, sa, b, sb, out_dtype=torch.float32))
+        stream.synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert all(torch.equal(y, alone) for ys in got for y in ys) and len(got[0]) == len(got[1]) == 20
+    assert B.device_error() == 0
 
 
 def test_python_refusals(B):
