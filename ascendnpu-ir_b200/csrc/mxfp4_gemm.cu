@@ -518,7 +518,12 @@ __device__ __forceinline__ void join_partials(const MxParams &p, const MxTile &t
   }
 }
 
-__device__ __forceinline__ void epilogue_barrier() { asm volatile("bar.sync 1, 128;" ::: "memory"); }      // its four warps
+// where the epilogue's four warps meet; true if all of them say so
+__device__ __forceinline__ bool epilogue_barrier(bool ok) {
+  uint32_t all;
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbar.red.and.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(all) : "r"(static_cast<uint32_t>(ok)) : "memory");
+  return all != 0;
+}
 
 // The bounded wait for a whole warp: all lanes go on or all give up, so that none is left at a warp barrier.
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int *abort_flag, int *err) {
@@ -779,7 +784,9 @@ __global__ void __launch_bounds__(MxCfg<BN, MODE>::kThreads, 1)
           __syncwarp();
         }
       }
-      if (!warp_wait(acc_full_bar(acc), acc_phase, abort_flag, p.err)) break;
+      bool landed = warp_wait(acc_full_bar(acc), acc_phase, abort_flag, p.err);
+      if constexpr (SWAP) landed = epilogue_barrier(landed);        // all four warps go on or none; the tile before has left
+      if (!landed) break;
       tc_fence_after();
       const uint32_t src = tmem + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>(acc * BN);
       auto release = [&]() {
@@ -793,10 +800,9 @@ __global__ void __launch_bounds__(MxCfg<BN, MODE>::kThreads, 1)
       if constexpr (SWAP) {                           // lane = column of C, register = row
         if (team == 1) {                              // through shared memory: rows of C leave in 8- or 16-byte pieces
           uint8_t *tile_s = gen + Cfg::kEpiOff;
-          epilogue_barrier();                         // the tile before has left
           store_partial_swapped<BN>(tile_s, src, quad * 32 + lane);
           release();
-          epilogue_barrier();
+          epilogue_barrier(true);
           const int64_t col = t.n0 + 4 * lane;
           float bias[4];
           load_bias4(p, t.group, col, bias);
