@@ -24,19 +24,12 @@ _BLOCK = 32
 _DT = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
 
 
-_library = None
-
-
 def _bsir():
-    """The package, imported once as a program would, not in every pass."""
-    global _library
-    if _library is None:
-        p = os.path.join(os.getcwd(), "ascendnpu-ir_b200")
-        if p not in sys.path:
-            sys.path.insert(0, p)
-        import bsir
-        _library = bsir
-    return _library
+    p = os.path.join(os.getcwd(), "ascendnpu-ir_b200")
+    if p not in sys.path:
+        sys.path.insert(0, p)
+    import bsir
+    return bsir
 
 
 # ------------------------------------------------------------------------------------------------ the cases
