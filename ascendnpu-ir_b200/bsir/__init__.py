@@ -883,7 +883,8 @@ def matmul_mxfp4(a: torch.Tensor, scale_a: torch.Tensor, b: torch.Tensor, scale_
 
     With ``offsets`` (int32 [groups + 1] on the device) b, scale_b are [groups, n, ..] and rows offsets[g] .. offsets[g + 1]
     of a meet matrix g (and bias [groups, n], or [n] for all): the experts' products.  Rows that no group holds keep
-    what ``out`` had in them.  Rows of codes and exponents start 16-byte aligned (:func:`quant_mxfp4` makes them so)."""
+    what ``out`` had in them, zeros when it is made here.  Rows of codes and exponents start 16-byte aligned
+    (:func:`quant_mxfp4` makes them so)."""
     if a.dim() != 2 or b.dim() != (3 if offsets is not None else 2) or scale_b.dim() != b.dim():
         raise BsirError(-2, "matmul_mxfp4: a [m, k / 2], b [n, k / 2] or, with offsets, [groups, n, k / 2]")
     m, kb = a.shape
@@ -901,6 +902,8 @@ def matmul_mxfp4(a: torch.Tensor, scale_a: torch.Tensor, b: torch.Tensor, scale_
     ldb, ldsb = (bst[-2], sbst[-2]) if n > 1 else (max(kb, 1), max(ks, 1))
     if out is None:
         out, ldo = _matrix(m, n, out_dtype or torch.bfloat16, a.device), max(n, 1)
+        if offsets is not None:
+            out.zero_()                                    # which rows no group holds is known on the device alone
     else:
         if out_dtype is not None and out.dtype != out_dtype:
             raise BsirError(-4, f"matmul_mxfp4: out is {out.dtype}, out_dtype {out_dtype}")

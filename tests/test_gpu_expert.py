@@ -326,3 +326,23 @@ def test_dispatched_codes_go_into_a_product(B, k):
             # sums of k products in f32, each order off by at most k / 2 ulps of the sum of magnitudes
             mags = B.dequant_mxfp4(q[t:t + 1], s[t:t + 1]).abs().double() @ B.dequant_mxfp4(qw, sw).abs().double()[70 * e:70 * e + 70].T
             assert ((y[int(slots[t, j])].double() - ref).abs() <= 2 * k * 2.0 ** -24 * mags[0]).all()
+
+
+@pytest.mark.parametrize("tokens,top_k,experts,n", [(7, 2, 4, 96), (300, 2, 4, 1000)])
+def test_grouped_product_makes_zeros_of_rows_without_a_group(B, tokens, top_k, experts, n):
+    """Masked choices leave rows behind the last expert's; a result made by the call holds zeros there, whatever the
+    memory held before."""
+    k = 256
+    g = torch.Generator().manual_seed(tokens)
+    ids = _ids(tokens, top_k, experts, tokens, masked=0.5).cuda()
+    off, slots = B.expert_sort(ids, experts)
+    q, s = B.quant_mxfp4(torch.randn(tokens, k, generator=g).cuda())
+    _, w = _expert_weights(B, experts, n, k, 1)
+    qr, sr = B.expert_dispatch(q, slots), B.expert_dispatch(s, slots)
+    want = B.matmul_mxfp4(qr, sr, *w, offsets=off, out=torch.zeros(tokens * top_k, n, dtype=torch.bfloat16, device="cuda"))
+    torch.cuda.synchronize()
+    held = int(off[-1])
+    assert 0 < held < tokens * top_k
+    torch.full((tokens * top_k, n), float("nan"), dtype=torch.bfloat16, device="cuda")     # freed at once, for the next call
+    got = B.matmul_mxfp4(qr, sr, *w, offsets=off)
+    assert (got[held:] == 0).all() and torch.equal(got, want)
