@@ -736,6 +736,29 @@ bool ranges_overlap(const void *a, int64_t na, const void *b, int64_t nb) {
   const char *a0 = static_cast<const char *>(a), *b0 = static_cast<const char *>(b);
   return a0 < b0 + nb && b0 < a0 + na;
 }
+// rows of bytes: `rows` stretches of `width`, `stride` apart
+struct ByteRows {
+  const uint8_t *p;
+  int64_t rows, width, stride;
+  int64_t span() const { return (rows - 1) * stride + width; }
+};
+// Whether two such sets share a byte.  Codes and exponents may lie side by side in rows of one buffer, so the stretches
+// count, not the spans from the first to the last.
+bool rows_overlap(ByteRows a, ByteRows b) {
+  if (!ranges_overlap(a.p, a.span(), b.p, b.span())) return false;
+  if (a.rows > b.rows) { const ByteRows t = a; a = b; b = t; }
+  if (a.stride == b.stride) {                    // one place within a row's pitch for all rows
+    const int64_t ahead = static_cast<int64_t>(reinterpret_cast<intptr_t>(b.p) - reinterpret_cast<intptr_t>(a.p));
+    const int64_t d = ((ahead % a.stride) + a.stride) % a.stride;
+    return d < a.width || d + b.width > a.stride;
+  }
+  for (int64_t i = 0; i < a.rows; ++i) {         // the first row of b that ends behind this one's start
+    const int64_t at = static_cast<int64_t>(reinterpret_cast<intptr_t>(a.p) - reinterpret_cast<intptr_t>(b.p)) + i * a.stride;
+    const int64_t j = at < b.width ? 0 : (at - b.width) / b.stride + 1;
+    if (j < b.rows && j * b.stride < at + a.width) return true;
+  }
+  return false;
+}
 
 }  // namespace
 }  // namespace bsir
@@ -767,6 +790,12 @@ extern "C" int32_t bsir_quant_mxfp4(int32_t dtype, int64_t rows, int64_t cols, c
     if (ranges_overlap(x, x_bytes, cq, (r - 1) * qs + (c + 1) / 2) || ranges_overlap(x, x_bytes, cs, (r - 1) * ss + ceil_div(c, kBlock)))
       return fail(BSIR_ERR_UNSUPPORTED, "quant_mxfp4: a result may not overlap the source");
   }
+  const ByteRows results[4] = {{q, rows, (cols + 1) / 2, q_row_stride}, {scale, rows, ceil_div(cols, kBlock), scale_row_stride},
+                               {qt, cols, (rows + 1) / 2, qt_row_stride}, {scale_t, cols, ceil_div(rows, kBlock), scale_t_row_stride}};
+  for (int i = 0; i < 4; ++i)
+    for (int j = i + 1; j < 4; ++j)
+      if (results[i].p && results[j].p && rows_overlap(results[i], results[j]))
+        return fail(BSIR_ERR_UNSUPPORTED, "quant_mxfp4: the results may not overlap each other");
   QuantParams p{};
   p.rows = rows; p.cols = cols; p.x = x; p.xs = x_row_stride;
   p.q = q; p.qs = q_row_stride; p.s = scale; p.ss = scale_row_stride;

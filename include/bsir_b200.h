@@ -520,7 +520,8 @@ BSIR_API int32_t bsir_matmul_w4a16_peers(int64_t m, int64_t n, int64_t k, int64_
  * down the columns, result transposed -- codes [cols, ceil(rows / 2)], exponents [cols, ceil(rows / 32)].  Either pair may
  * be NULL; with both the source is read once.  The products of a linear layer's backward pass contract other axes than
  * its forward product, so dY is wanted both ways, X and W down their columns.
- * x: f32, f16 or bf16; at most 2^31 rows and columns; results may not overlap x. */
+ * x: f32, f16 or bf16; at most 2^31 rows and columns; results may overlap neither x nor each other (rows of codes and
+ * of exponents may lie side by side in one buffer). */
 BSIR_API int32_t bsir_quant_mxfp4(int32_t dtype, int64_t rows, int64_t cols, const void *x, int64_t x_row_stride, uint8_t *q,
                                   int64_t q_row_stride, uint8_t *scale, int64_t scale_row_stride, uint8_t *qt,
                                   int64_t qt_row_stride, uint8_t *scale_t, int64_t scale_t_row_stride, void *stream);

@@ -128,3 +128,33 @@ def test_expert_refusals(L):
     assert grad(g=None) == -1 and grad(y=None) == -1 and grad(slots=None) == -1 and grad(dy=None) == -1 and grad(dw=None) == -1
     assert grad(gs=7) == -3 and grad(ys=7) == -3 and grad(dys=7) == -3 and grad(dw=A4 + 2) == -6
     assert grad(dy=A1) == -11 and grad(dw=A2) == -11 and grad(dw=A4 + 16) == -11
+
+
+# Results side by side in rows of one buffer are told from results that share bytes.
+@pytest.mark.parametrize("kw", [
+    dict(s=A1 + 31),                                             # the last byte of the first row of codes
+    dict(s=A1 - 1, ss=2),                                        # the second exponent of the first row
+    dict(qs=64, s=A1 + 63, ss=64),                               # wraps into the next row of codes
+    dict(qs=48, s=A1 + 40, ss=40),                               # other pitches: row 2's exponents lie in row 2's codes
+    dict(qt=A1 + 96, qts=2, st=A4, sts=1),                       # one direction with the other
+    dict(qt=A3, qts=2, st=A2 + 7, sts=1),
+    dict(qt=A3, qts=2, st=A3 + 127, sts=1),
+    dict(q=None, s=None, qt=A3, qts=2, st=A3 + 1, sts=2),
+    dict(rows=1, s=A1 + 31), dict(cols=1, qt=A3, qts=2, st=A3 + 1, sts=1),
+])
+def test_quant_results_that_share_bytes_are_refused(L, kw):
+    assert _quant(L, **kw) == -11
+    assert b"each other" in L.bsir_last_error()
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="the addresses are made up, and the call gets as far as the launch")
+@pytest.mark.parametrize("kw", [
+    dict(s=A1 + 128), dict(s=A1 - 8),                            # behind and ahead
+    dict(qs=48, s=A1 + 32, ss=48), dict(qs=48, s=A1 - 2, ss=48), # between the rows of codes
+    dict(qs=34, s=A1 + 32, ss=34), dict(qs=64, s=A1 + 33, ss=128),
+    dict(qs=64, ss=64, s=A1 + 32, qt=A3, qts=3, st=A3 + 2, sts=3),
+    dict(rows=1, s=A1 + 32), dict(rows=1, qs=1, s=A1 + 32, ss=1),
+])
+def test_quant_results_side_by_side_are_not(L, kw):
+    _quant(L, **kw)
+    assert b"overlap" not in L.bsir_last_error()
