@@ -188,11 +188,23 @@ int *device_error_word() {
   if (!p) return nullptr;
   std::lock_guard<std::mutex> lock(p->mu);
   if (!p->error_word) {
-    if (cudaMalloc(reinterpret_cast<void **>(&p->error_word), sizeof(int)) != cudaSuccess) {
+    // The first use may fall into a capture, which an allocation or anything on the legacy stream would end: the
+    // thread's capture mode is relaxed meanwhile, and the word is cleared on a stream of its own.
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    int *word = nullptr;
+    cudaStream_t st = nullptr;
+    const bool ok = cudaMalloc(reinterpret_cast<void **>(&word), sizeof(int)) == cudaSuccess &&
+                    cudaStreamCreateWithFlags(&st, cudaStreamNonBlocking) == cudaSuccess &&
+                    cudaMemsetAsync(word, 0, sizeof(int), st) == cudaSuccess && cudaStreamSynchronize(st) == cudaSuccess;
+    if (st) cudaStreamDestroy(st);
+    if (!ok && word) cudaFree(word);
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    if (!ok) {
       cudaGetLastError();
       return nullptr;
     }
-    cudaMemset(p->error_word, 0, sizeof(int));
+    p->error_word = word;
   }
   return p->error_word;
 }

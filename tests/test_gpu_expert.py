@@ -1,5 +1,9 @@
 """GPU: tokens sorted by expert and back, with weights and gradients, against plain loops in 64 bits; and a whole
 mixture-of-experts layer made of the library's calls."""
+import os
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 import torch
@@ -346,3 +350,43 @@ def test_grouped_product_makes_zeros_of_rows_without_a_group(B, tokens, top_k, e
     torch.full((tokens * top_k, n), float("nan"), dtype=torch.bfloat16, device="cuda")     # freed at once, for the next call
     got = B.matmul_mxfp4(qr, sr, *w, offsets=off)
     assert (got[held:] == 0).all() and torch.equal(got, want)
+
+
+FIRST_CALLS = """
+import sys
+sys.path.insert(0, sys.argv[1])
+import torch
+import bsir as B
+g = torch.Generator(device="cuda").manual_seed(1)
+x = torch.randn(96, 256, device="cuda", generator=g).bfloat16()
+w = torch.randn(4 * 64, 256, device="cuda", generator=g).bfloat16()
+ids = torch.randint(-1, 4, (96, 2), device="cuda", generator=g)
+wt = torch.rand(96, 2, device="cuda", generator=g)
+
+def step():
+    off, slots = B.expert_sort(ids, 4)
+    q, s, qt, st = B.quant_mxfp4_both(x)
+    qw, sw = B.quant_mxfp4(w)
+    cut = lambda t: t.as_strided((4, 64, t.shape[1]), (64 * t.stride(0), t.stride(0), 1))
+    y = B.matmul_mxfp4(B.expert_dispatch(q, slots), B.expert_dispatch(s, slots), cut(qw), cut(sw), offsets=off)
+    out = B.expert_combine(y, slots, wt)
+    return off, slots, B.dequant_mxfp4(qt, st), y, out, *B.expert_combine_grad(out, y, slots, wt)
+
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph, capture_error_mode=sys.argv[2]):
+    got = step()
+graph.replay()
+torch.cuda.synchronize()
+assert B.device_error() == 0
+assert all(torch.equal(a, b) for a, b in zip(got, step()))
+print("same")
+"""
+
+
+@pytest.mark.parametrize("mode", ["global", "thread_local"])
+def test_first_calls_inside_a_capture(mode):
+    """A process whose first calls are captured: nothing has to run once before."""
+    import bsir
+    root = os.path.dirname(os.path.dirname(os.path.abspath(bsir.__file__)))
+    r = subprocess.run([sys.executable, "-c", FIRST_CALLS, root, mode], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "same" in r.stdout, r.stdout + r.stderr
