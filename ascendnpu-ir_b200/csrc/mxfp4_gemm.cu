@@ -555,7 +555,7 @@ __global__ void __launch_bounds__(MxCfg<BN, MODE>::kThreads, 1)
   auto acc_empty_bar = [&](int b) { return bars + 8u * (kB3 + 2 + b); };
   static_assert(8 * (kB3 + 4) + 16 <= 512, "barriers");
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(gen + Cfg::kBarOff + 8 * (kB3 + 4));
-  volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);    // in a pair two counts of loads follow
   int *tile_start = reinterpret_cast<int *>(gen + Cfg::kTableOff);         // [groups + 1]
   int *row_start = tile_start + kMaxGroups + 1;                            // [groups + 1]
 
@@ -644,7 +644,7 @@ __global__ void __launch_bounds__(MxCfg<BN, MODE>::kThreads, 1)
     // ---------------- TMA producer
     if (lane == 0) {
       int stage = 0, sf = 0;
-      uint32_t phase = 0, sf_phase = 0;
+      uint32_t phase = 0, sf_phase = 0, issued = 0;
       bool ok = true;
       for (int tile = first_tile; tile < total_tiles && ok; tile += tile_step) {
         find_tile<kRows, kColsC>(tile, tile_start, row_start, group, t);
@@ -667,6 +667,7 @@ __global__ void __launch_bounds__(MxCfg<BN, MODE>::kThreads, 1)
             if (rank == 0) mbar_expect_tx(full_bar(stage), 2 * Cfg::kStage);
             tma_load_3d_pair(dst, &tmap_m, kb * 128, m0, zm, leader);
             tma_load_3d_pair(dst + kTileM * 128, &tmap_n, kb * 128, n0, zn, leader);
+            ++issued;
           } else {
             mbar_expect_tx(full_bar(stage), Cfg::kStage);
             tma_load_3d(dst, &tmap_m, kb * 128, m0, zm, full_bar(stage));
@@ -675,14 +676,10 @@ __global__ void __launch_bounds__(MxCfg<BN, MODE>::kThreads, 1)
           if (++stage == Cfg::kStages) { stage = 0; phase ^= 1u; }
         }
       }
-      if (!ok) {      // gave up: let the copies in flight land before the CTA leaves
-        for (int s = 0; s < Cfg::kStages; ++s)
-          for (int i = 0; i < 200000; ++i)
-            if (mbar_try_wait(full_bar(s), 0) || mbar_try_wait(full_bar(s), 1)) break;
-        for (int s = 0; s < Cfg::kSfStages; ++s)
-          for (int i = 0; i < 200000; ++i)
-            if (mbar_try_wait(sf_full_bar(s), 0) || mbar_try_wait(sf_full_bar(s), 1)) break;
-      }
+      // whoever gives up, the loads land before the CTA leaves; a pair's codes, which land on the leader's barriers, at its end
+      if constexpr (PAIR) store_cluster(map_to_cta(smem_u32(tmem_slot + 2 + rank), 0), issued);
+      else ring_drain(Cfg::kStages, stage, phase, full_bar);
+      ring_drain(Cfg::kSfStages, sf, sf_phase, sf_full_bar);
     }
   } else if (warp == 1) {
     // ---------------- MMA issuer (the pair's leader only)
@@ -726,6 +723,9 @@ __global__ void __launch_bounds__(MxCfg<BN, MODE>::kThreads, 1)
         }
         if (++acc == Cfg::kAccs) { acc = 0; acc_phase ^= 1u; }
       }
+      // and the instructions that were issued end before it gives its tensor memory back
+      const int last = ring_last_slot(Cfg::kStages, stage);
+      mbar_drain(empty_bar(last), ring_last_parity(last, stage, phase));
     }
   } else if (warp >= 2 + Cfg::kEpiWarps) {
     // ---------------- exponents: blocks of 128 rows, turned in place: row r's words w -> lane r % 32 of word w
@@ -851,7 +851,15 @@ __global__ void __launch_bounds__(MxCfg<BN, MODE>::kThreads, 1)
   }
   tc_fence_before();
   __syncthreads();
-  if (team > 1) cluster_sync_all();       // a peer may still signal into this CTA or read its shared memory
+  // a peer may still signal into this CTA or read its shared memory
+  if constexpr (PAIR) {
+    uint32_t again = smem_u32(smem_raw);          // worked out anew: kept from above it costs the epilogue registers that it spills
+    asm volatile("" : "+r"(again));
+    again = ((again + 1023u) & ~1023u) + Cfg::kBarOff;
+    pair_leave(again + 8 * (kB3 + 4) + 4, again, Cfg::kStages, Cfg::kStage);
+  } else if (team > 1) {
+    cluster_sync_all();
+  }
   if (warp == 1) {
     tc_fence_after();
     if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Cfg::kTmemCols) : "memory");

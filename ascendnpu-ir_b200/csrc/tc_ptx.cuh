@@ -6,6 +6,7 @@
 #include <cuda.h>
 
 #include "common.cuh"
+#include "ring.h"
 
 namespace bsir {
 
@@ -67,6 +68,18 @@ __device__ __forceinline__ bool mbar_wait_relaxed(uint32_t bar, uint32_t parity,
       }
     }
   }
+}
+
+// The wait of a role on its way out for what it has under way itself, which would otherwise land in shared or tensor memory
+// that may be another CTA's by then.  It looks at no flag, as the role may be leaving because of one; about 0.2 seconds.
+__device__ __forceinline__ void mbar_drain(uint32_t bar, uint32_t parity) {
+  const long long t0 = clock64();
+  while (!mbar_try_wait(bar, parity) && clock64() - t0 < 400000000LL) { }
+}
+// A producer's ring of `slots` barriers `full(slot)`: waits for the last load of each.
+template <class Full>
+__device__ __forceinline__ void ring_drain(int slots, int slot, uint32_t phase, Full full) {
+  for (int s = 0; s < slots; ++s) mbar_drain(full(s), ring_last_parity(s, slot, phase));
 }
 
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap *map, int x, int y, uint32_t bar) {
@@ -186,6 +199,9 @@ __device__ __forceinline__ uint32_t map_to_cta(uint32_t addr, uint32_t rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
   return r;
 }
+__device__ __forceinline__ void store_cluster(uint32_t cluster_addr, uint32_t v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr), "r"(v) : "memory");
+}
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
@@ -199,6 +215,35 @@ __device__ __forceinline__ void tc_commit_pair(uint32_t bar) {   // arrives on `
   asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
                "h"(static_cast<uint16_t>(3))
                : "memory");
+}
+
+// The end of a pair's kernel, by all threads of both CTAs after their roles have met.  `state` is the shared-memory address
+// of three words: the CTA's give-up flag and, in the leader, the loads issued by itself and by its peer, whose bytes all
+// complete on the leader's barriers, at `full` on.  Neither CTA goes on before the other is done, nor, if one gave up,
+// before the loads of both have landed.
+__device__ __forceinline__ uint32_t load_shared(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.volatile.shared::cta.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+struct PairRing {
+  uint32_t full;
+  __device__ __forceinline__ void complete(uint32_t s, uint32_t bytes) {
+    asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(full + 8u * s), "r"(bytes) : "memory");
+  }
+  __device__ __forceinline__ void expect(uint32_t s, uint32_t bytes) { mbar_expect_tx(full + 8u * s, bytes); }
+  __device__ __forceinline__ void wait(uint32_t s, uint32_t parity) { mbar_drain(full + 8u * s, parity); }
+};
+__device__ __forceinline__ void pair_leave(uint32_t state, uint32_t full, uint32_t slots, uint32_t bytes) {
+  const uint32_t rank = cluster_rank();
+  if (threadIdx.x == 0 && load_shared(state)) store_cluster(map_to_cta(state, rank ^ 1u), 1u);
+  __syncwarp();
+  cluster_sync_all();
+  if (load_shared(state)) {        // in both CTAs or in neither
+    if (rank == 0 && threadIdx.x == 0) ring_settle_pair(slots, load_shared(state + 4), load_shared(state + 8), bytes, PairRing{full});
+    __syncwarp();
+    cluster_sync_all();
+  }
 }
 
 // TMA stores from shared memory, one bulk group each
