@@ -471,10 +471,9 @@ __global__ void __launch_bounds__(BOTH ? 2 * kColThreads : kColThreads, BOTH ? (
         s += (kColThreads / 8) * p.ss;
       }
     }
-    if (!__syncthreads_and(ok)) {        // gave up: let the copies in flight land before the CTA leaves
-      if (tid == 0)
-        for (int s = 0; s < 2; ++s)
-          for (int i = 0; i < 200000 && !mbar_try_wait(smem_u32(&full_s[s]), ((n + ((n ^ s) & 1)) >> 1) & 1); ++i) { }
+    if (!__syncthreads_and(ok)) {        // gave up: the copies under way, of this tile and the next, land before the CTA leaves
+      const int issued = n + (t + static_cast<int64_t>(gridDim.x) < tiles ? 2 : 1);
+      if (tid == 0) ring_drain(2, issued & 1, issued >> 1 & 1, [&](int s) { return smem_u32(&full_s[s]); });
       break;
     }
     if (tid == 0 && t + 2 * static_cast<int64_t>(gridDim.x) < tiles) load(t + 2 * static_cast<int64_t>(gridDim.x), b);

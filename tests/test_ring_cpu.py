@@ -114,8 +114,10 @@ def test_ring_waits_for_what_is_under_way(tmp_path):
     assert r.returncode == 0 and r.stdout.strip() == "held", r.stdout
 
 
-@pytest.mark.parametrize("name", ["mxfp4_gemm.cu"])
-def test_no_wait_takes_either_parity(name):
-    """A wait that either parity of a barrier ends is over at once, whatever is under way."""
+@pytest.mark.parametrize("name", ["mxfp4_gemm.cu", "mxfp4_quant.cu"])
+def test_waits_on_the_way_out_go_by_the_ring(name):
+    """A wait that either parity of a barrier ends is over at once, whatever is under way; one for a load that was never
+    issued spins to its limit."""
     text = open(os.path.join(CSRC, name)).read()
     assert not re.search(r"try_wait\([^;]*, 0\) \|\| mbar_try_wait\([^;]*, 1\)", text)
+    assert not re.search(r"i < 200000", text) and re.search(r"ring_drain\(", text)
