@@ -431,13 +431,7 @@ __global__ void __launch_bounds__(kThreads + 32, 1)
           if (++stage == Cfg::kStages) { stage = 0; phase ^= 1u; }
         }
       }
-      if (!ok) {
-        // loads already issued still write this CTA's shared memory: wait (bounded) for them
-        for (int s = 0; s < Cfg::kStages; ++s) {
-          for (int i = 0; i < 200000; ++i)
-            if (mbar_try_wait(full_bar(s), 0) || mbar_try_wait(full_bar(s), 1)) break;
-        }
-      }
+      ring_drain(Cfg::kStages, stage, phase, full_bar);      // whoever gives up, the loads land before the CTA leaves
     }
   } else if (warp == 1 || warp == 6) {
     // ---------------- MMA issuers
@@ -487,6 +481,8 @@ __global__ void __launch_bounds__(kThreads + 32, 1)
         acc_phase[acc] ^= 1u;
         acc ^= 1;
       }
+      const int last = ring_last_slot(Cfg::kStages, stage);  // and the MMAs end before it gives its tensor memory back
+      mbar_drain(empty_bar(last), ring_last_parity(last, stage, phase));
     }
   } else {
     // ---------------- epilogue: warps 2..5, TMEM lane quadrant = warp % 4
@@ -706,16 +702,11 @@ __global__ void __launch_bounds__(kDecThreads, 1)
   if (warp == 0) {
     // ---------------- TMA producer
     if (lane == 0) {
-      bool ok = true;
       for (int it = preissued; it < total_its; ++it) {
-        if (!mbar_wait(empty_bar(p_stage), (p_round & 1u) ^ 1u, abort_flag, p.err)) { ok = false; break; }
+        if (!mbar_wait(empty_bar(p_stage), (p_round & 1u) ^ 1u, abort_flag, p.err)) break;
         issue_next();
       }
-      if (!ok) {
-        for (int s = 0; s < nstages; ++s)
-          for (int i = 0; i < 200000; ++i)
-            if (mbar_try_wait(full_bar(s), 0) || mbar_try_wait(full_bar(s), 1)) break;
-      }
+      ring_drain(nstages, p_stage, p_round & 1u, full_bar);  // whoever gives up, the loads land before the CTA leaves
     }
   } else if (warp == 1 || warp >= 6) {
     // ---------------- MMA issuers: warp 1 takes k step 0 of every block, warps 6..8 steps 1..3
@@ -759,6 +750,8 @@ __global__ void __launch_bounds__(kDecThreads, 1)
         acc_phase[acc] ^= 1u;
         acc ^= 1;
       }
+      const int last = ring_last_slot(nstages, stage);       // and the MMAs end before it gives its tensor memory back
+      mbar_drain(empty_bar(last), ring_last_parity(last, stage, phase));
     }
   } else {
     // ---------------- epilogue: warps 2..5, TMEM lane quadrant = warp % 4; lane = output column
@@ -976,8 +969,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   auto tfull_bar = [&](int a) { return bars + 8u * (2 * kPairStages + a); };
   auto tempty_bar = [&](int a) { return bars + 8u * (2 * kPairStages + 2 + a); };
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(gen_base + kPairStages * kPairStage + 8 * (2 * kPairStages + 4));
-  volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
-  volatile uint32_t *tiles_started = tmem_slot + 2;     // tiles whose overwriting MMA the first issuer has issued
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);    // the loads issued by either CTA follow
+  volatile uint32_t *tiles_started = tmem_slot + 4;     // tiles whose overwriting MMA the first issuer has issued
   constexpr int kIssuers = KIND == KI8 ? 2 : 1;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -1009,7 +1002,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     // ---------------- TMA producer (both CTAs): own half of the operands, completion on the leader's barrier
     if (lane == 0) {
       int stage = 0;
-      uint32_t phase = 0;
+      uint32_t phase = 0, issued = 0;
       bool ok = true;
       for (int tile = pair; tile < total_tiles && ok; tile += npairs) {
         const int m0 = (tile % m_tiles2) * 256 + static_cast<int>(rank) * 128;
@@ -1032,9 +1025,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
           } else {
             tma_load_2d_pair(sb, &tmap_b, kb * kBK, n0, leader_full);
           }
+          ++issued;
           if (++stage == kPairStages) { stage = 0; phase ^= 1u; }
         }
       }
+      store_cluster(map_to_cta(smem_u32(tmem_slot + 2 + rank), 0), issued);
     }
   } else if (warp == 1 || warp == 6) {
     // ---------------- MMA issuers: leader CTA only
@@ -1084,6 +1079,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         acc_phase[acc] ^= 1u;
         acc ^= 1;
       }
+      const int last = ring_last_slot(kPairStages, stage);   // the MMAs end before the CTAs give their tensor memory back
+      mbar_drain(empty_bar(last), ring_last_parity(last, stage, phase));
     }
   } else {
     // ---------------- epilogue (both CTAs): own 128 accumulator rows x 256 columns
@@ -1118,7 +1115,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 
   tc_fence_before();
   __syncthreads();
-  cluster_sync_all();      // the peer may still be signalling into this CTA / reading its shared memory
+  // the peer may still be signalling into this CTA / reading its shared memory
+  pair_leave(smem_u32(tmem_slot + 1), full_bar(0), kPairStages, kPairStage);
   if (warp == 1) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512) : "memory");
