@@ -429,18 +429,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 
   if (warp == kTcDqWarps) {
     if (lane == 0) {
-      bool ok = true;
       int slot = preissued % nstages;
       uint32_t phase = static_cast<uint32_t>(preissued / nstages) & 1u;
       for (int s = preissued; s < nstages_total; ++s) {
-        if (!mbar_wait_relaxed(wempty(slot), phase ^ 1u, abort_flag, err)) { ok = false; break; }
+        if (!mbar_wait_relaxed(wempty(slot), phase ^ 1u, abort_flag, err)) break;
         issue_stage(s);
         if (++slot == nstages) { slot = 0; phase ^= 1u; }
       }
-      if (!ok)
-        for (int s = 0; s < nstages; ++s)
-          for (int i = 0; i < 200000; ++i)
-            if (mbar_try_wait(wfull(s), 0) || mbar_try_wait(wfull(s), 1)) break;
+      ring_drain(nstages, slot, phase, wfull);               // whoever gives up, the loads land before the CTA leaves
     }
   } else if (warp > kTcDqWarps + kTcMmaWarps) {
     // ---------------- activation fix-up: every 16-byte piece of the stage into the nibble-pair k order
@@ -496,6 +492,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (++slot == nstages) { slot = 0; phase ^= 1u; }
       }
       tc_commit(dfull);   // arrives once this issuer's MMAs are done (immediately if it had none)
+      mbar_drain(dfull, 0);   // whoever gives up, all MMAs end before the CTA gives its tensor memory back
     }
   } else {
     // ---------------- dequantisers
@@ -701,20 +698,15 @@ __global__ void __launch_bounds__(kFoldThreads, 1)
     if (lane == 0) {
       int slot = 0;
       uint32_t round = 0;
-      bool ok = true;
       for (int s = 0; s < nstages; ++s) {
-        if (!mbar_wait(empty_p(slot), (round & 1u) ^ 1u, abort_flag, err)) { ok = false; break; }
+        if (!mbar_wait(empty_p(slot), (round & 1u) ^ 1u, abort_flag, err)) break;
         const uint32_t dst = p_base + slot * kFoldPStage;
         mbar_expect_tx(full_p(slot), kFoldPStage);
         tma_load_2d(dst, &tmap_w, n0, s * 8, full_p(slot));                               // [8 word rows x 128 columns]
         tma_load_2d(dst + 8 * kFoldCols * 4, &tmap_a, s * 64, static_cast<int>(m0), full_p(slot));   // [16 rows x 64 k]
         if (++slot == kFoldPStages) { slot = 0; ++round; }
       }
-      if (!ok) {
-        for (int q = 0; q < kFoldPStages; ++q)
-          for (int i = 0; i < 200000; ++i)
-            if (mbar_try_wait(full_p(q), 0) || mbar_try_wait(full_p(q), 1)) break;
-      }
+      ring_drain(kFoldPStages, slot, round & 1u, full_p);    // whoever gives up, the loads land before the CTA leaves
     }
   } else if (warp <= kFoldIssuers + 4) {
     // sums of the activations per (group, row), by the issuing and the folding warps together (they have nothing
@@ -748,15 +740,15 @@ __global__ void __launch_bounds__(kFoldThreads, 1)
       const int issuer = warp - 1;
       // D = f32, A = B = bf16, both K-major, N = 16, M = 128
       const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(16 >> 3) << 17) | (static_cast<uint32_t>(128 >> 4) << 24);
-      bool ok = true;
       static_assert(kFoldIssuers == kFoldOStages, "an issuer per operand slot");
       // spg is 1, 2 or 4: every stage of this issuer belongs to another group, its c-th stage (c = s / 4) goes to its
       // accumulator c % 2, whose (c / 2)-th use this is
-      for (int s = issuer; s < nstages && ok; s += kFoldIssuers) {
+      int s = issuer;
+      for (; s < nstages; s += kFoldIssuers) {
         const int c = s / kFoldIssuers, buf = c & 1;
         const uint32_t use = static_cast<uint32_t>(c >> 1);
-        if (!mbar_wait(tempty(issuer * 2 + buf), (use & 1u) ^ 1u, abort_flag, err)) { ok = false; break; }
-        if (!mbar_wait(full_o(issuer), static_cast<uint32_t>(c) & 1u, abort_flag, err)) { ok = false; break; }
+        if (!mbar_wait(tempty(issuer * 2 + buf), (use & 1u) ^ 1u, abort_flag, err)) break;
+        if (!mbar_wait(full_o(issuer), static_cast<uint32_t>(c) & 1u, abort_flag, err)) break;
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + static_cast<uint32_t>((issuer * 2 + buf) * 16);
         const uint32_t wt = o_base + issuer * kFoldOStage, at = wt + kFoldCols * 128;
@@ -766,6 +758,8 @@ __global__ void __launch_bounds__(kFoldThreads, 1)
         tc_commit(empty_o(issuer));
         tc_commit(tfull(issuer * 2 + buf));
       }
+      // whoever gives up, its MMAs end before the CTA gives its tensor memory back (none: a fresh barrier lets parity 1 through)
+      mbar_drain(empty_o(issuer), static_cast<uint32_t>(s / kFoldIssuers - 1) & 1u);
     }
     } else {
     // ---------------- group fold + output: warps 2..5, TMEM lane quadrant = warp % 4; lane = output column
