@@ -525,11 +525,6 @@ __device__ __forceinline__ bool epilogue_barrier(bool ok) {
   return all != 0;
 }
 
-// The bounded wait for a whole warp: all lanes go on or all give up, so that none is left at a warp barrier.
-__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int *abort_flag, int *err) {
-  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, err)) != 0;
-}
-
 template <int BN, int MODE>
 __global__ void __launch_bounds__(MxCfg<BN, MODE>::kThreads, 1)
     mxfp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_m, const __grid_constant__ CUtensorMap tmap_n,

@@ -70,6 +70,11 @@ __device__ __forceinline__ bool mbar_wait_relaxed(uint32_t bar, uint32_t parity,
   }
 }
 
+// The bounded wait for a whole warp: all lanes go on or all give up, so that none is left at a warp barrier.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int *abort_flag, int *err) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, err)) != 0;
+}
+
 // The wait of a role on its way out for what it has under way itself, which would otherwise land in shared or tensor memory
 // that may be another CTA's by then.  It looks at no flag, as the role may be leaving because of one; about 0.2 seconds.
 __device__ __forceinline__ void mbar_drain(uint32_t bar, uint32_t parity) {

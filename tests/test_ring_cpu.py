@@ -114,7 +114,7 @@ def test_ring_waits_for_what_is_under_way(tmp_path):
     assert r.returncode == 0 and r.stdout.strip() == "held", r.stdout
 
 
-@pytest.mark.parametrize("name", ["mxfp4_gemm.cu", "mxfp4_quant.cu", "gemm_dense.cu", "gemm_w4a16.cu"])
+@pytest.mark.parametrize("name", ["mxfp4_gemm.cu", "mxfp4_quant.cu", "gemm_dense.cu", "gemm_w4a16.cu", "cumulative.cu"])
 def test_waits_on_the_way_out_go_by_the_ring(name):
     """A wait that either parity of a barrier ends is over at once, whatever is under way; one for a load that was never
     issued spins to its limit."""
