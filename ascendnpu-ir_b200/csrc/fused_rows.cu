@@ -15,6 +15,7 @@
 #include <type_traits>
 
 #include "common.cuh"
+#include "ring.h"
 
 namespace bsir {
 namespace {
@@ -531,7 +532,14 @@ __global__ void __launch_bounds__(1024, 1) softmax_stream_kernel(RowGeom g, cons
   for (int64_t k = 0; k < my_rows; ++k) {
     const int b = static_cast<int>(k % kStreamBufs);
     const uint32_t parity = static_cast<uint32_t>((k / kStreamBufs) & 1);
-    if (ok && !mbar_wait_bounded(smem_addr(&bars[b]), parity, err)) ok = false;
+    if (ok && !mbar_wait_bounded(smem_addr(&bars[b]), parity, err)) {
+      ok = false;                 // no more rows are asked for, and those on their way land before the CTA leaves
+      if (t == 0) {
+        const int64_t issued = k + kStreamBufs - 1 < my_rows ? k + kStreamBufs - 1 : my_rows;
+        for (int i = 0; i < kStreamBufs; ++i)
+          mbar_wait_bounded(smem_addr(&bars[i]), ring_last_parity(i, static_cast<int>(issued % kStreamBufs), static_cast<uint32_t>(issued / kStreamBufs) & 1u), err);
+      }
+    }
     const Vec16 *buf = reinterpret_cast<const Vec16 *>(row_smem + static_cast<size_t>(b) * row_bytes);
     Vec16 v[VPT];
 #pragma unroll
@@ -561,7 +569,7 @@ __global__ void __launch_bounds__(1024, 1) softmax_stream_kernel(RowGeom g, cons
     m = row_reduce(m, 1024, red_max, ninf, 0, warp_red_maxnum);
     // every thread has its part of buffer b in registers (the barrier inside row_reduce is behind us),
     // and buffer (k + 2) % 3 was released one row ago: start the copy of the row after next
-    if (t == 0 && k + kStreamBufs - 1 < my_rows) issue(k + kStreamBufs - 1);
+    if (t == 0 && ok && k + kStreamBufs - 1 < my_rows) issue(k + kStreamBufs - 1);
 
     const float kLog2e = 1.4426950408889634f;
     const unsigned long long l2e2 = pack2(kLog2e, kLog2e);
