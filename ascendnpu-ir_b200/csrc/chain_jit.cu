@@ -520,7 +520,14 @@ std::string row_source(const ChainJitSpec &s) {
          "  bool ok = true;\n"
          "  for (i64 k = 0; k < my_rows; ++k) {\n"
          "  const i64 row = blockIdx.x + k * gridDim.x;\n"
-         "  if (ok && !mbar_wait_bounded(smem_u32(&bars[k % NBUF]), (u32)((k / NBUF) & 1), a.err)) ok = false;\n"
+         "  if (ok && !mbar_wait_bounded(smem_u32(&bars[k % NBUF]), (u32)((k / NBUF) & 1), a.err)) {\n"
+         "    ok = false;   // no more rows are asked for, and those on their way land before the block leaves\n"
+         "    if (threadIdx.x == 0) {\n"
+         "      const i64 issued = k + NBUF - 1 < my_rows ? k + NBUF - 1 : my_rows;\n"
+         "      for (int b = 0; b < NBUF; ++b)   // the parity of each buffer's last row (1: none, a fresh barrier lets that through)\n"
+         "        mbar_wait_bounded(smem_u32(&bars[b]), (u32)((issued / NBUF) & 1) ^ (b < issued % NBUF ? 0u : 1u), a.err);\n"
+         "    }\n"
+         "  }\n"
          "  const bool row_ok = ok;\n"
          "  const unsigned char *buf = ring_mem + (size_t)(k % NBUF) * row_bytes;\n";
   } else {
@@ -577,7 +584,7 @@ std::string row_source(const ChainJitSpec &s) {
     c += "  // every thread has its part of this row in registers, and the buffer the row before was read from is free:\n"
          "  // start the copy of the row NBUF - 1 ahead into it\n"
          "  __syncthreads();\n"
-         "  if (threadIdx.x == 0 && k + NBUF - 1 < my_rows) issue(k + NBUF - 1);\n";
+         "  if (threadIdx.x == 0 && ok && k + NBUF - 1 < my_rows) issue(k + NBUF - 1);\n";
   bool tmp_used[4] = {false, false, false, false};
   for (int i = 0; i < s.n_instr; ++i)
     if (s.tape[i].op == BSIR_CHAIN_SAVE) tmp_used[s.tape[i].src] = true;
