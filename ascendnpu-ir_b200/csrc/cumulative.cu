@@ -152,10 +152,8 @@ __global__ void __launch_bounds__(32) cum_first_tma_kernel(const __grid_constant
     prefetch_tmap(&tdst);
   }
   __syncwarp();
-  int64_t issued = 0;
   auto fetch = [&](int64_t it) {                      // lane 0 only
     if (it < ntiles) {
-      issued = it + 1;
       const int64_t s = reverse ? ntiles - 1 - it : it;
       const int b = static_cast<int>(it % depth);
       mbar_expect_tx(smem_u32(&full[b]), kCumColTileBytes);
@@ -167,12 +165,13 @@ __global__ void __launch_bounds__(32) cum_first_tma_kernel(const __grid_constant
   A acc[EPW];
 #pragma unroll
   for (int e = 0; e < EPW; ++e) acc[e] = A{};
-  for (int64_t it = 0; it < ntiles; ++it) {
+  int64_t it = 0;
+  for (; it < ntiles; ++it) {
     const int64_t s = reverse ? ntiles - 1 - it : it;
     const int b = static_cast<int>(it % depth);
     const int64_t left = rows - s * kCumColRows;
     const int nv = left < kCumColRows ? static_cast<int>(left) : kCumColRows;       // rows of this tile that exist
-    if (!warp_wait(smem_u32(&full[b]), static_cast<uint32_t>(it / depth) & 1u, &abort_flag, err)) break;
+    if (!mbar_wait(smem_u32(&full[b]), static_cast<uint32_t>(it / depth) & 1u, &abort_flag, err)) break;
     uint32_t *col = reinterpret_cast<uint32_t *>(tiles + b * kCumColTileBytes) + lane;   // 32 words a row
     if (it > 0 && nv == kCumColRows) {
       if (reverse) cum_col_full_tile<T, KIND, NANP, true, kCumColRows>(col, acc);
@@ -216,11 +215,11 @@ __global__ void __launch_bounds__(32) cum_first_tma_kernel(const __grid_constant
       asm volatile("cp.async.bulk.commit_group;" ::: "memory");
     }
   }
-  if (lane == 0) {
-    // after a wait that gave up the tiles on their way land before the CTA leaves
-    ring_drain(depth, static_cast<int>(issued % depth), static_cast<uint32_t>(issued / depth) & 1u, [&](int s) { return smem_u32(&full[s]); });
-    asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+  if (it < ntiles && lane == 0) {        // gave up: the tiles on their way land before the CTA leaves
+    const int64_t issued = it + depth - 2 < ntiles ? it + depth - 2 : ntiles;
+    ring_drain(depth, static_cast<int>(issued % depth), static_cast<uint32_t>(issued / depth) & 1u, [&](int i) { return smem_u32(&full[i]); });
   }
+  if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
 }
 
 // ------------------------------------------------------------------ axis 1: a warp per 32 rows, tiles of 128 bytes
@@ -339,10 +338,8 @@ __global__ void __launch_bounds__(32) cum_last_tma_kernel(const __grid_constant_
     prefetch_tmap(&tdst);
   }
   __syncwarp();
-  int64_t issued = 0;
   auto fetch = [&](int64_t it) {                      // lane 0 only
     if (it < nsteps) {
-      issued = it + 1;
       const int64_t s = reverse ? nsteps - 1 - it : it;
       const int b = static_cast<int>(it % depth);
       const int nb = static_cast<int>(ntiles - s * W < W ? ntiles - s * W : W);
@@ -354,11 +351,12 @@ __global__ void __launch_bounds__(32) cum_last_tma_kernel(const __grid_constant_
   if (lane == 0)
     for (int64_t it = 0; it < depth - 1; ++it) fetch(it);
   A acc{};
-  for (int64_t it = 0; it < nsteps; ++it) {
+  int64_t it = 0;
+  for (; it < nsteps; ++it) {
     const int64_t s = reverse ? nsteps - 1 - it : it;
     const int b = static_cast<int>(it % depth);
     const int nb = static_cast<int>(ntiles - s * W < W ? ntiles - s * W : W);
-    if (!warp_wait(smem_u32(&full[b]), static_cast<uint32_t>(it / depth) & 1u, &abort_flag, err)) break;
+    if (!mbar_wait(smem_u32(&full[b]), static_cast<uint32_t>(it / depth) & 1u, &abort_flag, err)) break;
 #pragma unroll
     for (int jj = 0; jj < W; ++jj) {
       if (jj < nb) {
@@ -405,11 +403,11 @@ __global__ void __launch_bounds__(32) cum_last_tma_kernel(const __grid_constant_
       asm volatile("cp.async.bulk.commit_group;" ::: "memory");
     }
   }
-  if (lane == 0) {
-    // after a wait that gave up the tiles on their way land before the CTA leaves
-    ring_drain(depth, static_cast<int>(issued % depth), static_cast<uint32_t>(issued / depth) & 1u, [&](int s) { return smem_u32(&full[s]); });
-    asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+  if (it < nsteps && lane == 0) {        // gave up: the tiles on their way land before the CTA leaves
+    const int64_t issued = it + depth - 1 < nsteps ? it + depth - 1 : nsteps;
+    ring_drain(depth, static_cast<int>(issued % depth), static_cast<uint32_t>(issued / depth) & 1u, [&](int i) { return smem_u32(&full[i]); });
   }
+  if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
 }
 
 // generality path for axis 1: a thread per row (ragged or unaligned rows)
