@@ -780,7 +780,9 @@ __global__ void __launch_bounds__(kDecThreads, 1)
         bias_col = (p.bias && col_ok) ? load_f32_as(p.bias, p.bias_dtype, col) : 0.0f;
       }
       const float sa_lane = (p.scale_a && lane < p.m) ? p.scale_a[lane] : 1.0f;   // rows 0..31, one per lane
-      if (!mbar_wait(tfull_bar(acc), acc_phase[acc], abort_flag, p.err)) { ok = false; break; }
+      bool landed = warp_wait(tfull_bar(acc), acc_phase[acc], abort_flag, p.err);
+      if (parts > 1) landed = epilogue_barrier(landed);      // the four warps meet again below: all go on or none
+      if (!landed) { ok = false; break; }
       if (threadIdx.x == 64) TL(4);
       tc_fence_after();
       const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>(acc * nacc * nb);

@@ -518,13 +518,6 @@ __device__ __forceinline__ void join_partials(const MxParams &p, const MxTile &t
   }
 }
 
-// where the epilogue's four warps meet; true if all of them say so
-__device__ __forceinline__ bool epilogue_barrier(bool ok) {
-  uint32_t all;
-  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbar.red.and.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(all) : "r"(static_cast<uint32_t>(ok)) : "memory");
-  return all != 0;
-}
-
 template <int BN, int MODE>
 __global__ void __launch_bounds__(MxCfg<BN, MODE>::kThreads, 1)
     mxfp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_m, const __grid_constant__ CUtensorMap tmap_n,

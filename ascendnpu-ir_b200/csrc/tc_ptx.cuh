@@ -70,6 +70,13 @@ __device__ __forceinline__ bool mbar_wait_relaxed(uint32_t bar, uint32_t parity,
   }
 }
 
+// where the epilogue's four warps meet; true if all of them say so
+__device__ __forceinline__ bool epilogue_barrier(bool ok) {
+  uint32_t all;
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbar.red.and.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(all) : "r"(static_cast<uint32_t>(ok)) : "memory");
+  return all != 0;
+}
+
 // The bounded wait for a whole warp: all lanes go on or all give up, so that none is left at a warp barrier.
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int *abort_flag, int *err) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, err)) != 0;
