@@ -156,9 +156,13 @@ __device__ __forceinline__ void commit_to(uint32_t elected, uint32_t bar) {   //
         "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar), "r"(elected)
         : "memory");
 }
+template <bool CLUSTER>
 __device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {      // without waiting
   uint32_t done;
-  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+  if constexpr (CLUSTER)
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+  else
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(done) : "r"(bar), "r"(parity) : "memory");
   return done != 0;
 }
 // e2m1 x e2m1, exponents E8M0, both K-major; `sf_id` (0 or 2): which two of a cell's four bytes belong to these 64
@@ -172,11 +176,12 @@ __device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(leader_bar)
       : "memory");
 }
-// Arrival on a barrier of the pair's leader by a thread that hands over nothing but its own CTA's shared memory (made
-// visible to the tensor core by fence.proxy.async) or tensor memory (ordered by tcgen05.fence): no release at cluster
-// scope, which took about 1400 cycles next to running copies.
+// Arrival on a barrier of the pair's leader by a thread that hands over its own CTA's shared memory (made visible to the
+// tensor core by fence.proxy.async) or tensor memory (ordered by tcgen05.fence).  The release at cluster scope is restricted
+// to shared memory: the arrival's own, of everything, took about 1400 cycles next to running copies.
 __device__ __forceinline__ void mbar_arrive_leader(uint32_t cluster_addr) {
-  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+  asm volatile("fence.release.sync_restrict::shared::cta.cluster;" ::: "memory");
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 __device__ __forceinline__ uint32_t elect_one() {       // 1 in one lane of the (whole) warp
   uint32_t one;
@@ -678,13 +683,13 @@ __global__ void __launch_bounds__(MxCfg<BN, MODE>::kThreads, 1)
       uint32_t phase = 0, sf_phase = 0, acc_phase = 0;
       bool ok = true, here = false, sf_here = false;
       for (int tile = first_tile; tile < total_tiles && ok; tile += tile_step) {
-        if (!warp_wait(acc_empty_bar(acc), acc_phase ^ 1u, abort_flag, p.err)) break;
+        if (!warp_wait<PAIR>(acc_empty_bar(acc), acc_phase ^ 1u, abort_flag, p.err)) break;
         const uint32_t d = tmem + static_cast<uint32_t>(acc * BN);
         for (int kb = kb0; kb < kb1; ++kb) {
           const uint32_t part = static_cast<uint32_t>(kb) % kChunk;          // of the chunk
           // the next barriers were looked at while the last stage's instructions went out
-          if (part == 0 && !sf_here && !warp_wait(sf_ready_bar(sf), sf_phase, abort_flag, p.err)) { ok = false; break; }
-          if (!here && !warp_wait(full_bar(stage), phase, abort_flag, p.err)) { ok = false; break; }
+          if (part == 0 && !sf_here && !warp_wait<PAIR>(sf_ready_bar(sf), sf_phase, abort_flag, p.err)) { ok = false; break; }
+          if (!here && !warp_wait<PAIR>(full_bar(stage), phase, abort_flag, p.err)) { ok = false; break; }
           tc_fence_after();
           // the stage's codes have landed, so the instructions that used its columns of exponents before are done
           const uint32_t sfb = tmem + static_cast<uint32_t>(Cfg::kSfBase + stage * Cfg::kSfCols), sfa = sfb + 2 * Cfg::kSfN;
@@ -706,8 +711,8 @@ __global__ void __launch_bounds__(MxCfg<BN, MODE>::kThreads, 1)
           if (kb + 1 == kb1) commit_to<MODE>(elected, acc_full_bar(acc));
           if (++stage == Cfg::kStages) { stage = 0; phase ^= 1u; }
           if (sf_done && ++sf == Cfg::kSfStages) { sf = 0; sf_phase ^= 1u; }
-          here = __all_sync(0xffffffffu, mbar_test(full_bar(stage), phase));
-          sf_here = sf_done && __all_sync(0xffffffffu, mbar_test(sf_ready_bar(sf), sf_phase));
+          here = __all_sync(0xffffffffu, mbar_test<PAIR>(full_bar(stage), phase));
+          sf_here = sf_done && __all_sync(0xffffffffu, mbar_test<PAIR>(sf_ready_bar(sf), sf_phase));
         }
         if (++acc == Cfg::kAccs) { acc = 0; acc_phase ^= 1u; }
       }

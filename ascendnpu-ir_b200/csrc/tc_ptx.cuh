@@ -34,12 +34,26 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
+// the same where threads of another CTA of the cluster arrive: what they released at cluster scope is seen
+__device__ __forceinline__ bool mbar_try_wait_cluster(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
 // Bounded wait.  Returns false when it gave up or another role raised the abort flag.
+template <bool CLUSTER = false>
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int *abort_flag, int *err) {
-  if (mbar_try_wait(bar, parity)) return true;
+  auto tried = [&]() { return CLUSTER ? mbar_try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity); };
+  if (tried()) return true;
   const long long t0 = clock64();
   for (uint32_t spin = 0;; ++spin) {
-    if (mbar_try_wait(bar, parity)) return true;
+    if (tried()) return true;
     if ((spin & 255u) == 255u) {
       if (*abort_flag) return false;
       if (clock64() - t0 > 4000000000LL) {  // about two seconds
@@ -78,8 +92,9 @@ __device__ __forceinline__ bool epilogue_barrier(bool ok) {
 }
 
 // The bounded wait for a whole warp: all lanes go on or all give up, so that none is left at a warp barrier.
+template <bool CLUSTER = false>
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int *abort_flag, int *err) {
-  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, err)) != 0;
+  return __all_sync(0xffffffffu, mbar_wait<CLUSTER>(bar, parity, abort_flag, err)) != 0;
 }
 
 // The wait of a role on its way out for what it has under way itself, which would otherwise land in shared or tensor memory
