@@ -931,6 +931,14 @@ def matmul_mxfp4(a: torch.Tensor, scale_a: torch.Tensor, b: torch.Tensor, scale_
     return out
 
 
+def matmul_mxfp4_form(m: int, n: int, k: int, groups: int = 1):
+    """The form that :func:`matmul_mxfp4` takes for these sizes on the current device: (rows and columns of a tile of C, CTAs
+    that work on one).  Where several CTAs share a tile's K their number depends on the device, and so may the last bits."""
+    r, c, ctas = C.c_int32(), C.c_int32(), C.c_int32()
+    _check(lib().bsir_matmul_mxfp4_form(C.c_int64(m), C.c_int64(n), C.c_int64(k), C.c_int64(groups), C.byref(r), C.byref(c), C.byref(ctas)))
+    return r.value, c.value, ctas.value
+
+
 # ---------------------------------------------------------------------------- mixtures of experts
 def _choices(slots: torch.Tensor, what: str):
     if slots.dim() != 2 or slots.dtype != torch.int32 or not slots.is_contiguous():

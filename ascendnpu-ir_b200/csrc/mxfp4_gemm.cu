@@ -922,10 +922,76 @@ int32_t launch_mx(const MxOperand &a, const MxOperand &b, int64_t k, MxParams p,
   return check_launch("matmul_mxfp4");
 }
 
+struct MxForm {
+  MxMode mode;
+  int rows, cols;        // of C in a tile
+  int split;             // CTAs that work on one
+  int64_t tiles;         // at most
+};
+MxForm choose_form(int64_t m, int64_t n, int64_t k, int64_t groups) {
+  // Which form: from the rows of a group, all of them or one and a half times the groups' mean, which most groups stay
+  // under (their sizes are on the device; a group that needs a second tile reads its weights twice.  128 groups of 16 rows
+  // on average, 4096 x 1536: 90 us in tiles of 16, 74 in tiles of 32; of 32 rows: 93 in tiles of 32, 78 in tiles of 64).
+  const int64_t rows = groups > 1 ? ceil_div(3 * m, 2 * groups) : m, stages = ceil_div(k, kStageK), chunks = ceil_div(stages, kChunk);
+  const int64_t sms = device_info().sm_count > 0 ? device_info().sm_count : 148;
+  auto tiles = [&](int64_t r, int64_t c) { return (groups > 1 ? m / r + groups : ceil_div(m, r)) * ceil_div(n, c); };   // at most
+  // K may be shared out over a cluster if every CTA gets a part and all clusters are at work at once (37 of four CTAs in
+  // two rounds: 13 us where one CTA a tile takes 8).
+  auto can_split = [&](auto at_once, int64_t nt, int s) { return nt * s <= sms && ceil_div(chunks, s) * (s - 1) < chunks && nt <= at_once(s); };
+  if (rows <= 32) {
+    // the more CTAs the better (1 row, N x K = 4096 x 4096: 6.7 us whole, 6.4 by two, 6.2 by four; 4096 x 14336: 15.4,
+    // 11.2, 9.6); kSingle takes 8.2 and 18 to 21 us there, and 10 to 13 us on 14336 x 4096, where this takes 8.7 to 9.9
+    int split = 1;
+    auto widest = [&](auto at_once, int64_t nt) {
+      for (int s = 8; s > 1 && split == 1; s /= 2)
+        if (can_split(at_once, nt, s)) split = s;
+      return nt;
+    };
+    const int64_t nt = rows <= 16 ? widest(clusters_at_once<16, kFew>, tiles(16, kTileM)) : widest(clusters_at_once<32, kFew>, tiles(32, kTileM));
+    return {kFew, rows <= 16 ? 16 : 32, kTileM, split, nt};
+  }
+  // Otherwise the least of these estimates, in units of 5 ns beside what every launch takes: rounds of tiles over the SMs x
+  // (stages x a stage's time + a tile's own), plus the join of a shared K, which grows with the rows of a tile.  Measured
+  // over 33 .. 4096 rows, N x K from 1000 x 8192 to 40000 x 1024.  Groups leave half of a last tile empty on average, and
+  // their last round is half full.
+  auto cost = [&](int64_t r, int64_t c, int64_t at_once, int64_t tile) {
+    if (groups == 1) return ceil_div(tiles(r, c), at_once) * tile;
+    const int64_t most = m < groups ? m : groups, mean = m / r + groups / 2 + 1;     // every group has a tile
+    return (mean < most ? most : mean) * ceil_div(n, c) * tile / at_once + tile / 2;
+  };
+  auto part = [&](int s) { return kChunk * ceil_div(chunks, s); };            // stages of a CTA
+  const int64_t r64 = rows < 64 ? rows : 64, r128 = rows < 128 ? rows : 128;
+  const int64_t tail = groups > 1 ? 128 : 0;              // rows next to another group's are stored by the warps
+  int64_t few = cost(64, kTileM, sms, 50 * stages + 5 * (r64 - 24)), single = cost(kTileM, 128, sms, 61 * stages + tail);
+  int few_split = 1, single_split = 1;
+  for (int s = 2; s <= 8; s *= 2) {
+    const int64_t f = s == 2 ? 51 * part(s) + 180 + 23 * r64 / 10 : 58 * part(s) + (s == 4 ? 370 : 470) + 24 * r64 / 10;
+    if (f < few && can_split(clusters_at_once<64, kFew>, tiles(64, kTileM), s)) { few = f; few_split = s; }
+    const int64_t g = s == 2 ? 57 * part(s) + 240 + 26 * r128 / 10 : 63 * part(s) + (s == 4 ? 350 : 450) + 41 * r128 / 10;
+    if (g < single && can_split(clusters_at_once<128, kSingle>, tiles(kTileM, 128), s)) { single = g; single_split = s; }
+  }
+  const int64_t pair = cost(256, 256, sms / 2, 69 * stages + 260 + tail);
+  if (few < single && few < pair) return {kFew, 64, kTileM, few_split, tiles(64, kTileM)};
+  if (single <= pair) return {kSingle, kTileM, 128, single_split, tiles(kTileM, 128)};
+  return {kPair, 256, 256, 2, tiles(256, 256)};
+}
+
 }  // namespace
 }  // namespace bsir
 
 using namespace bsir;
+
+extern "C" int32_t bsir_matmul_mxfp4_form(int64_t m, int64_t n, int64_t k, int64_t groups, int32_t *tile_rows, int32_t *tile_cols, int32_t *tile_ctas) {
+  clear_error();
+  constexpr int64_t kMax = int64_t{1} << 30;
+  if (m < 1 || n < 1 || k < 1 || m > kMax || n > kMax || k > kMax || m > (int64_t{1} << 40) / n || groups < 1 || groups > kMaxGroups)
+    return fail(BSIR_ERR_SHAPE, "matmul_mxfp4_form: m %lld, n %lld, k %lld (1 to 2^30, at most 2^40 results), %lld groups (1 to %d)", (long long)m,
+                (long long)n, (long long)k, (long long)groups, kMaxGroups);
+  if (!tile_rows || !tile_cols || !tile_ctas) return fail(BSIR_ERR_NULL, "matmul_mxfp4_form: null pointer");
+  const MxForm f = choose_form(m, n, k, groups);
+  *tile_rows = f.rows; *tile_cols = f.cols; *tile_ctas = f.split;
+  return BSIR_OK;
+}
 
 extern "C" int32_t bsir_matmul_mxfp4(const bsir_matmul_mxfp4_desc *d, void *stream) {
   clear_error();
@@ -982,53 +1048,10 @@ extern "C" int32_t bsir_matmul_mxfp4(const bsir_matmul_mxfp4_desc *d, void *stre
   if (!p.err) return fail(BSIR_ERR_WORKSPACE, "matmul_mxfp4: no device error word");
   cudaStream_t st = resolve_stream(stream);
   p.tma_out = aligned_to(d->out, 16) && (ldo * eb) % 16 == 0 && d->n * eb <= 0x7fffffff;     // its coordinates are 32-bit bytes
-  // Which form: from the rows of a group, all of them or one and a half times the groups' mean, which most groups stay
-  // under (their sizes are on the device; a group that needs a second tile reads its weights twice.  128 groups of 16 rows
-  // on average, 4096 x 1536: 90 us in tiles of 16, 74 in tiles of 32; of 32 rows: 93 in tiles of 32, 78 in tiles of 64).
-  const int64_t rows = groups > 1 ? ceil_div(3 * d->m, 2 * groups) : d->m, stages = p.k_blocks, chunks = ceil_div(stages, kChunk);
-  const int64_t sms = device_info().sm_count > 0 ? device_info().sm_count : 148;
-  auto tiles = [&](int64_t r, int64_t c) { return (groups > 1 ? d->m / r + groups : ceil_div(d->m, r)) * ceil_div(d->n, c); };   // at most
-  // K may be shared out over a cluster if every CTA gets a part and all clusters are at work at once (37 of four CTAs in
-  // two rounds: 13 us where one CTA a tile takes 8).
-  auto can_split = [&](auto at_once, int64_t nt, int s) { return nt * s <= sms && ceil_div(chunks, s) * (s - 1) < chunks && nt <= at_once(s); };
-  if (rows <= 32) {
-    // the more CTAs the better (1 row, N x K = 4096 x 4096: 6.7 us whole, 6.4 by two, 6.2 by four; 4096 x 14336: 15.4,
-    // 11.2, 9.6); kSingle takes 8.2 and 18 to 21 us there, and 10 to 13 us on 14336 x 4096, where this takes 8.7 to 9.9
-    int split = 1;
-    auto widest = [&](auto at_once, int64_t nt) {
-      for (int s = 8; s > 1 && split == 1; s /= 2)
-        if (can_split(at_once, nt, s)) split = s;
-      return nt;
-    };
-    if (rows <= 16) {
-      const int64_t nt = widest(clusters_at_once<16, kFew>, tiles(16, kTileM));
-      return launch_mx<16, kFew>(a, b, d->k, p, split, nt, st);
-    }
-    const int64_t nt = widest(clusters_at_once<32, kFew>, tiles(32, kTileM));
-    return launch_mx<32, kFew>(a, b, d->k, p, split, nt, st);
-  }
-  // Otherwise the least of these estimates, in units of 5 ns beside what every launch takes: rounds of tiles over the SMs x
-  // (stages x a stage's time + a tile's own), plus the join of a shared K, which grows with the rows of a tile.  Measured
-  // over 33 .. 4096 rows, N x K from 1000 x 8192 to 40000 x 1024.  Groups leave half of a last tile empty on average, and
-  // their last round is half full.
-  auto cost = [&](int64_t r, int64_t c, int64_t at_once, int64_t tile) {
-    if (groups == 1) return ceil_div(tiles(r, c), at_once) * tile;
-    const int64_t most = d->m < groups ? d->m : groups, mean = d->m / r + groups / 2 + 1;     // every group has a tile
-    return (mean < most ? most : mean) * ceil_div(d->n, c) * tile / at_once + tile / 2;
-  };
-  auto part = [&](int s) { return kChunk * ceil_div(chunks, s); };            // stages of a CTA
-  const int64_t r64 = rows < 64 ? rows : 64, r128 = rows < 128 ? rows : 128;
-  const int64_t tail = groups > 1 ? 128 : 0;              // rows next to another group's are stored by the warps
-  int64_t few = cost(64, kTileM, sms, 50 * stages + 5 * (r64 - 24)), single = cost(kTileM, 128, sms, 61 * stages + tail);
-  int few_split = 1, single_split = 1;
-  for (int s = 2; s <= 8; s *= 2) {
-    const int64_t f = s == 2 ? 51 * part(s) + 180 + 23 * r64 / 10 : 58 * part(s) + (s == 4 ? 370 : 470) + 24 * r64 / 10;
-    if (f < few && can_split(clusters_at_once<64, kFew>, tiles(64, kTileM), s)) { few = f; few_split = s; }
-    const int64_t g = s == 2 ? 57 * part(s) + 240 + 26 * r128 / 10 : 63 * part(s) + (s == 4 ? 350 : 450) + 41 * r128 / 10;
-    if (g < single && can_split(clusters_at_once<128, kSingle>, tiles(kTileM, 128), s)) { single = g; single_split = s; }
-  }
-  const int64_t pair = cost(256, 256, sms / 2, 69 * stages + 260 + tail);
-  if (few < single && few < pair) return launch_mx<64, kFew>(a, b, d->k, p, few_split, tiles(64, kTileM), st);
-  if (single <= pair) return launch_mx<128, kSingle>(a, b, d->k, p, single_split, tiles(128, 128), st);
-  return launch_mx<256, kPair>(a, b, d->k, p, 1, tiles(256, 256), st);
+  const MxForm f = choose_form(d->m, d->n, d->k, groups);
+  if (f.mode == kPair) return launch_mx<256, kPair>(a, b, d->k, p, 1, f.tiles, st);
+  if (f.mode == kSingle) return launch_mx<128, kSingle>(a, b, d->k, p, f.split, f.tiles, st);
+  if (f.rows == 64) return launch_mx<64, kFew>(a, b, d->k, p, f.split, f.tiles, st);
+  if (f.rows == 32) return launch_mx<32, kFew>(a, b, d->k, p, f.split, f.tiles, st);
+  return launch_mx<16, kFew>(a, b, d->k, p, f.split, f.tiles, st);
 }

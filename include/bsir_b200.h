@@ -559,6 +559,10 @@ typedef struct bsir_matmul_mxfp4_desc {
   int64_t ldo;
 } bsir_matmul_mxfp4_desc;
 BSIR_API int32_t bsir_matmul_mxfp4(const bsir_matmul_mxfp4_desc *desc, void *stream);
+/* Which form a product of these sizes takes on the current device: rows and columns of C in a tile (16, 32, 64 or 128 x 128,
+ * 256 x 256) and the CTAs that work on one (two on 256 x 256; otherwise those that share its K, as many as the device runs
+ * at once: results can differ in their last bits between devices that differ there).  groups: 1 without offsets. */
+BSIR_API int32_t bsir_matmul_mxfp4_form(int64_t m, int64_t n, int64_t k, int64_t groups, int32_t *tile_rows, int32_t *tile_cols, int32_t *tile_ctas);
 
 /* Tokens sorted by expert.  ids [tokens, top_k] (int32 or int64): the expert of each choice; a number outside
  * 0 .. experts - 1 names none (a padding token, an expert of another rank): such a choice is masked.

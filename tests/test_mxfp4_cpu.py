@@ -158,3 +158,23 @@ def test_quant_results_that_share_bytes_are_refused(L, kw):
 def test_quant_results_side_by_side_are_not(L, kw):
     _quant(L, **kw)
     assert b"overlap" not in L.bsir_last_error()
+
+
+@pytest.mark.parametrize("m,n,k,groups,form", [
+    (1, 4096, 4096, 1, (16, 128)), (17, 4096, 512, 1, (32, 128)), (40, 40000, 512, 1, (128, 128)), (40, 40000, 2100, 1, (64, 128)), (400, 1000, 512, 1, (128, 128)),
+    (1500, 3001, 2100, 1, (256, 256)), (2100, 5001, 2100, 1, (256, 256)), (4096, 4096, 4096, 1, (256, 256)),
+    (3800, 2500, 1100, 4, (256, 256)), (2500, 4100, 2100, 4, (256, 256)),
+    (600, 1200, 544, 60, (16, 128)), (900, 1300, 544, 48, (32, 128)), (1600, 1300, 544, 48, (64, 128)),
+])
+def test_product_form(L, m, n, k, groups, form):
+    """The rows and columns of a tile go by the sizes alone (the CTAs that share one by the device too)."""
+    import bsir
+    assert bsir.matmul_mxfp4_form(m, n, k, groups)[:2] == form
+
+
+def test_product_form_refusals(L):
+    import bsir
+    for bad in ((0, 1, 1, 1), (1, 0, 1, 1), (1, 1, 0, 1), ((1 << 30) + 1, 1, 1, 1), (1 << 30, 1 << 30, 1, 1), (1, 1, 1, 0), (1, 1, 1, 1025)):
+        with pytest.raises(bsir.BsirError):
+            bsir.matmul_mxfp4_form(*bad)
+    assert L.bsir_matmul_mxfp4_form(I(1), I(1), I(1), I(1), None, None, None) == -1
