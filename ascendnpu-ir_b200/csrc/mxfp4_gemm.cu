@@ -245,8 +245,8 @@ __device__ __forceinline__ void stage_half(uint8_t *row, int lane, int half, con
 }
 
 // An epilogue warp's 32 rows of C, 128 bytes a row at a time: staged in shared memory and sent by a TMA store; where
-// that cannot be (rows behind the group's end in the box, C's rows not 16-byte aligned) the warp stores them itself,
-// row by row.
+// that cannot be (rows behind the group's end in the box, C's rows not 16-byte aligned, a last piece of other than whole 16
+// bytes) the warp stores them itself, row by row.
 template <int BUFS> struct RowWriter {
   const MxParams &p;
   const CUtensorMap *tmap_out;
@@ -271,7 +271,9 @@ template <int BUFS> struct RowWriter {
   }
   __device__ __forceinline__ void send(int64_t col0, int cols) {     // `cols` of C from col0 on, at most 128 bytes
     uint8_t *buf = stage + nstores % BUFS * 4096;
-    if (by_tma) {
+    const int have = static_cast<int>(p.n - col0 < cols ? p.n - col0 : cols) * eb;    // bytes of a row
+    // (a TMA store writes whole 16-byte pieces, whatever the map's extent and type: up to 15 bytes behind C's last column)
+    if (by_tma && have % 16 == 0) {
       fence_proxy_async();
       __syncwarp();
       if (lane == 0) tma_store_2d(tmap_out, static_cast<int>(col0) * eb, row0, stage_addr + nstores % BUFS * 4096);
@@ -279,7 +281,6 @@ template <int BUFS> struct RowWriter {
       return;
     }
     __syncwarp();
-    const int have = static_cast<int>(p.n - col0 < cols ? p.n - col0 : cols) * eb;    // bytes of a row
     if (p.tma_out) {                                       // eight lanes a row, four rows at a time, sixteen in flight
       const int piece = lane & 7;
       if (have == 128) {
