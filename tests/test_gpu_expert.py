@@ -390,3 +390,22 @@ def test_first_calls_inside_a_capture(mode):
     root = os.path.dirname(os.path.dirname(os.path.abspath(bsir.__file__)))
     r = subprocess.run([sys.executable, "-c", FIRST_CALLS, root, mode], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "same" in r.stdout, r.stdout + r.stderr
+
+
+@pytest.mark.parametrize("tokens,top_k", [(20000, 4), (45000, 4)])
+def test_long_sorts_on_two_streams(B, tokens, top_k):
+    """Two clusters at work side by side; the longer sort's warps go over their choices twice."""
+    ids = [_ids(tokens, top_k, 64, s).cuda() for s in (3, 4)]
+    alone = [B.expert_sort(i, 64) for i in ids]
+    want = [R.sort(i.tolist(), 64) for i in ids]
+    streams = [torch.cuda.Stream() for _ in ids]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        got = []
+        for st, i in zip(streams, ids):
+            with torch.cuda.stream(st):
+                got.append(B.expert_sort(i, 64))
+        torch.cuda.synchronize()
+        for (o, s), (ao, as_), (wo, ws) in zip(got, alone, want):
+            assert torch.equal(o, ao) and torch.equal(s, as_)
+    assert np.array_equal(o.cpu().numpy(), wo) and np.array_equal(s.cpu().numpy(), ws)
