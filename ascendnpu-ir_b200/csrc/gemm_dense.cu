@@ -237,7 +237,9 @@ __device__ __forceinline__ void epilogue_tile(const GemmParams &p, const CUtenso
 #pragma unroll
         for (int j = 0; j < 16; ++j) packed[j] = pack_bf16x2(f[2 * j], f[2 * j + 1]);
       }
-      if (p.tma_out) {
+      // (a TMA store writes whole 16-byte pieces, whatever the map's extent and type: a last piece of other than a multiple
+      // of 8 columns would run over what lies behind it in wider rows)
+      if (p.tma_out && (full || (p.n & 7) == 0)) {
         const uint32_t b = nstores & 1u;
         // the store that read this buffer two chunks ago must have finished reading it
         if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");

@@ -263,3 +263,21 @@ def test_matmul_library_symbols(bsir):
         C.byref(mr(ai.t().contiguous())), C.byref(mr(bi)), C.byref(mr(c)))
     assert rc == 0
     assert_bits_equal(c, O.matmul(O.I8, to_bits(ai.t().contiguous()), to_bits(bi), O.F16, transpose_a=True), "int8 transposeA symbol")
+
+
+@pytest.mark.parametrize("dtype,out_dtype", [(torch.bfloat16, torch.bfloat16), (torch.float16, torch.float16), (torch.int8, torch.bfloat16),
+                                             (torch.bfloat16, torch.float32)])
+@pytest.mark.parametrize("batch,m,n,k", [(1, 256, 1001, 512), (1, 1500, 3004, 512), (1, 700, 1003, 1024), (3, 200, 513, 256), (1, 16, 1001, 2048)])
+def test_results_leave_what_lies_behind_their_columns(bsir, dtype, out_dtype, batch, m, n, k):
+    """Aligned rows of C in wider ones, n of other than whole 16-byte pieces: the last piece of a row ends inside one."""
+    g = torch.Generator(device="cuda").manual_seed(n)
+    mk = lambda *s: (torch.randint(-9, 10, s, device="cuda", generator=g) if dtype == torch.int8 else torch.randn(s, device="cuda", generator=g)).to(dtype)
+    a, b = mk(batch, m, k), mk(batch, n, k)
+    want = bsir.matmul(a, b, transpose_b=True, out_dtype=out_dtype)
+    whole = torch.full((batch, m + 1, (n + 47) // 16 * 16), 7.0, dtype=out_dtype, device="cuda")
+    if batch == 1:
+        bsir.matmul(a[0], b[0], transpose_b=True, out=whole[0, :m, 16:16 + n], out_dtype=out_dtype)
+    else:
+        bsir.matmul(a, b, transpose_b=True, out=whole[:, :m, 16:16 + n], out_dtype=out_dtype)
+    assert torch.equal(whole[:, :m, 16:16 + n], want)
+    assert (whole[:, m] == 7).all() and (whole[:, :, :16] == 7).all() and (whole[:, :, 16 + n:] == 7).all()
