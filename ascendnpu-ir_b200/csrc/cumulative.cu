@@ -134,7 +134,7 @@ __device__ __forceinline__ void cum_col_full_tile(uint32_t *col, typename CumAcc
 
 template <typename T, int KIND, bool NANP, int kCumColRows>
 __global__ void __launch_bounds__(32) cum_first_tma_kernel(const __grid_constant__ CUtensorMap tsrc, const __grid_constant__ CUtensorMap tdst,
-                                                           int64_t rows, int reverse, int depth, int *err) {
+                                                           T *dst, int64_t ds, int64_t rows, int64_t cols, int reverse, int depth, int *err) {
   using A = typename CumAcc<T>::type;
   constexpr int EPW = 4 / sizeof(T);                 // columns in a lane's word
   constexpr int kCumColTileBytes = kCumColRows * 128;
@@ -144,6 +144,10 @@ __global__ void __launch_bounds__(32) cum_first_tma_kernel(const __grid_constant
   const int lane = threadIdx.x;
   const int x0 = static_cast<int>(blockIdx.x) * 128;
   const int64_t ntiles = (rows + kCumColRows - 1) / kCumColRows;
+  // A TMA store writes whole 16-byte pieces, whatever the map's extent: where the row ends inside one the lanes store their
+  // columns themselves, or what lies behind them in wider rows would go.
+  const int64_t left_bytes = cols * static_cast<int64_t>(sizeof(T)) - x0;
+  const bool by_lanes = left_bytes < 128 && left_bytes % 16 != 0;
   if (lane == 0) {
     for (int b = 0; b < kCumColMaxDepth; ++b) mbar_init(smem_u32(&full[b]), 1);
     abort_flag = 0;
@@ -208,7 +212,17 @@ __global__ void __launch_bounds__(32) cum_first_tma_kernel(const __grid_constant
     }
     fence_proxy_async();                              // the lanes' writes, before the copy engine reads them
     __syncwarp();
-    if (lane == 0) {
+    if (by_lanes) {
+      T *out = dst + s * kCumColRows * ds + x0 / static_cast<int>(sizeof(T)) + lane * EPW;
+      const int have = static_cast<int>((left_bytes - lane * 4) / static_cast<int>(sizeof(T)));
+      for (int q = 0; q < nv; ++q, out += ds) {
+        T x[EPW];
+        memcpy(x, &col[q * 32], 4);
+#pragma unroll
+        for (int e = 0; e < EPW; ++e)
+          if (e < have) out[e] = x[e];
+      }
+    } else if (lane == 0) {
       asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(reinterpret_cast<uint64_t>(&tdst)),
                    "r"(x0), "r"(static_cast<int>(s * kCumColRows)), "r"(smem_u32(tiles + b * kCumColTileBytes))
                    : "memory");
@@ -450,10 +464,10 @@ void launch_cum(int axis, int reverse, int64_t rows, int64_t cols, const void *s
             make_byte_tmap(&tdst, dst, static_cast<uint64_t>(row_bytes), static_cast<uint64_t>(rows), static_cast<uint64_t>(ds) * sizeof(T), tile_rows, false)) {
           if (tile_rows == 128) {
             cudaFuncSetAttribute(cum_first_tma_kernel<T, KIND, NANP, 128>, cudaFuncAttributeMaxDynamicSharedMemorySize, kCumColMaxDepth * 64 * 128);
-            cum_first_tma_kernel<T, KIND, NANP, 128><<<static_cast<unsigned>(groups), 32, smem, st>>>(tsrc, tdst, rows, reverse, depth, device_error_word());
+            cum_first_tma_kernel<T, KIND, NANP, 128><<<static_cast<unsigned>(groups), 32, smem, st>>>(tsrc, tdst, d, ds, rows, cols, reverse, depth, device_error_word());
           } else {
             cudaFuncSetAttribute(cum_first_tma_kernel<T, KIND, NANP, 64>, cudaFuncAttributeMaxDynamicSharedMemorySize, kCumColMaxDepth * 64 * 128);
-            cum_first_tma_kernel<T, KIND, NANP, 64><<<static_cast<unsigned>(groups), 32, smem, st>>>(tsrc, tdst, rows, reverse, depth, device_error_word());
+            cum_first_tma_kernel<T, KIND, NANP, 64><<<static_cast<unsigned>(groups), 32, smem, st>>>(tsrc, tdst, d, ds, rows, cols, reverse, depth, device_error_word());
           }
           return;
         }

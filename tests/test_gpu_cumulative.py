@@ -114,3 +114,17 @@ def test_first_axis_scan_of_wide_problems(bsir, dtype, cols, kind):
     for reverse in (False, True):
         y = bsir.cumulative(kind, x, dim=0, reverse=reverse)
         assert_bits_equal(y, O.cumulative(kind, oracle_dtype(x), to_bits(x), axis=0, reverse=reverse), f"cum{kind} axis 0 {dtype} reverse {reverse}")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.int8, torch.int16])
+@pytest.mark.parametrize("rows,cols", [(300, 33), (700, 1001), (1025, 70), (400, 5)])
+@pytest.mark.parametrize("reverse", [False, True])
+def test_first_axis_scan_leaves_what_lies_behind_its_columns(bsir, dtype, rows, cols, reverse):
+    """Aligned rows in wider ones whose last column ends inside a 16-byte piece."""
+    pad = 16 // torch.empty(0, dtype=dtype).element_size()
+    whole = torch.full((rows + 1, (cols + pad) // pad * pad + 2 * pad), 7, device="cuda").to(dtype)
+    x = _data((rows, whole.shape[1]), dtype, rows + cols)[:, :cols]
+    bsir.cumulative("sum", x, dim=0, reverse=reverse, out=whole[:rows, pad:pad + cols])
+    want = O.cumulative("sum", oracle_dtype(x), to_bits(x.contiguous()), axis=0, reverse=reverse)
+    assert_bits_equal(whole[:rows, pad:pad + cols].contiguous(), want, f"cumsum {dtype} [{rows},{cols}]")
+    assert (whole[rows] == 7).all() and (whole[:, :pad] == 7).all() and (whole[:, pad + cols:] == 7).all()
