@@ -84,7 +84,9 @@ inline bool aligned_to(const void *p, size_t a) { return (reinterpret_cast<uintp
 // A kernel launched with launch_pdl may be scheduled before the kernel ahead of it in the stream has finished, if
 // that one called pdl_launch_dependents(); it must call pdl_wait() before its first access to global memory
 // (the wait returns when the kernel ahead has completed and its writes are visible).  Kernels ahead that never
-// call pdl_launch_dependents() serialise as usual.  BSIR_NO_PDL=1 launches plainly.
+// call pdl_launch_dependents() serialise as usual.  A kernel that allocates tensor memory calls it after the allocation:
+// one let in earlier could take what this one is still waiting for, and then wait for this one.  BSIR_NO_PDL=1 launches
+// plainly.
 __device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 

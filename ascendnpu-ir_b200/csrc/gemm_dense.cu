@@ -374,7 +374,6 @@ __global__ void __launch_bounds__(kThreads + 32, 1)
   const bool batched = p.batch > 1;
   const int total_tiles = tiles_per * (batched ? p.batch : 1);
 
-  pdl_launch_dependents();   // the set-up below overlaps the tail of the kernel ahead (see launch_pdl)
   if (threadIdx.x == 0) {
     for (int s = 0; s < Cfg::kStages; ++s) { mbar_init(full_bar(s), 1); mbar_init(empty_bar(s), kIssuers); }
     for (int a = 0; a < 2; ++a) { mbar_init(tfull_bar(a), kIssuers); mbar_init(tempty_bar(a), 4); }
@@ -384,7 +383,10 @@ __global__ void __launch_bounds__(kThreads + 32, 1)
     prefetch_tmap(&tmap_a);
     prefetch_tmap(&tmap_b);
   }
-  if (warp == 1) tmem_alloc(smem_u32(tmem_slot), Cfg::kTmemCols);
+  if (warp == 1) {
+    tmem_alloc(smem_u32(tmem_slot), Cfg::kTmemCols);
+    pdl_launch_dependents(); // the next kernel's set-up overlaps this one (launch_pdl)
+  }
   pdl_wait();                // no global memory is touched before this
   tc_fence_before();
   __syncthreads();
@@ -673,7 +675,6 @@ __global__ void __launch_bounds__(kDecThreads, 1)
   // Programmatic dependent launch: the next kernel of the stream may be scheduled while this one runs (its
   // blocks take SMs as ours leave them), and this kernel touches global memory only after the one before it
   // has completed -- so launch latency and the barrier / tensor-memory set-up overlap the predecessor's tail.
-  pdl_launch_dependents();
   if (warp == 0) {
     if (lane == 0) {
       prefetch_tmap(&tmap_w);
@@ -694,7 +695,10 @@ __global__ void __launch_bounds__(kDecThreads, 1)
       for (int it = 0; it < preissued; ++it) issue_next();
     TL(1);
   }
-  if (warp == 1) tmem_alloc(smem_u32(tmem_slot), tmem_cols);
+  if (warp == 1) {
+    tmem_alloc(smem_u32(tmem_slot), tmem_cols);
+    pdl_launch_dependents();
+  }
   if (warp != 0) pdl_wait();
   tc_fence_before();
   __syncthreads();

@@ -372,7 +372,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       tma_load_2d(dst + kTcWeightBytes + c * 2048, &tmap_a, (s * 4 + c) * 64, static_cast<int>(m0), wfull(slot));
   };
   const int preissued = nstages_total < nstages ? nstages_total : nstages;
-  pdl_launch_dependents();   // barrier set-up and the tensor-memory allocation overlap the kernel ahead (launch_pdl)
   if (warp == kTcDqWarps && lane == 0) {
     for (int s = 0; s < nstages; ++s) {
       mbar_init(wfull(s), 1);
@@ -387,7 +386,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     // the first ring of loads goes out before the CTA meets
     for (int s = 0; s < preissued; ++s) issue_stage(s);
   } else {
-    if (warp == kTcDqWarps + 1) tmem_alloc(smem_u32(tmem_slot), 512);
+    if (warp == kTcDqWarps + 1) {
+      tmem_alloc(smem_u32(tmem_slot), 512);
+      pdl_launch_dependents();   // the next kernel's set-up overlaps this one (launch_pdl)
+    }
     pdl_wait();              // global memory is read from here on
   }
   // scales and zero points of all groups of this CTA's columns, every load issued before the first store
@@ -676,7 +678,6 @@ __global__ void __launch_bounds__(kFoldThreads, 1)
   const int n0 = blockIdx.x * kFoldCols;
   const int rows = static_cast<int>(p.m - m0 < 16 ? p.m - m0 : 16);
 
-  pdl_launch_dependents();
   if (threadIdx.x == 0) {
     prefetch_tmap(&tmap_w);
     prefetch_tmap(&tmap_a);
@@ -686,7 +687,10 @@ __global__ void __launch_bounds__(kFoldThreads, 1)
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 1) tmem_alloc(smem_u32(tmem_slot), 128);
+  if (warp == 1) {
+    tmem_alloc(smem_u32(tmem_slot), 128);
+    pdl_launch_dependents();
+  }
   pdl_wait();
   tc_fence_before();
   __syncthreads();

@@ -558,7 +558,6 @@ __global__ void __launch_bounds__(MxCfg<BN, MODE>::kThreads, 1)
   const int team = PAIR ? 2 : p.split;
   const int rank = team > 1 ? static_cast<int>(cluster_rank()) : 0;
   const int first_tile = blockIdx.x / team, tile_step = gridDim.x / team;
-  pdl_launch_dependents();
   if (threadIdx.x == 0) {
     for (int s = 0; s < Cfg::kStages; ++s) { mbar_init(full_bar(s), 1); mbar_init(empty_bar(s), 1); }
     for (int s = 0; s < Cfg::kSfStages; ++s) {
@@ -578,6 +577,7 @@ __global__ void __launch_bounds__(MxCfg<BN, MODE>::kThreads, 1)
     } else {
       tmem_alloc(smem_u32(tmem_slot), Cfg::kTmemCols);
     }
+    pdl_launch_dependents();
   }
   pdl_wait();                       // no global memory is touched before this
   if (warp == 2) {                  // the groups' first rows (clamped to what exists) and tiles

@@ -130,3 +130,18 @@ def test_streamed_rows_stop_after_a_wait_that_gave_up(name):
     for line in re.findall(r".*\bissue\(k \+ .*", text):
         assert "ok &&" in line
     assert re.search(r"ring_last_parity\(|each buffer's last row", text)
+
+
+@pytest.mark.parametrize("name", ["mxfp4_gemm.cu", "gemm_dense.cu", "gemm_w4a16.cu"])
+def test_next_kernel_is_let_in_after_tensor_memory_is_allocated(name):
+    """One that is let in earlier may take the tensor memory that this one is still waiting for, and then wait for it."""
+    text = open(os.path.join(CSRC, name)).read()
+    kernels = re.split(r"\n__global__ ", text)[1:]
+    seen = 0
+    for body in kernels:
+        body = body.split("\n}\n", 1)[0]
+        alloc, let_in = re.search(r"tmem_alloc\(smem|tcgen05\.alloc", body), body.find("pdl_launch_dependents()")
+        if alloc and let_in >= 0:
+            seen += 1
+            assert alloc.start() < let_in
+    assert seen
