@@ -48,7 +48,7 @@ int *device_error_word();
 // shape.
 bool make_byte_tmap(::CUtensorMap_st *map, const void *ptr, uint64_t inner, uint64_t outer, uint64_t pitch, uint32_t box_rows,
                     bool swizzle = true);
-// The same without a swizzle, box_inner bytes (at most 256) x box_rows rows a box.
+// The same with a box of box_inner bytes (at most 256; 128 with the swizzle) x box_rows rows.
 bool make_byte_tmap2(::CUtensorMap_st *map, const void *ptr, uint64_t inner, uint64_t outer, uint64_t pitch, uint32_t box_inner, uint32_t box_rows,
                      bool swizzle);
 // The same over `batch` matrices `batch_stride` bytes apart (rank 3), with a box of box_inner bytes x box_rows rows of one.

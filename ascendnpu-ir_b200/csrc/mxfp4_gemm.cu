@@ -12,10 +12,10 @@
 // eight words into a lane's four rows, and the MMA issuer copies them to tensor memory with tcgen05.cp ahead of the
 // instructions that use them, in order and without a barrier between.
 //
-// What bounds it (B200, 4096 x 14336 x 4096): a stage of 256 x 256 tiles is 512 cycles of multiplication and takes about
-// 550, with the pair's 35 KB a CTA coming from L2 at 60 of the 64 bytes a cycle that reach an SM; the accumulator's way
-// out costs 1400 cycles a tile; sustained, the board's power limit lowers the clock to 1.5 GHz.  92 us when cool, 110
-// sustained (4.4 PFLOP/s).  Up to 32 rows the weights' way from HBM bounds it.
+// What bounds it (B200, 4096 x 14336 x 4096): one more tile a pair takes 6.6 us, of which 16 stages at 0.36 us (512 cycles
+// of multiplication each, 0.27) and 0.8 for the accumulator's way out; the tensor pipe is active 68 % of the launch, and 46
+// of the 64 bytes a cycle that reach an SM come from L2.  Sustained, the board's power limit lowers the clock to 1.5 GHz: 92 us
+// when cool, 113 sustained (4.3 PFLOP/s).  Up to 32 rows the weights' way from HBM bounds it.
 //
 // A persistent kernel, one CTA per SM, 256 threads (384 with one accumulator):
 //   warp 0            TMA producer of codes (a ring of stages of 256 elements of K) and exponents (a ring of 1024)
@@ -30,7 +30,8 @@
 //            are streamed for as few as 16 rows of A.
 // With few tiles a cluster of up to eight CTAs shares the K of a tile of kSingle or kFew, and has that tile only: each CTA
 // leaves its part in shared memory and adds its share of the rows from all of them, in their order (the same bits on every
-// run).  64 x 4096 x 14336: 11.4 us, 18.8 whole; 1 x 2048 x 8192: 6.3, 11 whole.  (Parts handed over by asynchronous
+// run of a device; how many share it goes by how many clusters the device runs at once).  64 x 4096 x 14336: 11.3 us, 18.8
+// whole; 1 x 2048 x 8192: 6.4, 11 whole.  (Parts handed over by asynchronous
 // stores straight from tensor memory cost 0.6 to 2 us more: eight bytes each, and more instructions to fetch.)
 #include "tc_ptx.cuh"
 
@@ -57,7 +58,7 @@ struct MxParams {
   int64_t ldo;
   int *err;
   int tma_out;                     // 1: C's rows start 16-byte aligned (TMA stores, 16-byte pieces)
-  int split;                       // kFew: CTAs that share a tile's K (a cluster)
+  int split;                       // CTAs that work on a tile: those that share its K (kFew, kSingle), two of kPair
 };
 
 template <int BN, int MODE>
