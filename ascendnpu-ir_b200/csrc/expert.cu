@@ -455,7 +455,7 @@ bool sixteen_at_once() {
           cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess ||
           cudaOccupancyMaxActiveClusters(&fits, kernel, &cfg) != cudaSuccess) {
         cudaGetLastError();
-        fits = 0;
+        return false;               // not remembered: the next call asks again
       }
       n = fits < n ? fits : n;
     }

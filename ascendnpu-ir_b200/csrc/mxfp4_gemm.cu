@@ -892,7 +892,7 @@ template <int BN, int MODE> int64_t clusters_at_once(int split) {
     cfg.numAttrs = 1;
     if (cudaOccupancyMaxActiveClusters(&n, mxfp4_gemm_kernel<BN, MODE>, &cfg) != cudaSuccess) {
       cudaGetLastError();
-      n = 0;
+      return 0;                    // not remembered: the next call asks again
     }
     slot.store(n + 1, std::memory_order_relaxed);
   }

@@ -362,6 +362,9 @@ x = torch.randn(96, 256, device="cuda", generator=g).bfloat16()
 w = torch.randn(4 * 64, 256, device="cuda", generator=g).bfloat16()
 ids = torch.randint(-1, 4, (96, 2), device="cuda", generator=g)
 wt = torch.rand(96, 2, device="cuda", generator=g)
+longer = torch.randn(16, 8192, device="cuda", generator=g).bfloat16()
+wide = torch.randn(2048, 8192, device="cuda", generator=g).bfloat16()
+many = torch.randint(-1, 60, (9000, 2), device="cuda", generator=g)        # the largest cluster
 
 def step():
     off, slots = B.expert_sort(ids, 4)
@@ -370,7 +373,8 @@ def step():
     cut = lambda t: t.as_strided((4, 64, t.shape[1]), (64 * t.stride(0), t.stride(0), 1))
     y = B.matmul_mxfp4(B.expert_dispatch(q, slots), B.expert_dispatch(s, slots), cut(qw), cut(sw), offsets=off)
     out = B.expert_combine(y, slots, wt)
-    return off, slots, B.dequant_mxfp4(qt, st), y, out, *B.expert_combine_grad(out, y, slots, wt)
+    few = B.matmul_mxfp4(*B.quant_mxfp4(longer), *B.quant_mxfp4(wide), out_dtype=torch.float32)     # a cluster shares K
+    return off, slots, B.dequant_mxfp4(qt, st), y, out, *B.expert_combine_grad(out, y, slots, wt), few, *B.expert_sort(many, 60)
 
 graph = torch.cuda.CUDAGraph()
 with torch.cuda.graph(graph, capture_error_mode=sys.argv[2]):
@@ -379,6 +383,7 @@ graph.replay()
 torch.cuda.synchronize()
 assert B.device_error() == 0
 assert all(torch.equal(a, b) for a, b in zip(got, step()))
+assert B.matmul_mxfp4_form(16, 2048, 8192)[2] > 1
 print("same")
 """
 
